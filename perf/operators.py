@@ -252,7 +252,8 @@ def prepare(case, seed):
             s["rope"] = kv8.Rope(d, theta, rotary_dim=case["rot"], interleaved=case["inter"],
                                  scaling=scaling)
         if case["op"] == "attention":
-            s["workspace"] = kv8.attention_workspace(len(rows), t, hq, hkv, d)
+            s["most"] = max(c for _, c in rows)
+            s["workspace"] = kv8.attention_workspace(len(rows), t, s["most"], hq, hkv, d)
     return s
 
 
@@ -395,7 +396,7 @@ def run(state):
                             first=s["first"], dtype=IN_TYPES[s["case"]["dtype"]])
         else:
             return kv8.attention(s["cache"], s["q"], s["cu"], s["lengths"], s["tables"],
-                                 out=s["out"], workspace=s["workspace"])
+                                 max_tokens=s["most"], out=s["out"], workspace=s["workspace"])
     elif op == "write":
         q = _plain_write(s)
     elif op == "read":
