@@ -78,6 +78,20 @@ class Sampled(C.Structure):
                 ("top_logprobs", C.c_double * 5)]
 
 
+class KV8(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_codes", C.c_void_p),
+                ("v_scales", C.c_void_p), ("blocks", C.c_uint64), ("kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32)]
+
+
+class Rope(C.Structure):
+    _fields_ = [("rotary_dim", C.c_uint32), ("interleaved", C.c_uint32), ("theta", C.c_double),
+                ("scaling", C.c_uint32), ("factor", C.c_double),
+                ("low_freq_factor", C.c_double), ("high_freq_factor", C.c_double),
+                ("beta_fast", C.c_double), ("beta_slow", C.c_double),
+                ("original_max_position", C.c_double), ("attention_factor", C.c_double)]
+
+
 _lib = None
 vp = C.c_void_p
 u32, u64, i32, f32 = C.c_uint32, C.c_uint64, C.c_int32, C.c_float
@@ -149,6 +163,15 @@ def lib():
                                          vp, vp]),
         "hllm_b200_sample": (C.c_int, [vp, u32, u64, u64, C.POINTER(Sampling), C.POINTER(u64),
                                        C.POINTER(Sampled), vp]),
+        "hllm_b200_rope_turns": (C.c_int, [C.POINTER(Rope), vp, C.POINTER(f32)]),
+        "hllm_b200_kv8_write": (C.c_int, [C.POINTER(KV8), vp, C.c_int, u64, u32, vp, vp, vp, vp,
+                                          f32, vp, u32, u32, f32, vp, vp, vp]),
+        "hllm_b200_kv8_read": (C.c_int, [C.POINTER(KV8), vp, u32, u32, vp, vp, vp, u64, C.c_int,
+                                         vp, vp, vp, vp]),
+        "hllm_b200_kv8_attention_workspace": (C.c_int, [u32, u64, u64, u32, u32, u32,
+                                                        C.POINTER(u64)]),
+        "hllm_b200_kv8_attention": (C.c_int, [C.POINTER(KV8), vp, u64, vp, vp, vp, u32, u64, u64,
+                                              u32, u32, f32, vp, u64, vp, u64, vp, vp]),
         "hllm_b200_synth_matrix": (C.c_int, [u64, u64, u64, u64, u64, f32, vp, vp]),
     }
     for name, (res, args) in sig.items():

@@ -1,0 +1,116 @@
+// kv8.cuh -- the 8-bit paged KV cache: host launchers of its write, its
+// read-back and its attention, and the number format they share.
+//
+// Format.  A (token, kv head) row of K or of V is d e4m3 codes and one scale
+// 2^e, e the least integer in [-24, 39] with max |x| <= 448 * 2^e, kept as the
+// byte e + 127.  Powers of two lose nothing that e4m3 has: a code's relative
+// rounding error is 2^-4 at most whatever the scale's mantissa, and code * 2^e
+// is exact in F32 (and in F16 where F16 has the range), so the attention can
+// put the scales into its scores' and weights' exponents without a rounding.
+// The clamp at -24 only coarsens rows below 448 * 2^-24 = 2.7e-5, whose steps
+// are then 2^-33, finer than the F16 cache's 2^-24; the clamp at 39 lets every
+// sum of 2^63 ratios stay in F32.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace hb {
+
+constexpr int kKv8Page = 16;     // tokens of a page, as in the F16 pool
+constexpr int kKv8MaxDim = 256;  // head sizes: multiples of 32 up to this
+constexpr int kKv8ExpMin = -24, kKv8ExpMax = 39;
+constexpr float kKv8Limit = 448.0f * 549755813888.0f;  // 448 * 2^39: larger values are stored as NaN
+
+// Codes [blocks][Hkv][16][d], scale bytes [blocks][Hkv][16].
+struct Kv8Cache {
+  uint8_t *k, *k_scale, *v, *v_scale;
+  long long blocks;
+  int hkv, dim;
+};
+
+// Element types of the write's input and the read's output (hllm_b200_dtype).
+enum Kv8Type : int { kKv8F32 = 0, kKv8F16 = 1, kKv8BF16 = 2 };
+
+struct Kv8WriteArgs {
+  Kv8Cache cache;
+  const void* qkv;           // [T][(Hq + 2 Hkv) d]
+  int type;                  // Kv8Type
+  int tokens, hq;
+  const int32_t* positions;  // [T]
+  const int32_t* slots;      // [T], -1: the token is not stored
+  const float *q_norm, *k_norm;  // [d] or null
+  float eps;
+  const double* turns;       // [rotary / 2] turns per position
+  int rotary, interleaved;
+  float factor;              // on cos and sin
+  __half* q_out;             // [T][Hq d]
+  uint32_t* status;
+};
+cudaError_t kv8_write_launch(const Kv8WriteArgs& a, cudaStream_t stream);
+
+struct Kv8ReadArgs {
+  Kv8Cache cache;
+  const int32_t* tables;   // [rows][max_blocks]
+  const int32_t* first;    // [rows] or null: 0
+  const int32_t* lengths;  // [rows] end positions
+  const int32_t* offsets;  // [rows + 1] output rows
+  int rows, max_blocks, tokens, type;
+  void *k_out, *v_out;     // [tokens][Hkv][d]
+  uint32_t* status;
+};
+cudaError_t kv8_read_launch(const Kv8ReadArgs& a, cudaStream_t stream);
+
+struct Kv8AttnArgs {
+  Kv8Cache cache;
+  const __half* q;            // [T][ld_q]
+  long long ld_q;
+  const int32_t* cu_seqlens;  // [rows + 1]
+  const int32_t* lengths;     // [rows] keys of a row, its new tokens included
+  const int32_t* tables;      // [rows][max_blocks]
+  int rows, tokens, max_row_tokens, hq, max_blocks;
+  float scale;
+  __half* out;                // [T][ld_out]
+  long long ld_out;
+  float* workspace;
+  uint32_t* status;
+  int sm_count;
+};
+size_t kv8_attention_workspace(int rows, int tokens, int max_row_tokens, int hq, int hkv, int dim,
+                               int sm_count);
+cudaError_t kv8_attention_launch(const Kv8AttnArgs& a, cudaStream_t stream);
+
+// ---------------------------------------------------------------- device side
+#ifdef __CUDACC__
+// The value of a scale byte.
+__device__ __forceinline__ float kv8_scale(uint32_t byte) {
+  return __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fc00000u : byte << 23);
+}
+// Two codes as F16: the low or the high half of a word of four.
+__device__ __forceinline__ uint32_t kv8_half2_lo(uint32_t w) {
+  uint32_t h;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}"
+      : "=r"(h)
+      : "r"(w));
+  return h;
+}
+__device__ __forceinline__ uint32_t kv8_half2_hi(uint32_t w) {
+  uint32_t h;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}"
+      : "=r"(h)
+      : "r"(w));
+  return h;
+}
+// Two values as codes (the first in the low byte), ties to even.
+__device__ __forceinline__ uint32_t kv8_codes(float lo, float hi) {
+  uint32_t w;
+  asm("{\n\t.reg .b16 c;\n\tcvt.rn.satfinite.e4m3x2.f32 c, %2, %1;\n\tcvt.u32.u16 %0, c;\n\t}"
+      : "=r"(w)
+      : "f"(lo), "f"(hi));
+  return w;
+}
+#endif
+
+}  // namespace hb

@@ -1,0 +1,673 @@
+// kv8_attention.cu -- attention over the 8-bit paged KV cache: the pass that
+// streams pages through registers (new tokens one or a few at a time), and the
+// join of what it split.
+//
+// o = sum_j softmax_j(scale q.k_j) v_j over the keys j <= the query's position.
+// With k_j = 2^ek_j c_j and v_j = 2^ev_j d_j (codes c, d) and s_j = scale
+// log2(e) 2^ek_j (q.c_j):
+//   l = sum 2^(s_j - m),   O = sum 2^(s_j + ev_j - m') d_j,   o = O / l * 2^(m' - m)
+// for any references m, m'.  The value scales are added to the weights'
+// exponents, so the weights that the tensor cores multiply (F16, rounded by
+// 2^-11) have their own reference m' and keep their precision whatever the
+// sizes of the value rows.  A reference is raised only when a score passes it
+// by 2^8: most pages rescale nothing.
+//
+// Work.  A row's new tokens and the query heads of one kv head form columns
+// (token, head), 8 NT of them a stream; a stream walks the row's pages.  The
+// batch's (row, stream, page) units in order are one sequence, cut evenly over
+// the CTAs of one wave and, within a CTA, over its warps, whatever the rows'
+// lengths.  Everything about the cut follows from the lengths on the device:
+// a captured launch serves any lengths.  What a cut leaves of a stream is
+// joined first in the CTA (shared memory), then, where a stream spans CTAs, by
+// a second small launch, in order: results do not depend on timing.
+//
+// Per page a warp computes S^T = K Q^T and O^T = V^T P^T with m16n8k16 F16
+// products: the 16 keys, then 16 value dimensions, are the M side, so that the
+// columns are the 8-wide N side and one decode row wastes half of a tile, not
+// three quarters.  Codes go from global memory straight into the registers of
+// the fragments: the order of the products' inner dimension is free, so a lane
+// takes 16 consecutive bytes of a key for four steps of QK, and for PV the
+// bytes of four keys, paired by byte permutes.  No shared memory, no barrier,
+// no transpose is in the stream; the next page's loads are in flight while one
+// is multiplied.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "kv8.cuh"
+
+namespace hb {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoReference = -1e30f;  // below every finite score
+constexpr float kLazy = 8.f;            // log2 of the growth that moves a reference
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+      "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t o;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(o) : "r"(v));
+  return o;
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Words (4 codes) a lane holds of one key row, and of one value row.
+template <int W>
+__device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint8_t* p) {
+  if constexpr (W == 4) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
+  } else if constexpr (W == 2) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  }
+}
+
+template <int D>
+struct Shape {
+  // K: four lanes share a key row, KW words each, KS steps.  V: eight lanes
+  // share a value row, VW words each, VS steps.
+  static constexpr int KW = D % 64 == 0 ? 4 : 2, KS = D / (16 * KW);
+  static constexpr int VW = D % 128 == 0 ? 4 : D % 64 == 0 ? 2 : 1, VS = D / (32 * VW);
+};
+
+// One page in registers.
+template <int D>
+struct Page {
+  using S = Shape<D>;
+  uint32_t k[S::KS][2][S::KW];  // key rows g and g + 8
+  uint32_t v[S::VS][4][S::VW];  // value rows 2t, 2t + 1, 2t + 8, 2t + 9
+  uint32_t ks[2], vs[2];        // scale bytes of rows g and g + 8
+};
+
+// A row's place in the packed batch and its streams.
+struct RowInfo {
+  int count, len, t0;  // new tokens, keys, first packed token
+  int pages;           // at least 1, so that a row without keys is answered too
+  int chunks;          // streams per kv head
+};
+
+// Rows that this pass does not answer have count 0: rows out of the batch's
+// bounds (reported) and rows long enough for the tile pass.
+__device__ __forceinline__ RowInfo row_info(const Kv8AttnArgs& a, int r, int group, int cols,
+                                            int tile_from, bool report) {
+  RowInfo x;
+  x.t0 = __ldg(a.cu_seqlens + r);
+  const int end = __ldg(a.cu_seqlens + r + 1);
+  x.len = __ldg(a.lengths + r);
+  x.count = end - x.t0;
+  const bool bad = x.t0 < 0 || x.count < 0 || end > a.tokens || x.count > a.max_row_tokens ||
+                   x.len < 0 || x.len > a.max_blocks * static_cast<long long>(kKv8Page);
+  if (bad && report) atomicOr(a.status, kDevBadIndex);
+  if (bad || x.count * static_cast<long long>(group) >= tile_from) x.count = 0;
+  x.pages = max(1, static_cast<int>((static_cast<long long>(x.len) + kKv8Page - 1) / kKv8Page));
+  x.chunks = static_cast<int>((static_cast<long long>(x.count) * group + cols - 1) / cols);
+  return x;
+}
+__device__ __forceinline__ long long row_units(const RowInfo& x, int hkv) {
+  return static_cast<long long>(x.chunks) * hkv * x.pages;
+}
+
+struct Cut {
+  int ctas;         // CTAs with work
+  long long total;  // units
+};
+__device__ __forceinline__ long long cut_begin(const Cut& c, long long i) {
+  return c.total * i / c.ctas;
+}
+__device__ __forceinline__ int cut_owner(const Cut& c, long long unit) {
+  return static_cast<int>(((unit + 1) * c.ctas - 1) / c.total);
+}
+
+// The workspace: per CTA a record and two pieces (the stream it continues, the
+// stream it leaves open), a piece being cols x D sums and cols x (m, m', l).
+struct Record {
+  int row, stream, first;  // first: the CTA that holds the stream's first unit; -1: nothing to join
+  int pad;
+};
+__host__ __device__ constexpr size_t piece_floats(int dim, int cols) {
+  return static_cast<size_t>(cols) * (dim + 4);
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, 1)
+    kv8_stream_kernel(const Kv8AttnArgs a, int group, int tile_from) {
+  using S = Shape<D>;
+  constexpr int kCols = 8 * NT;
+  constexpr int kPiece = kCols * (D + 4);
+  extern __shared__ __align__(16) float pieces[];  // [kWarps][2][kPiece]
+  __shared__ int piece_row[kWarps][2], piece_stream[kWarps][2];
+  __shared__ bool piece_starts[kWarps][2], piece_ends[kWarps][2];
+  __shared__ long long units_before;  // units before the row of the CTA's first one
+  griddep_enter();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, tq = lane & 3;
+  const int hkv = a.cache.hkv;
+
+  // All units, and the row of this warp's first one.
+  Cut cut{};
+  long long mine[4];
+  for (int base = 0; base < a.rows; base += 128) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = base + 32 * k + lane;
+      mine[k] = r < a.rows ? row_units(row_info(a, r, group, kCols, tile_from,
+                                                blockIdx.x == 0 && warp == 0), hkv)
+                           : 0;
+    }
+    long long n = mine[0] + mine[1] + mine[2] + mine[3];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    cut.total += n;
+  }
+  // A CTA takes kWarps pages at least, where there are so many.
+  cut.ctas = static_cast<int>(
+      min(static_cast<long long>(gridDim.x), max(1LL, (cut.total + kWarps - 1) / kWarps)));
+  Record* records = reinterpret_cast<Record*>(a.workspace);
+  if (cut.total == 0 || static_cast<int>(blockIdx.x) >= cut.ctas) {
+    if (threadIdx.x == 0) records[blockIdx.x].first = -1;
+    return;
+  }
+  const long long c0 = cut_begin(cut, blockIdx.x), c1 = cut_begin(cut, blockIdx.x + 1);
+  const long long w0 = c0 + (c1 - c0) * warp / kWarps, w1 = c0 + (c1 - c0) * (warp + 1) / kWarps;
+  int n = static_cast<int>(w1 - w0);
+  if (threadIdx.x < kWarps * 2) piece_row[threadIdx.x >> 1][threadIdx.x & 1] = -1;
+  __syncthreads();
+
+  if (n > 0) {
+    int row = -1;
+    long long before = 0;  // units before the row
+    for (int base = 0; base < a.rows && row < 0; base += 128) {
+      if (a.rows > 128) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = base + 32 * k + lane;
+          mine[k] =
+              r < a.rows ? row_units(row_info(a, r, group, kCols, tile_from, false), hkv) : 0;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        long long incl = mine[k];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, before + incl > w0);
+        if (row < 0) {
+          if (hit) {
+            const int src = __ffs(hit) - 1;
+            row = base + 32 * k + src;
+            before += __shfl_sync(0xffffffffu, incl - mine[k], src);
+          } else {
+            before += __shfl_sync(0xffffffffu, incl, 31);
+          }
+        }
+      }
+    }
+    if (w0 == c0 && lane == 0) units_before = before;
+    RowInfo x = row_info(a, row, group, kCols, tile_from, false);
+    int stream = static_cast<int>((w0 - before) / x.pages);
+    int q = static_cast<int>((w0 - before) % x.pages);
+    const float sl2 = a.scale * kLog2e;
+
+    // The loader runs one unit ahead of the arithmetic.
+    int lrow = row, lstream = stream, lq = q;
+    RowInfo lx = x;
+    int tab_row = -1, tab_q0 = 0, tab = -1;  // 32 entries of the block table, one a lane
+    auto advance = [&](int& r, RowInfo& xi, int& st, int& page) {
+      if (++page < xi.pages) return;
+      page = 0;
+      if (++st < xi.chunks * hkv) return;
+      st = 0;
+      while (++r < a.rows) {
+        xi = row_info(a, r, group, kCols, tile_from, false);
+        if (xi.chunks) return;
+      }
+    };
+    Page<D> pg[2];
+    bool have[2];
+    auto fetch = [&](Page<D>& p, bool& ok) {
+      if (lrow != tab_row || lq < tab_q0 || lq >= tab_q0 + 32) {
+        tab_row = lrow;
+        tab_q0 = lq;
+        const int i = lq + lane;
+        tab = i < lx.pages && i < a.max_blocks
+                  ? __ldg(a.tables + static_cast<size_t>(lrow) * a.max_blocks + i)
+                  : -1;
+      }
+      const int b = __shfl_sync(0xffffffffu, tab, lq - tab_q0);
+      const int valid = lx.len - lq * kKv8Page;  // keys of the page
+      ok = valid > 0 && b >= 0 && b < a.cache.blocks;
+      if (valid > 0 && !ok && lane == 0) atomicOr(a.status, kDevBadIndex);
+      const int kvh = lstream / lx.chunks;
+      const size_t at = (static_cast<size_t>(ok ? b : 0) * hkv + kvh) * kKv8Page;
+      const uint8_t* kp = a.cache.k + at * D;
+      const uint8_t* vp = a.cache.v + at * D;
+      // Rows past the last key may hold anything: they are not read.
+      const bool r0 = ok && g < valid, r1 = ok && g + 8 < valid;
+#pragma unroll
+      for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int w = 0; w < S::KW; ++w) p.k[s][h][w] = 0u;
+          if (h ? r1 : r0)
+            load_words<S::KW>(p.k[s][h], kp + (g + 8 * h) * D + (s * 4 + tq) * S::KW * 4);
+        }
+      p.ks[0] = r0 ? __ldg(a.cache.k_scale + at + g) : 127u;
+      p.ks[1] = r1 ? __ldg(a.cache.k_scale + at + g + 8) : 127u;
+      p.vs[0] = r0 ? __ldg(a.cache.v_scale + at + g) : 127u;
+      p.vs[1] = r1 ? __ldg(a.cache.v_scale + at + g + 8) : 127u;
+#pragma unroll
+      for (int s = 0; s < S::VS; ++s)
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int key = 2 * tq + (h & 1) + (h >> 1) * 8;
+#pragma unroll
+          for (int w = 0; w < S::VW; ++w) p.v[s][h][w] = 0u;
+          if (ok && key < valid)
+            load_words<S::VW>(p.v[s][h], vp + key * D + (s * 8 + g) * S::VW * 4);
+        }
+      advance(lrow, lx, lstream, lq);
+    };
+
+    uint32_t qb[NT][D / 16][2];
+    float o[NT][D / 16][4];
+    float m[NT][2], mo[NT][2], l[NT][2];
+    int lim[NT][2];  // last key that columns 2t, 2t + 1 see; -1: none
+
+    auto open = [&]() {
+      const int kvh = stream / x.chunks, x0 = (stream % x.chunks) * kCols;
+      const int cols = x.count * group;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int c = x0 + nt * 8 + g;
+        const bool live = c < cols;
+        const __half* src = a.q + static_cast<size_t>(x.t0 + (live ? c / group : 0)) * a.ld_q +
+                            static_cast<size_t>(kvh * group + (live ? c % group : 0)) * D;
+#pragma unroll
+        for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+          for (int w = 0; w < S::KW; ++w) {
+            const uint2 v =
+                live ? __ldg(reinterpret_cast<const uint2*>(src + ((s * 4 + tq) * S::KW + w) * 4))
+                     : make_uint2(0u, 0u);
+            qb[nt][s * S::KW + w][0] = v.x;
+            qb[nt][s * S::KW + w][1] = v.y;
+          }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int cc = x0 + nt * 8 + 2 * tq + e;
+          lim[nt][e] = cc < cols ? max(-1, x.len - x.count + cc / group) : -1;
+          m[nt][e] = mo[nt][e] = kNoReference;
+          l[nt][e] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+      }
+    };
+
+    auto multiply = [&](const Page<D>& p, bool ok) {
+      float s[NT][2][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][0][e] = s[nt][1][e] = 0.f;
+#pragma unroll
+      for (int st = 0; st < S::KS; ++st)
+#pragma unroll
+        for (int w = 0; w < S::KW; ++w) {
+          const int i = st * S::KW + w;
+          const uint32_t a0 = kv8_half2_lo(p.k[st][0][w]), a2 = kv8_half2_hi(p.k[st][0][w]);
+          const uint32_t a1 = kv8_half2_lo(p.k[st][1][w]), a3 = kv8_half2_hi(p.k[st][1][w]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma16816(s[nt][i & 1], a0, a1, a2, a3, qb[nt][i][0], qb[nt][i][1]);
+        }
+      const int key = q * kKv8Page + g;
+      const float ks0 = kv8_scale(p.ks[0]) * sl2, ks1 = kv8_scale(p.ks[1]) * sl2;
+      const float ev0 = static_cast<float>(static_cast<int>(p.vs[0]) - 127);
+      const float ev1 = static_cast<float>(static_cast<int>(p.vs[1]) - 127);
+      bool grown = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool seen = ok && key + (e >> 1) * 8 <= lim[nt][e & 1];
+          const float v = (s[nt][0][e] + s[nt][1][e]) * (e >> 1 ? ks1 : ks0);
+          s[nt][0][e] = seen ? v : -INFINITY;
+          s[nt][1][e] = s[nt][0][e] + (e >> 1 ? ev1 : ev0);
+          grown |= s[nt][0][e] > m[nt][e & 1] + kLazy || s[nt][1][e] > mo[nt][e & 1] + kLazy;
+        }
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float a0 = fmaxf(s[nt][0][e], s[nt][0][e + 2]), a1 = fmaxf(s[nt][1][e], s[nt][1][e + 2]);
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+              a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, off));
+              a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, off));
+            }
+            const float m1 = fmaxf(m[nt][e], a0), mo1 = fmaxf(mo[nt][e], a1);
+            l[nt][e] *= ex2(m[nt][e] - m1);
+            const float f = ex2(mo[nt][e] - mo1);
+            m[nt][e] = m1;
+            mo[nt][e] = mo1;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              o[nt][i][e] *= f;
+              o[nt][i][e + 2] *= f;
+            }
+          }
+      }
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float p2[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          l[nt][e & 1] += ex2(s[nt][0][e] - m[nt][e & 1]);
+          p2[e] = ex2(s[nt][1][e] - mo[nt][e & 1]);
+        }
+        pb[nt][0] = transpose8x8(half2_bits(p2[0], p2[1]));
+        pb[nt][1] = transpose8x8(half2_bits(p2[2], p2[3]));
+      }
+#pragma unroll
+      for (int st = 0; st < S::VS; ++st)
+#pragma unroll
+        for (int w = 0; w < S::VW; ++w)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t sel = h ? 0x7362u : 0x5140u;
+            const uint32_t lo = __byte_perm(p.v[st][0][w], p.v[st][1][w], sel);
+            const uint32_t hi = __byte_perm(p.v[st][2][w], p.v[st][3][w], sel);
+            const uint32_t a0 = kv8_half2_lo(lo), a1 = kv8_half2_hi(lo);
+            const uint32_t a2 = kv8_half2_lo(hi), a3 = kv8_half2_hi(hi);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(o[nt][(st * S::VW + w) * 2 + h], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+          }
+    };
+
+    // Value dimension of this lane's sums o[nt][i][e]: rows g and g + 8 of
+    // product i hold consecutive dimensions.
+    auto dim_of = [&](int i) {
+      const int st = i / (2 * S::VW), rest = i % (2 * S::VW);
+      return (st * 8 + g) * S::VW * 4 + rest * 2;
+    };
+
+    bool starts = q == 0;
+    auto close = [&](bool ends) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1)
+            l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
+      if (starts && ends) {
+        const int kvh = stream / x.chunks, x0 = (stream % x.chunks) * kCols;
+        const int cols = x.count * group;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int c = x0 + nt * 8 + 2 * tq + e;
+            if (c < cols) {
+              const float f = lim[nt][e] < 0 ? 0.f : ex2(mo[nt][e] - m[nt][e]) / l[nt][e];
+              __half* dst = a.out + static_cast<size_t>(x.t0 + c / group) * a.ld_out +
+                            static_cast<size_t>(kvh * group + c % group) * D;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i)
+                *reinterpret_cast<__half2*>(dst + dim_of(i)) =
+                    __floats2half2_rn(o[nt][i][e] * f, o[nt][i][e + 2] * f);
+            }
+          }
+        return;
+      }
+      const int which = starts ? 1 : 0;
+      float* piece = pieces + (warp * 2 + which) * kPiece;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = nt * 8 + 2 * tq + e;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+            *reinterpret_cast<float2*>(piece + c * D + dim_of(i)) =
+                make_float2(o[nt][i][e], o[nt][i][e + 2]);
+          if (g == 0) {
+            float* ml = piece + kCols * D + c * 4;
+            ml[0] = m[nt][e];
+            ml[1] = mo[nt][e];
+            ml[2] = l[nt][e];
+          }
+        }
+      if (lane == 0) {
+        piece_row[warp][which] = row;
+        piece_stream[warp][which] = stream;
+        piece_starts[warp][which] = starts;
+        piece_ends[warp][which] = ends;
+      }
+    };
+
+    fetch(pg[0], have[0]);
+    open();
+#pragma unroll 1
+    for (int i = 0; i < n; i += 2) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        if (i + b < n) {
+          if (i + b + 1 < n) fetch(pg[b ^ 1], have[b ^ 1]);
+          multiply(pg[b], have[b]);
+          const bool ends = q == x.pages - 1;
+          if (ends || i + b + 1 == n) close(ends);
+          if (i + b + 1 < n) {
+            advance(row, x, stream, q);
+            if (q == 0) {
+              starts = true;
+              open();
+            }
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  // Join the warps' pieces: a chain is a run of pieces of one stream.
+  Record rec{0, 0, -1, 0};
+  auto next_piece = [&](int from) {
+    while (from < kWarps * 2 && piece_row[from >> 1][from & 1] < 0) ++from;
+    return from;
+  };
+  int i = next_piece(0);
+  while (i < kWarps * 2) {
+    const int row = piece_row[i >> 1][i & 1], stream = piece_stream[i >> 1][i & 1];
+    int last = i, j = next_piece(i + 1);
+    while (j < kWarps * 2 && piece_row[j >> 1][j & 1] == row && piece_stream[j >> 1][j & 1] == stream) {
+      last = j;
+      j = next_piece(j + 1);
+    }
+    const bool begins = piece_starts[i >> 1][i & 1], ends = piece_ends[last >> 1][last & 1];
+    const RowInfo x = row_info(a, row, group, kCols, tile_from, false);
+    const int kvh = stream / x.chunks, x0 = (stream % x.chunks) * kCols;
+    float* dst = a.workspace + gridDim.x * 4 +
+                 (static_cast<size_t>(blockIdx.x) * 2 + (begins ? 1 : 0)) * kPiece;
+    for (int u = threadIdx.x; u < kCols * D / 4; u += kWarps * 32) {
+      const int c = u / (D / 4), dd = (u % (D / 4)) * 4;
+      float M = kNoReference, MO = kNoReference;
+      for (int k = i; k <= last; ++k)
+        if (piece_row[k >> 1][k & 1] >= 0) {
+          M = fmaxf(M, pieces[k * kPiece + kCols * D + c * 4]);
+          MO = fmaxf(MO, pieces[k * kPiece + kCols * D + c * 4 + 1]);
+        }
+      float L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = i; k <= last; ++k)
+        if (piece_row[k >> 1][k & 1] >= 0) {
+          const float* ml = pieces + k * kPiece + kCols * D + c * 4;
+          L += ml[2] * ex2(ml[0] - M);
+          const float f = ex2(ml[1] - MO);
+          const float4 v = *reinterpret_cast<const float4*>(pieces + k * kPiece + c * D + dd);
+          acc.x += v.x * f;
+          acc.y += v.y * f;
+          acc.z += v.z * f;
+          acc.w += v.w * f;
+        }
+      if (begins && ends) {
+        const int col = x0 + c;
+        if (col < x.count * group) {
+          const float f = x.len - x.count + col / group < 0 ? 0.f : ex2(MO - M) / L;
+          __half* out = a.out + static_cast<size_t>(x.t0 + col / group) * a.ld_out +
+                        static_cast<size_t>(kvh * group + col % group) * D + dd;
+          *reinterpret_cast<uint2*>(out) =
+              make_uint2(half2_bits(acc.x * f, acc.y * f), half2_bits(acc.z * f, acc.w * f));
+        }
+      } else {
+        *reinterpret_cast<float4*>(dst + c * D + dd) = acc;
+        if (dd == 0) *reinterpret_cast<float4*>(dst + kCols * D + c * 4) = make_float4(M, MO, L, 0.f);
+      }
+    }
+    if (!begins && ends) {
+      // The stream that earlier CTAs began ends here: the join pass takes it.
+      // It is the CTA's first chain, so its row is the CTA's first.
+      rec.row = row;
+      rec.stream = stream;
+      rec.first = cut_owner(cut, units_before + static_cast<long long>(stream) * x.pages);
+    }
+    i = j;
+  }
+  if (threadIdx.x == 0) records[blockIdx.x] = rec;
+}
+
+// Joins the pieces of a stream that spans CTAs, in order; one CTA for each CTA
+// of the stream pass, with work where that one ended such a stream.
+template <int D, int NT>
+__global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a, int group, int tile_from) {
+  constexpr int kCols = 8 * NT;
+  constexpr int kPiece = kCols * (D + 4);
+  griddep_enter();
+  const Record rec = reinterpret_cast<const Record*>(a.workspace)[blockIdx.x];
+  const int first = rec.first, end = blockIdx.x;
+  if (first < 0 || first >= end) return;
+  const RowInfo x = row_info(a, rec.row, group, kCols, tile_from, false);
+  if (x.chunks == 0) return;
+  const int kvh = rec.stream / x.chunks, x0 = (rec.stream % x.chunks) * kCols;
+  const float* base = a.workspace + gridDim.x * 4;
+  // Piece of CTA c: the one it left open for the first, else the one it continued.
+  auto piece = [&](int c) { return base + (static_cast<size_t>(c) * 2 + (c == first ? 1 : 0)) * kPiece; };
+  for (int u = threadIdx.x; u < kCols * D / 4; u += 256) {
+    const int c = u / (D / 4), dd = (u % (D / 4)) * 4;
+    const int col = x0 + c;
+    if (col >= x.count * group) continue;
+    float M = kNoReference, MO = kNoReference;
+    for (int k = first; k <= end; ++k) {
+      const float4 ml = __ldcg(reinterpret_cast<const float4*>(piece(k) + kCols * D + c * 4));
+      M = fmaxf(M, ml.x);
+      MO = fmaxf(MO, ml.y);
+    }
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = first; k <= end; ++k) {
+      const float4 ml = __ldcg(reinterpret_cast<const float4*>(piece(k) + kCols * D + c * 4));
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(k) + c * D + dd));
+      L += ml.z * ex2(ml.x - M);
+      const float f = ex2(ml.y - MO);
+      acc.x += v.x * f;
+      acc.y += v.y * f;
+      acc.z += v.z * f;
+      acc.w += v.w * f;
+    }
+    const float f = x.len - x.count + col / group < 0 ? 0.f : ex2(MO - M) / L;
+    __half* out = a.out + static_cast<size_t>(x.t0 + col / group) * a.ld_out +
+                  static_cast<size_t>(kvh * group + col % group) * D + dd;
+    *reinterpret_cast<uint2*>(out) =
+        make_uint2(half2_bits(acc.x * f, acc.y * f), half2_bits(acc.z * f, acc.w * f));
+  }
+}
+
+int stream_ctas(int sm_count) { return sm_count; }
+
+template <int D, int NT>
+cudaError_t launch_stream(const Kv8AttnArgs& a, int tile_from, cudaStream_t stream) {
+  constexpr size_t smem = static_cast<size_t>(kWarps) * 2 * 8 * NT * (D + 4) * sizeof(float);
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !configured[dev]) {
+    e = cudaFuncSetAttribute(kv8_stream_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    if (dev < 64) configured[dev] = true;
+  }
+  const int group = a.hq / a.cache.hkv;
+  const int ctas = stream_ctas(a.sm_count);
+  e = launch_dependent(kv8_stream_kernel<D, NT>, dim3(ctas), dim3(kWarps * 32), smem, stream, a,
+                       group, tile_from);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(kv8_join_kernel<D, NT>, dim3(ctas), dim3(256), 0, stream, a, group,
+                          tile_from);
+}
+
+}  // namespace
+
+size_t kv8_attention_workspace(int, int, int, int, int, int dim, int sm_count) {
+  return static_cast<size_t>(stream_ctas(sm_count)) * (4 + 2 * piece_floats(dim, 16)) * sizeof(float);
+}
+
+cudaError_t kv8_attention_launch(const Kv8AttnArgs& a, cudaStream_t stream) {
+  if (a.rows == 0 || a.tokens == 0) return cudaSuccess;
+  const int tile_from = 0x7fffffff;
+  const int group = a.hq / a.cache.hkv;
+  const bool wide = group > 8 || a.max_row_tokens > 1;
+  switch (a.cache.dim) {
+#define HB_KV8_DIM(D)                                                   \
+  case D:                                                               \
+    return wide && D <= 128 ? launch_stream<D, D <= 128 ? 2 : 1>(a, tile_from, stream) \
+                            : launch_stream<D, 1>(a, tile_from, stream);
+    HB_KV8_DIM(32)
+    HB_KV8_DIM(64)
+    HB_KV8_DIM(96)
+    HB_KV8_DIM(128)
+    HB_KV8_DIM(160)
+    HB_KV8_DIM(192)
+    HB_KV8_DIM(224)
+    HB_KV8_DIM(256)
+#undef HB_KV8_DIM
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace hb

@@ -441,6 +441,110 @@ hllm_b200_status hllm_b200_sample(const float* logits, uint32_t rows, uint64_t v
                                   const uint64_t* generated_index, hllm_b200_sampled* out,
                                   void* stream);
 
+/* ---------------------------------------------------- 8-bit paged KV cache
+ * A KV cache of half the bytes, beside the F16 pages above (no counterpart in
+ * the reference, whose cache is F16/F32).  Pages are 16 tokens, block tables
+ * and slots as the packer makes them.  A (token, kv head) row of K or of V is
+ * head_dim e4m3 codes and one scale 2^e, kept as the byte e + 127:
+ *   e = the least integer in [-24, 39] with max |x| <= 448 * 2^e,
+ *   code_i = e4m3(x_i * 2^-e), ties to even; value_i = code_i * 2^e.
+ * The maximum is over finite values of at most 448 * 2^39 in size; any other
+ * value is stored as NaN.  head_dim is a multiple of 32, at most 256.
+ * The arrays are 16-byte aligned.  All calls below are asynchronous, allocate
+ * nothing, keep nothing between calls and run on the current device, whose
+ * memory every pointer names; they can be captured into a graph, and a
+ * captured call serves any positions, slots, lengths and tables within the
+ * counts it was captured with.  Calls on several streams may overlap where
+ * they share no buffer that one of them writes (the workspace is one).
+ * `status` (device u32) receives error bits, as hllm_b200_pack's does: a slot,
+ * a block or a row out of range sets one and is skipped. */
+typedef struct hllm_b200_kv8 {
+  uint8_t* k_codes;  /* device, e4m3 [blocks][kv_heads][16][head_dim] */
+  uint8_t* k_scales; /* device, e + 127 [blocks][kv_heads][16] */
+  uint8_t* v_codes;
+  uint8_t* v_scales;
+  uint64_t blocks;
+  uint32_t kv_heads;
+  uint32_t head_dim;
+} hllm_b200_kv8;
+
+/* How positions turn the pairs of a head (cpp/src/cpu/llama.cpp:214-240 is
+ * HALF over the whole head, unscaled, with F32 angles). */
+typedef enum {
+  HLLM_B200_ROPE_NONE = 0,   /* f_i = theta^(-2i / rotary_dim) */
+  HLLM_B200_ROPE_LINEAR = 1, /* f_i / factor */
+  HLLM_B200_ROPE_LLAMA3 = 2, /* by wavelength 2 pi / f_i against original_max_position / high_freq_factor
+                              * (shorter: f_i) and / low_freq_factor (longer: f_i / factor), mixed between */
+  HLLM_B200_ROPE_YARN = 3    /* f_i below the pair that turns beta_fast times in original_max_position,
+                              * f_i / factor above the one that turns beta_slow times, mixed between */
+} hllm_b200_rope_scaling;
+typedef struct hllm_b200_rope {
+  uint32_t rotary_dim;  /* even; pairs i < rotary_dim / 2, the rest of the head is not turned */
+  uint32_t interleaved; /* 0: pairs (i, i + rotary_dim / 2); 1: pairs (2i, 2i + 1) */
+  double theta;         /* > 1 */
+  uint32_t scaling;     /* hllm_b200_rope_scaling */
+  double factor;        /* scaled forms: >= 1 */
+  double low_freq_factor, high_freq_factor; /* LLAMA3: 0 < low < high */
+  double beta_fast, beta_slow;              /* YARN: beta_fast > beta_slow > 0 */
+  double original_max_position;             /* LLAMA3, YARN: > 0 */
+  double attention_factor; /* on cos and sin; 0: 0.1 ln(factor) + 1 for YARN, else 1 */
+} hllm_b200_rope;
+/* The turns per position f_i / (2 pi) of the pairs [rotary_dim / 2], in 64
+ * bits, and the factor on cos and sin.  Host only. */
+hllm_b200_status hllm_b200_rope_turns(const hllm_b200_rope* rope, double* turns, float* factor);
+
+/* hllm_b200_qkv_post for the 8-bit cache and any rotary form: per token and
+ * head of qkv [tokens][(Hq + 2 Hkv) d] (`dtype` F32, F16 or BF16), q and k
+ * RMSNorm where q_norm / k_norm (F32 [d]) are given, rotation at positions[t]
+ * (angles reduced in 64 bits; turns [rotary_dim / 2] F64 and factor from
+ * hllm_b200_rope_turns, turns on the device), q to q_out F16 [tokens][Hq d],
+ * K and V quantised into slots[t].  A token with slot -1 is not stored.  The
+ * slots of a call are distinct, as the packer's are; of tokens that share one,
+ * each stored byte is from one of them.  qkv and q_out are 16-byte aligned. */
+hllm_b200_status hllm_b200_kv8_write(const hllm_b200_kv8* cache, const void* qkv,
+                                     hllm_b200_dtype dtype, uint64_t tokens, uint32_t hq,
+                                     const int32_t* positions, const int32_t* slots,
+                                     const float* q_norm, const float* k_norm, float eps,
+                                     const double* turns, uint32_t rotary_dim,
+                                     uint32_t interleaved, float factor, uint16_t* q_out,
+                                     uint32_t* status, void* stream);
+
+/* The cache's values, rounded once to `dtype`: row r's positions [first[r],
+ * lengths[r]) (first NULL: 0) to rows [offsets[r], offsets[r + 1]) of k_out and
+ * v_out [tokens][kv_heads][head_dim], gathered through block_tables
+ * [rows][max_blocks].  Output rows at or past offsets[rows] are left as they
+ * are; a position without a page, or past its row's length, is zeros and sets
+ * a status bit. */
+hllm_b200_status hllm_b200_kv8_read(const hllm_b200_kv8* cache, const int32_t* block_tables,
+                                    uint32_t rows, uint32_t max_blocks, const int32_t* first,
+                                    const int32_t* lengths, const int32_t* offsets,
+                                    uint64_t tokens, hllm_b200_dtype dtype, void* k_out,
+                                    void* v_out, uint32_t* status, void* stream);
+
+/* hllm_b200_attention over the 8-bit cache, for decode rows, prefill chunks
+ * and mixes of them: row r's new tokens are rows [cu_seqlens[r],
+ * cu_seqlens[r + 1]) of q (F16, row stride ld_q), at positions lengths[r] -
+ * count ... lengths[r] - 1, and each attends to the keys up to its own.  A
+ * token whose position is negative has no key: its output is zeros.  Outputs
+ * are F16 at row stride ld_out; rows of no sequence are left as they are.
+ * max_row_tokens bounds the rows' new tokens (1 for a decode batch); a longer
+ * row, or one past `tokens` or max_blocks, is skipped and sets a status bit.
+ * Keys of a missing page are left out and set one.  q and out are 16-byte
+ * aligned, ld_q and ld_out multiples of 8.  `workspace` (16-byte aligned) has
+ * at least hllm_b200_kv8_attention_workspace bytes for the same counts; its
+ * contents before and after the call mean nothing. */
+hllm_b200_status hllm_b200_kv8_attention_workspace(uint32_t rows, uint64_t tokens,
+                                                   uint64_t max_row_tokens, uint32_t hq,
+                                                   uint32_t kv_heads, uint32_t head_dim,
+                                                   uint64_t* bytes);
+hllm_b200_status hllm_b200_kv8_attention(const hllm_b200_kv8* cache, const uint16_t* q,
+                                         uint64_t ld_q, const int32_t* cu_seqlens,
+                                         const int32_t* lengths, const int32_t* block_tables,
+                                         uint32_t rows, uint64_t tokens, uint64_t max_row_tokens,
+                                         uint32_t hq, uint32_t max_blocks, float scale,
+                                         uint16_t* out, uint64_t ld_out, void* workspace,
+                                         uint64_t workspace_bytes, uint32_t* status, void* stream);
+
 /* Seeded synthetic F16 matrix [rows][cols] at row stride ld (device). */
 hllm_b200_status hllm_b200_synth_matrix(uint64_t seed, uint64_t tag, uint64_t rows, uint64_t cols,
                                         uint64_t ld, float stddev, uint16_t* out, void* stream);
