@@ -40,7 +40,7 @@
 namespace hb {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kLeast = 4;               // pages of a CTA, where there are so many
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoReference = -1e30f;  // below every finite score
 constexpr float kLazy = 8.f;            // log2 of the growth that moves a reference
@@ -68,39 +68,72 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Words (4 codes) a lane holds of one key row, and of one value row.
+// Words (4 codes) of a lane's own slot of the ring.
 template <int W>
-__device__ __forceinline__ void load_words(uint32_t (&w)[W], const uint8_t* p) {
+__device__ __forceinline__ void read_words(uint32_t (&w)[W], const uint8_t* p) {
   if constexpr (W == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
     w[0] = v.x;
     w[1] = v.y;
     w[2] = v.z;
     w[3] = v.w;
   } else if constexpr (W == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x;
     w[1] = v.y;
   } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
+// BYTES from global to shared memory, asynchronously; zeros where !live.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {
+  const int n = live ? BYTES : 0;
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(BYTES)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
-template <int D>
+template <int D, int NT>
 struct Shape {
-  // K: four lanes share a key row, KW words each, KS steps.  V: eight lanes
-  // share a value row, VW words each, VS steps.
+  // K: four lanes share a key row, KW words (of four codes) each, KS steps.
+  // V: eight lanes share a value row, VW words each, VS steps.
   static constexpr int KW = D % 64 == 0 ? 4 : 2, KS = D / (16 * KW);
   static constexpr int VW = D % 128 == 0 ? 4 : D % 64 == 0 ? 2 : 1, VS = D / (32 * VW);
-};
-
-// One page in registers.
-template <int D>
-struct Page {
-  using S = Shape<D>;
-  uint32_t k[S::KS][2][S::KW];  // key rows g and g + 8
-  uint32_t v[S::VS][4][S::VW];  // value rows 2t, 2t + 1, 2t + 8, 2t + 9
-  uint32_t ks[2], vs[2];        // scale bytes of rows g and g + 8
+  static constexpr int kCols = 8 * NT;
+  // 16 warps hide the latency of one page's chain of products; where the sums
+  // and the queries take more than half of 128 registers, 8 warps.
+  static constexpr int kWarps = D * NT <= 128 ? 16 : 8;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kStage = 32 * D + 32;  // a page's codes, each lane's own, and its scales
+  static constexpr int kVAt = 16 * D, kScalesAt = 32 * D;
+  // A piece: D / 16 x NT fragments of 32 lanes x 4 sums, then cols x (m, m', l, 0).
+  static constexpr int kUnits = D / 16 * NT * 32;
+  static constexpr int kPiece = kUnits * 4 + kCols * 4;  // floats
+  // A warp's shared memory: its ring, whose place the piece it leaves open
+  // takes at the end, and the piece it continues, which may be done earlier.
+  static constexpr int kPieceBytes = kPiece * static_cast<int>(sizeof(float));
+  static constexpr int kRoom = 220 * 1024 / kWarps;
+  static constexpr int kStages = 3 * kStage + kPieceBytes <= kRoom ? 3 : 2;
+  static constexpr int kWarpBytes = kStages * kStage + kPieceBytes;
+  static constexpr int kSmem = kWarps * kWarpBytes;
+  static_assert(kStages * kStage >= kPieceBytes && kWarpBytes <= kRoom, "shared memory of a warp");
+  __device__ static float* piece(uint8_t* smem, int p) {
+    return reinterpret_cast<float*>(smem + (p >> 1) * kWarpBytes + (p & 1 ? 0 : kStages * kStage));
+  }
+  // Value dimension of unit (i, lane): rows g and g + 8 of product i are
+  // consecutive dimensions.
+  __device__ static int dim_of(int i, int g) {
+    const int st = i / (2 * VW), rest = i % (2 * VW);
+    return (st * 8 + g) * VW * 4 + rest * 2;
+  }
 };
 
 // A row's place in the packed batch and its streams.
@@ -143,24 +176,40 @@ __device__ __forceinline__ int cut_owner(const Cut& c, long long unit) {
 }
 
 // The workspace: per CTA a record and two pieces (the stream it continues, the
-// stream it leaves open), a piece being cols x D sums and cols x (m, m', l).
+// stream it leaves open).
 struct Record {
   int row, stream, first;  // first: the CTA that holds the stream's first unit; -1: nothing to join
   int pad;
 };
-__host__ __device__ constexpr size_t piece_floats(int dim, int cols) {
-  return static_cast<size_t>(cols) * (dim + 4);
+
+// The output of one unit of a finished stream: sums of columns 2t, 2t + 1 and
+// of dimensions dim, dim + 1, times the columns' factors.
+__device__ __forceinline__ void store_unit(const Kv8AttnArgs& a, const RowInfo& x, int group,
+                                           int kvh, int col, int dim, const float4& v, float f0,
+                                           float f1) {
+  const int cols = x.count * group;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int c = col + e;
+    if (c < cols) {
+      const bool none = x.len - x.count + c / group < 0;  // no key: zeros
+      const float f = e ? f1 : f0;
+      const __half2 h = none ? __floats2half2_rn(0.f, 0.f)
+                             : __floats2half2_rn((e ? v.y : v.x) * f, (e ? v.w : v.z) * f);
+      *reinterpret_cast<__half2*>(a.out + static_cast<size_t>(x.t0 + c / group) * a.ld_out +
+                                  static_cast<size_t>(kvh * group + c % group) * a.cache.dim + dim) = h;
+    }
+  }
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, 1)
+__global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     kv8_stream_kernel(const Kv8AttnArgs a, int group, int tile_from) {
-  using S = Shape<D>;
-  constexpr int kCols = 8 * NT;
-  constexpr int kPiece = kCols * (D + 4);
-  extern __shared__ __align__(16) float pieces[];  // [kWarps][2][kPiece]
-  __shared__ int piece_row[kWarps][2], piece_stream[kWarps][2];
-  __shared__ bool piece_starts[kWarps][2], piece_ends[kWarps][2];
+  using S = Shape<D, NT>;
+  constexpr int kCols = S::kCols, kWarps = S::kWarps, ST = S::kStages;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int piece_row[kWarps * 2], piece_stream[kWarps * 2];
+  __shared__ bool piece_starts[kWarps * 2], piece_ends[kWarps * 2];
   __shared__ long long units_before;  // units before the row of the CTA's first one
   griddep_enter();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -183,9 +232,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     cut.total += n;
   }
-  // A CTA takes kWarps pages at least, where there are so many.
+  // A CTA takes kLeast pages at least, where there are so many.
   cut.ctas = static_cast<int>(
-      min(static_cast<long long>(gridDim.x), max(1LL, (cut.total + kWarps - 1) / kWarps)));
+      min(static_cast<long long>(gridDim.x), max(1LL, (cut.total + kLeast - 1) / kLeast)));
   Record* records = reinterpret_cast<Record*>(a.workspace);
   if (cut.total == 0 || static_cast<int>(blockIdx.x) >= cut.ctas) {
     if (threadIdx.x == 0) records[blockIdx.x].first = -1;
@@ -193,9 +242,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   }
   const long long c0 = cut_begin(cut, blockIdx.x), c1 = cut_begin(cut, blockIdx.x + 1);
   const long long w0 = c0 + (c1 - c0) * warp / kWarps, w1 = c0 + (c1 - c0) * (warp + 1) / kWarps;
-  int n = static_cast<int>(w1 - w0);
-  if (threadIdx.x < kWarps * 2) piece_row[threadIdx.x >> 1][threadIdx.x & 1] = -1;
-  __syncthreads();
+  const int n = static_cast<int>(w1 - w0);
+
+  float o[NT][D / 16][4];
+  float m[NT][2], mo[NT][2], l[NT][2];
+  if (lane < 2) piece_row[warp * 2 + lane] = -1;
+  __syncwarp();
 
   if (n > 0) {
     int row = -1;
@@ -213,9 +265,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       for (int k = 0; k < 4; ++k) {
         long long incl = mine[k];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += v;
+        for (int off = 1; off < 32; off <<= 1) {
+          const long long v = __shfl_up_sync(0xffffffffu, incl, off);
+          if (lane >= off) incl += v;
         }
         const unsigned hit = __ballot_sync(0xffffffffu, before + incl > w0);
         if (row < 0) {
@@ -235,7 +287,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     int q = static_cast<int>((w0 - before) % x.pages);
     const float sl2 = a.scale * kLog2e;
 
-    // The loader runs one unit ahead of the arithmetic.
+    // The loader runs ST - 1 units ahead of the arithmetic.
     int lrow = row, lstream = stream, lq = q;
     RowInfo lx = x;
     int tab_row = -1, tab_q0 = 0, tab = -1;  // 32 entries of the block table, one a lane
@@ -249,9 +301,9 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         if (xi.chunks) return;
       }
     };
-    Page<D> pg[2];
-    bool have[2];
-    auto fetch = [&](Page<D>& p, bool& ok) {
+    uint8_t* ring = smem + warp * S::kWarpBytes;
+    unsigned have = 0;  // bit s: stage s holds a page
+    auto fetch = [&](int stage) {
       if (lrow != tab_row || lq < tab_q0 || lq >= tab_q0 + 32) {
         tab_row = lrow;
         tab_q0 = lq;
@@ -262,43 +314,39 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       }
       const int b = __shfl_sync(0xffffffffu, tab, lq - tab_q0);
       const int valid = lx.len - lq * kKv8Page;  // keys of the page
-      ok = valid > 0 && b >= 0 && b < a.cache.blocks;
-      if (valid > 0 && !ok && lane == 0) atomicOr(a.status, kDevBadIndex);
-      const int kvh = lstream / lx.chunks;
-      const size_t at = (static_cast<size_t>(ok ? b : 0) * hkv + kvh) * kKv8Page;
-      const uint8_t* kp = a.cache.k + at * D;
-      const uint8_t* vp = a.cache.v + at * D;
-      // Rows past the last key may hold anything: they are not read.
-      const bool r0 = ok && g < valid, r1 = ok && g + 8 < valid;
+      const bool ok = valid > 0 && b >= 0 && b < a.cache.blocks;
+      have = (have & ~(1u << stage)) | (ok ? 1u << stage : 0u);
+      if (ok) {
+        const size_t at = (static_cast<size_t>(b) * hkv + lstream / lx.chunks) * kKv8Page;
+        const uint8_t* kp = a.cache.k + at * D + g * D + tq * S::KW * 4;
+        const uint8_t* vp = a.cache.v + at * D + 2 * tq * D + g * S::VW * 4;
+        const uint32_t base = smem_u32(ring + stage * S::kStage);
+        const uint32_t kd = base + lane * S::KW * 4, vd = base + S::kVAt + lane * S::VW * 4;
+        // Rows past the last key may hold anything: they are not read.
 #pragma unroll
-      for (int s = 0; s < S::KS; ++s)
+        for (int s = 0; s < S::KS; ++s)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < 2; ++h)
+            copy_async<S::KW * 4>(kd + (s * 2 + h) * S::KW * 128, kp + 8 * h * D + s * S::KW * 16,
+                                  g + 8 * h < valid);
 #pragma unroll
-          for (int w = 0; w < S::KW; ++w) p.k[s][h][w] = 0u;
-          if (h ? r1 : r0)
-            load_words<S::KW>(p.k[s][h], kp + (g + 8 * h) * D + (s * 4 + tq) * S::KW * 4);
-        }
-      p.ks[0] = r0 ? __ldg(a.cache.k_scale + at + g) : 127u;
-      p.ks[1] = r1 ? __ldg(a.cache.k_scale + at + g + 8) : 127u;
-      p.vs[0] = r0 ? __ldg(a.cache.v_scale + at + g) : 127u;
-      p.vs[1] = r1 ? __ldg(a.cache.v_scale + at + g + 8) : 127u;
+        for (int s = 0; s < S::VS; ++s)
 #pragma unroll
-      for (int s = 0; s < S::VS; ++s)
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int key = 2 * tq + (h & 1) + (h >> 1) * 8;
-#pragma unroll
-          for (int w = 0; w < S::VW; ++w) p.v[s][h][w] = 0u;
-          if (ok && key < valid)
-            load_words<S::VW>(p.v[s][h], vp + key * D + (s * 8 + g) * S::VW * 4);
-        }
+          for (int h = 0; h < 4; ++h) {
+            const int key = (h & 1) + (h >> 1) * 8;
+            copy_async<S::VW * 4>(vd + (s * 4 + h) * S::VW * 128, vp + key * D + s * S::VW * 32,
+                                  2 * tq + key < valid);
+          }
+        if (lane < 8)
+          copy_async<4>(base + S::kScalesAt + lane * 4,
+                        (lane < 4 ? a.cache.k_scale : a.cache.v_scale) + at + (lane & 3) * 4, true);
+      } else if (valid > 0 && lane == 0) {
+        atomicOr(a.status, kDevBadIndex);
+      }
       advance(lrow, lx, lstream, lq);
     };
 
     uint32_t qb[NT][D / 16][2];
-    float o[NT][D / 16][4];
-    float m[NT][2], mo[NT][2], l[NT][2];
     int lim[NT][2];  // last key that columns 2t, 2t + 1 see; -1: none
 
     auto open = [&]() {
@@ -334,33 +382,39 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
       }
     };
 
-    auto multiply = [&](const Page<D>& p, bool ok) {
+    auto multiply = [&](const uint8_t* page, bool ok) {
+      if (!ok) return;  // no keys here
       float s[NT][2][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[nt][0][e] = s[nt][1][e] = 0.f;
 #pragma unroll
-      for (int st = 0; st < S::KS; ++st)
+      for (int st = 0; st < S::KS; ++st) {
+        uint32_t k0[S::KW], k1[S::KW];
+        read_words<S::KW>(k0, page + (st * 2) * S::KW * 128 + lane * S::KW * 4);
+        read_words<S::KW>(k1, page + (st * 2 + 1) * S::KW * 128 + lane * S::KW * 4);
 #pragma unroll
         for (int w = 0; w < S::KW; ++w) {
           const int i = st * S::KW + w;
-          const uint32_t a0 = kv8_half2_lo(p.k[st][0][w]), a2 = kv8_half2_hi(p.k[st][0][w]);
-          const uint32_t a1 = kv8_half2_lo(p.k[st][1][w]), a3 = kv8_half2_hi(p.k[st][1][w]);
+          const uint32_t a0 = kv8_half2_lo(k0[w]), a2 = kv8_half2_hi(k0[w]);
+          const uint32_t a1 = kv8_half2_lo(k1[w]), a3 = kv8_half2_hi(k1[w]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
             mma16816(s[nt][i & 1], a0, a1, a2, a3, qb[nt][i][0], qb[nt][i][1]);
         }
+      }
       const int key = q * kKv8Page + g;
-      const float ks0 = kv8_scale(p.ks[0]) * sl2, ks1 = kv8_scale(p.ks[1]) * sl2;
-      const float ev0 = static_cast<float>(static_cast<int>(p.vs[0]) - 127);
-      const float ev1 = static_cast<float>(static_cast<int>(p.vs[1]) - 127);
+      const uint8_t* sc = page + S::kScalesAt + g;
+      const float ks0 = kv8_scale(sc[0]) * sl2, ks1 = kv8_scale(sc[8]) * sl2;
+      const float ev0 = static_cast<float>(static_cast<int>(sc[16]) - 127);
+      const float ev1 = static_cast<float>(static_cast<int>(sc[24]) - 127);
       bool grown = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool seen = ok && key + (e >> 1) * 8 <= lim[nt][e & 1];
+          const bool seen = key + (e >> 1) * 8 <= lim[nt][e & 1];
           const float v = (s[nt][0][e] + s[nt][1][e]) * (e >> 1 ? ks1 : ks0);
           s[nt][0][e] = seen ? v : -INFINITY;
           s[nt][1][e] = s[nt][0][e] + (e >> 1 ? ev1 : ev0);
@@ -402,31 +456,28 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
         pb[nt][1] = transpose8x8(half2_bits(p2[2], p2[3]));
       }
 #pragma unroll
-      for (int st = 0; st < S::VS; ++st)
+      for (int st = 0; st < S::VS; ++st) {
+        uint32_t v[4][S::VW];
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          read_words<S::VW>(v[h], page + S::kVAt + (st * 4 + h) * S::VW * 128 + lane * S::VW * 4);
 #pragma unroll
         for (int w = 0; w < S::VW; ++w)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t sel = h ? 0x7362u : 0x5140u;
-            const uint32_t lo = __byte_perm(p.v[st][0][w], p.v[st][1][w], sel);
-            const uint32_t hi = __byte_perm(p.v[st][2][w], p.v[st][3][w], sel);
+            const uint32_t lo = __byte_perm(v[0][w], v[1][w], sel);
+            const uint32_t hi = __byte_perm(v[2][w], v[3][w], sel);
             const uint32_t a0 = kv8_half2_lo(lo), a1 = kv8_half2_hi(lo);
             const uint32_t a2 = kv8_half2_lo(hi), a3 = kv8_half2_hi(hi);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
               mma16816(o[nt][(st * S::VW + w) * 2 + h], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
           }
+      }
     };
 
-    // Value dimension of this lane's sums o[nt][i][e]: rows g and g + 8 of
-    // product i hold consecutive dimensions.
-    auto dim_of = [&](int i) {
-      const int st = i / (2 * S::VW), rest = i % (2 * S::VW);
-      return (st * 8 + g) * S::VW * 4 + rest * 2;
-    };
-
-    bool starts = q == 0;
-    auto close = [&](bool ends) {
+    auto sum_l = [&]() {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -434,72 +485,76 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1)
             l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
+    };
+
+    bool starts = q == 0;
+    // The stream's sums so far: its output where this warp had it whole, else a piece.
+    auto close = [&](bool ends) {
+      sum_l();
       if (starts && ends) {
         const int kvh = stream / x.chunks, x0 = (stream % x.chunks) * kCols;
-        const int cols = x.count * group;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int c = x0 + nt * 8 + 2 * tq + e;
-            if (c < cols) {
-              const float f = lim[nt][e] < 0 ? 0.f : ex2(mo[nt][e] - m[nt][e]) / l[nt][e];
-              __half* dst = a.out + static_cast<size_t>(x.t0 + c / group) * a.ld_out +
-                            static_cast<size_t>(kvh * group + c % group) * D;
-#pragma unroll
-              for (int i = 0; i < D / 16; ++i)
-                *reinterpret_cast<__half2*>(dst + dim_of(i)) =
-                    __floats2half2_rn(o[nt][i][e] * f, o[nt][i][e + 2] * f);
-            }
-          }
-        return;
-      }
-      const int which = starts ? 1 : 0;
-      float* piece = pieces + (warp * 2 + which) * kPiece;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = nt * 8 + 2 * tq + e;
+        for (int nt = 0; nt < NT; ++nt) {
+          const float f0 = ex2(mo[nt][0] - m[nt][0]) / l[nt][0];
+          const float f1 = ex2(mo[nt][1] - m[nt][1]) / l[nt][1];
 #pragma unroll
           for (int i = 0; i < D / 16; ++i)
-            *reinterpret_cast<float2*>(piece + c * D + dim_of(i)) =
-                make_float2(o[nt][i][e], o[nt][i][e + 2]);
-          if (g == 0) {
-            float* ml = piece + kCols * D + c * 4;
-            ml[0] = m[nt][e];
-            ml[1] = mo[nt][e];
-            ml[2] = l[nt][e];
-          }
+            store_unit(a, x, group, kvh, x0 + nt * 8 + 2 * tq, S::dim_of(i, g),
+                       make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]), f0, f1);
         }
+        return;
+      }
+      const int p = warp * 2 + (starts ? 1 : 0);
+      float* piece = S::piece(smem, p);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          *reinterpret_cast<float4*>(piece + ((nt * (D / 16) + i) * 32 + lane) * 4) =
+              make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
+        if (g == 0) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float4*>(piece + S::kUnits * 4 + (nt * 8 + 2 * tq + e) * 4) =
+                make_float4(m[nt][e], mo[nt][e], l[nt][e], 0.f);
+        }
+      }
       if (lane == 0) {
-        piece_row[warp][which] = row;
-        piece_stream[warp][which] = stream;
-        piece_starts[warp][which] = starts;
-        piece_ends[warp][which] = ends;
+        piece_row[p] = row;
+        piece_stream[p] = stream;
+        piece_starts[p] = starts;
+        piece_ends[p] = ends;
       }
     };
 
-    fetch(pg[0], have[0]);
-    open();
-#pragma unroll 1
-    for (int i = 0; i < n; i += 2) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (i + b < n) {
-          if (i + b + 1 < n) fetch(pg[b ^ 1], have[b ^ 1]);
-          multiply(pg[b], have[b]);
-          const bool ends = q == x.pages - 1;
-          if (ends || i + b + 1 == n) close(ends);
-          if (i + b + 1 < n) {
-            advance(row, x, stream, q);
-            if (q == 0) {
-              starts = true;
-              open();
-            }
-          }
+    for (int i = 0; i < ST - 1; ++i) {
+      if (i < n) fetch(i);
+      copy_commit();
+    }
+    open();
+    int stage = 0, ahead = ST - 1;  // of the page at hand, and of the one to fetch
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      copy_wait<ST - 2>();
+      __syncwarp();  // the scales are other lanes' copies; the stage to fill is read by none
+      if (i + ST - 1 < n) fetch(ahead);
+      copy_commit();
+      multiply(ring + stage * S::kStage, (have >> stage) & 1u);
+      const bool ends = q == x.pages - 1;
+      if (ends || i + 1 == n) {
+        __syncwarp();  // an open piece takes the ring's place
+        close(ends);
+      }
+      if (i + 1 < n) {
+        advance(row, x, stream, q);
+        if (q == 0) {
+          starts = true;
+          open();
         }
       }
+      stage = stage + 1 == ST ? 0 : stage + 1;
+      ahead = ahead + 1 == ST ? 0 : ahead + 1;
     }
   }
   __syncthreads();
@@ -507,55 +562,64 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   // Join the warps' pieces: a chain is a run of pieces of one stream.
   Record rec{0, 0, -1, 0};
   auto next_piece = [&](int from) {
-    while (from < kWarps * 2 && piece_row[from >> 1][from & 1] < 0) ++from;
+    while (from < kWarps * 2 && piece_row[from] < 0) ++from;
     return from;
   };
   int i = next_piece(0);
   while (i < kWarps * 2) {
-    const int row = piece_row[i >> 1][i & 1], stream = piece_stream[i >> 1][i & 1];
+    const int row = piece_row[i], stream = piece_stream[i];
     int last = i, j = next_piece(i + 1);
-    while (j < kWarps * 2 && piece_row[j >> 1][j & 1] == row && piece_stream[j >> 1][j & 1] == stream) {
+    while (j < kWarps * 2 && piece_row[j] == row && piece_stream[j] == stream) {
       last = j;
       j = next_piece(j + 1);
     }
-    const bool begins = piece_starts[i >> 1][i & 1], ends = piece_ends[last >> 1][last & 1];
+    const bool begins = piece_starts[i], ends = piece_ends[last];
     const RowInfo x = row_info(a, row, group, kCols, tile_from, false);
     const int kvh = stream / x.chunks, x0 = (stream % x.chunks) * kCols;
-    float* dst = a.workspace + gridDim.x * 4 +
-                 (static_cast<size_t>(blockIdx.x) * 2 + (begins ? 1 : 0)) * kPiece;
-    for (int u = threadIdx.x; u < kCols * D / 4; u += kWarps * 32) {
-      const int c = u / (D / 4), dd = (u % (D / 4)) * 4;
-      float M = kNoReference, MO = kNoReference;
+    float* dst = reinterpret_cast<float*>(records + gridDim.x) +
+                 (static_cast<size_t>(blockIdx.x) * 2 + (begins ? 1 : 0)) * S::kPiece;
+    for (int u = threadIdx.x; u < S::kUnits; u += S::kThreads) {
+      const int nt = u / (D / 16 * 32), col = nt * 8 + 2 * (u & 3);
+      if (x0 + col >= x.count * group) continue;
+      float M[2] = {kNoReference, kNoReference}, MO[2] = {kNoReference, kNoReference};
       for (int k = i; k <= last; ++k)
-        if (piece_row[k >> 1][k & 1] >= 0) {
-          M = fmaxf(M, pieces[k * kPiece + kCols * D + c * 4]);
-          MO = fmaxf(MO, pieces[k * kPiece + kCols * D + c * 4 + 1]);
+        if (piece_row[k] >= 0) {
+          const float4* ml = reinterpret_cast<const float4*>(S::piece(smem, k) + S::kUnits * 4) + col;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            M[e] = fmaxf(M[e], ml[e].x);
+            MO[e] = fmaxf(MO[e], ml[e].y);
+          }
         }
-      float L = 0.f;
+      float L[2] = {0.f, 0.f};
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k = i; k <= last; ++k)
-        if (piece_row[k >> 1][k & 1] >= 0) {
-          const float* ml = pieces + k * kPiece + kCols * D + c * 4;
-          L += ml[2] * ex2(ml[0] - M);
-          const float f = ex2(ml[1] - MO);
-          const float4 v = *reinterpret_cast<const float4*>(pieces + k * kPiece + c * D + dd);
-          acc.x += v.x * f;
-          acc.y += v.y * f;
-          acc.z += v.z * f;
-          acc.w += v.w * f;
+        if (piece_row[k] >= 0) {
+          const float* piece = S::piece(smem, k);
+          const float4* ml = reinterpret_cast<const float4*>(piece + S::kUnits * 4) + col;
+          float f[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            L[e] += ml[e].z * ex2(ml[e].x - M[e]);
+            f[e] = ex2(ml[e].y - MO[e]);
+          }
+          const float4 v = *reinterpret_cast<const float4*>(piece + u * 4);
+          acc.x += v.x * f[0];
+          acc.y += v.y * f[1];
+          acc.z += v.z * f[0];
+          acc.w += v.w * f[1];
         }
       if (begins && ends) {
-        const int col = x0 + c;
-        if (col < x.count * group) {
-          const float f = x.len - x.count + col / group < 0 ? 0.f : ex2(MO - M) / L;
-          __half* out = a.out + static_cast<size_t>(x.t0 + col / group) * a.ld_out +
-                        static_cast<size_t>(kvh * group + col % group) * D + dd;
-          *reinterpret_cast<uint2*>(out) =
-              make_uint2(half2_bits(acc.x * f, acc.y * f), half2_bits(acc.z * f, acc.w * f));
-        }
+        store_unit(a, x, group, kvh, x0 + col, S::dim_of((u >> 5) % (D / 16), (u >> 2) & 7), acc,
+                   ex2(MO[0] - M[0]) / L[0], ex2(MO[1] - M[1]) / L[1]);
       } else {
-        *reinterpret_cast<float4*>(dst + c * D + dd) = acc;
-        if (dd == 0) *reinterpret_cast<float4*>(dst + kCols * D + c * 4) = make_float4(M, MO, L, 0.f);
+        *reinterpret_cast<float4*>(dst + u * 4) = acc;
+        if (u % (D / 16 * 32) < 4) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float4*>(dst + S::kUnits * 4 + (col + e) * 4) =
+                make_float4(M[e], MO[e], L[e], 0.f);
+        }
       }
     }
     if (!begins && ends) {
@@ -571,49 +635,86 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
 }
 
 // Joins the pieces of a stream that spans CTAs, in order; one CTA for each CTA
-// of the stream pass, with work where that one ended such a stream.
+// of the stream pass, with work where that one ended such a stream.  A warp a
+// column finds the references and the pieces' weights; then the units are
+// summed, kJoinGroups shares of the pieces at a time.
+constexpr int kJoinThreads = 512, kJoinGroups = 4;
 template <int D, int NT>
-__global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a, int group, int tile_from) {
-  constexpr int kCols = 8 * NT;
-  constexpr int kPiece = kCols * (D + 4);
+__global__ void __launch_bounds__(kJoinThreads)
+    kv8_join_kernel(const Kv8AttnArgs a, int group, int tile_from) {
+  using S = Shape<D, NT>;
+  constexpr int kCols = S::kCols;
+  extern __shared__ __align__(16) float weight[];  // [pieces][kCols]
+  __shared__ float factor[kCols];
+  __shared__ float4 share[kJoinGroups - 1][kJoinThreads / kJoinGroups];
   griddep_enter();
-  const Record rec = reinterpret_cast<const Record*>(a.workspace)[blockIdx.x];
+  const Record* records = reinterpret_cast<const Record*>(a.workspace);
+  const Record rec = records[blockIdx.x];
   const int first = rec.first, end = blockIdx.x;
   if (first < 0 || first >= end) return;
   const RowInfo x = row_info(a, rec.row, group, kCols, tile_from, false);
   if (x.chunks == 0) return;
   const int kvh = rec.stream / x.chunks, x0 = (rec.stream % x.chunks) * kCols;
-  const float* base = a.workspace + gridDim.x * 4;
+  const int cols = min(kCols, x.count * group - x0);
+  const float* base = reinterpret_cast<const float*>(records + gridDim.x);
   // Piece of CTA c: the one it left open for the first, else the one it continued.
-  auto piece = [&](int c) { return base + (static_cast<size_t>(c) * 2 + (c == first ? 1 : 0)) * kPiece; };
-  for (int u = threadIdx.x; u < kCols * D / 4; u += 256) {
-    const int c = u / (D / 4), dd = (u % (D / 4)) * 4;
-    const int col = x0 + c;
-    if (col >= x.count * group) continue;
+  auto piece = [&](int c) {
+    return base + (static_cast<size_t>(c) * 2 + (c == first ? 1 : 0)) * S::kPiece;
+  };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp < cols) {
     float M = kNoReference, MO = kNoReference;
-    for (int k = first; k <= end; ++k) {
-      const float4 ml = __ldcg(reinterpret_cast<const float4*>(piece(k) + kCols * D + c * 4));
+    for (int k = first + lane; k <= end; k += 32) {
+      const float4 ml = __ldcg(reinterpret_cast<const float4*>(piece(k) + S::kUnits * 4) + warp);
       M = fmaxf(M, ml.x);
       MO = fmaxf(MO, ml.y);
     }
+    M = warp_max(M);
+    MO = warp_max(MO);
     float L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = first; k <= end; ++k) {
-      const float4 ml = __ldcg(reinterpret_cast<const float4*>(piece(k) + kCols * D + c * 4));
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(k) + c * D + dd));
+    for (int k = first + lane; k <= end; k += 32) {
+      const float4 ml = __ldcg(reinterpret_cast<const float4*>(piece(k) + S::kUnits * 4) + warp);
       L += ml.z * ex2(ml.x - M);
-      const float f = ex2(ml.y - MO);
-      acc.x += v.x * f;
-      acc.y += v.y * f;
-      acc.z += v.z * f;
-      acc.w += v.w * f;
+      weight[(k - first) * kCols + warp] = ex2(ml.y - MO);
     }
-    const float f = x.len - x.count + col / group < 0 ? 0.f : ex2(MO - M) / L;
-    __half* out = a.out + static_cast<size_t>(x.t0 + col / group) * a.ld_out +
-                  static_cast<size_t>(kvh * group + col % group) * D + dd;
-    *reinterpret_cast<uint2*>(out) =
-        make_uint2(half2_bits(acc.x * f, acc.y * f), half2_bits(acc.z * f, acc.w * f));
+    L = warp_sum(L);
+    if (lane == 0) factor[warp] = ex2(MO - M) / L;
+  }
+  __syncthreads();
+  constexpr int kAtOnce = kJoinThreads / kJoinGroups;
+  const int part = threadIdx.x / kAtOnce, mine = threadIdx.x % kAtOnce;
+  for (int u0 = 0; u0 < S::kUnits; u0 += kAtOnce) {
+    const int u = u0 + mine;
+    const int col = u / (D / 16 * 32) * 8 + 2 * (u & 3);
+    const bool live = u < S::kUnits && col < cols;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live) {
+#pragma unroll 8
+      for (int k = first + part; k <= end; k += kJoinGroups) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(k) + u * 4));
+        const float f0 = weight[(k - first) * kCols + col];
+        const float f1 = col + 1 < cols ? weight[(k - first) * kCols + col + 1] : 0.f;
+        acc.x += v.x * f0;
+        acc.y += v.y * f1;
+        acc.z += v.z * f0;
+        acc.w += v.w * f1;
+      }
+    }
+    if (part > 0) share[part - 1][mine] = acc;
+    __syncthreads();
+    if (part == 0 && live) {
+#pragma unroll
+      for (int p = 0; p < kJoinGroups - 1; ++p) {
+        const float4 v = share[p][mine];
+        acc.x += v.x;
+        acc.y += v.y;
+        acc.z += v.z;
+        acc.w += v.w;
+      }
+      store_unit(a, x, group, kvh, x0 + col, S::dim_of((u >> 5) % (D / 16), (u >> 2) & 7), acc,
+                 factor[col], col + 1 < cols ? factor[col + 1] : 0.f);
+    }
+    __syncthreads();
   }
 }
 
@@ -621,30 +722,34 @@ int stream_ctas(int sm_count) { return sm_count; }
 
 template <int D, int NT>
 cudaError_t launch_stream(const Kv8AttnArgs& a, int tile_from, cudaStream_t stream) {
-  constexpr size_t smem = static_cast<size_t>(kWarps) * 2 * 8 * NT * (D + 4) * sizeof(float);
+  using S = Shape<D, NT>;
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !configured[dev]) {
     e = cudaFuncSetAttribute(kv8_stream_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem));
+                             static_cast<int>(S::kSmem));
     if (e != cudaSuccess) return e;
     if (dev < 64) configured[dev] = true;
   }
   const int group = a.hq / a.cache.hkv;
   const int ctas = stream_ctas(a.sm_count);
-  e = launch_dependent(kv8_stream_kernel<D, NT>, dim3(ctas), dim3(kWarps * 32), smem, stream, a,
+  e = launch_dependent(kv8_stream_kernel<D, NT>, dim3(ctas), dim3(S::kThreads), S::kSmem, stream, a,
                        group, tile_from);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kv8_join_kernel<D, NT>, dim3(ctas), dim3(256), 0, stream, a, group,
+  return launch_dependent(kv8_join_kernel<D, NT>, dim3(ctas), dim3(kJoinThreads),
+                          static_cast<size_t>(ctas) * S::kCols * sizeof(float), stream, a, group,
                           tile_from);
 }
+
+// Bytes of a piece: Shape<dim, nt>::kPieceBytes.
+size_t piece_bytes(int dim, int nt) { return (static_cast<size_t>(dim) / 16 * nt * 32 * 4 + 8 * nt * 4) * sizeof(float); }
 
 }  // namespace
 
 size_t kv8_attention_workspace(int, int, int, int, int, int dim, int sm_count) {
-  return static_cast<size_t>(stream_ctas(sm_count)) * (4 + 2 * piece_floats(dim, 16)) * sizeof(float);
+  return static_cast<size_t>(stream_ctas(sm_count)) * (sizeof(Record) + 2 * piece_bytes(dim, dim <= 128 ? 2 : 1));
 }
 
 cudaError_t kv8_attention_launch(const Kv8AttnArgs& a, cudaStream_t stream) {
