@@ -17,6 +17,10 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
+#include "common.cuh"
+
 namespace hb {
 
 constexpr int kKv8Page = 16;     // tokens of a page, as in the F16 pool
@@ -78,12 +82,55 @@ struct Kv8AttnArgs {
   uint32_t* status;
   int sm_count;
 };
+// Whether the tile pass (kv8_tile.cu: prompt chunks on tcgen05) takes a head
+// size, its share of the workspace, and its launches: tiles, then, once the
+// stream pass is launched, the join of their key splits.
+bool kv8_tile_supported(int dim);
+size_t kv8_tile_workspace(int rows, int tokens, int hq, int hkv, int dim, int sm_count);
+cudaError_t kv8_tile_launch(const Kv8AttnArgs& a, int tile_from, float* partial, cudaStream_t stream);
+cudaError_t kv8_tile_join_launch(const Kv8AttnArgs& a, int tile_from, const float* partial,
+                                 cudaStream_t stream);
+
 size_t kv8_attention_workspace(int rows, int tokens, int max_row_tokens, int hq, int hkv, int dim,
                                int sm_count);
 cudaError_t kv8_attention_launch(const Kv8AttnArgs& a, cudaStream_t stream);
 
-// ---------------------------------------------------------------- device side
 #ifdef __CUDACC__
+// A kernel's dynamic shared memory limit, raised once a device.  `registers`:
+// refused with fewer registers a thread, for a kernel that moves registers
+// between its warps and would wait for ever for those it was not launched with.
+struct Kv8Configured {
+  std::atomic<bool> done[64] = {};
+  template <typename K>
+  cudaError_t once(K kernel, int bytes, int registers = 0) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+    cudaFuncAttributes f{};
+    e = cudaFuncGetAttributes(&f, kernel);
+    if (e != cudaSuccess) return e;
+    if (f.numRegs < registers) return cudaErrorInvalidConfiguration;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_relaxed);
+    return e;
+  }
+};
+
+// ---------------------------------------------------------------- device side
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoReference = -1e30f;  // below every finite score
+constexpr float kLazy = 8.f;            // log2 of the growth that moves a softmax reference
+
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // The value of a scale byte.
 __device__ __forceinline__ float kv8_scale(uint32_t byte) {
   return __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fc00000u : byte << 23);
@@ -110,6 +157,34 @@ __device__ __forceinline__ uint32_t kv8_codes(float lo, float hi) {
       : "=r"(w)
       : "f"(lo), "f"(hi));
   return w;
+}
+
+// A row's place in the packed batch and its streams: groups of `cols` columns,
+// a column being one query head of the kv head's group at one new token.
+struct Kv8Row {
+  int count, len, t0;  // new tokens, keys, first packed token
+  int pages;           // at least 1, so that a row without keys is answered too
+  int chunks;          // column groups per kv head
+};
+
+// Row r as the stream pass (tiles false: rows under tile_from columns) or the
+// tile pass (the others) sees it: rows of the other pass, and rows out of the
+// batch's bounds (reported), have count 0.
+__device__ __forceinline__ Kv8Row kv8_row(const Kv8AttnArgs& a, int r, int group, int cols,
+                                          int tile_from, bool report, bool tiles = false) {
+  Kv8Row x;
+  x.t0 = __ldg(a.cu_seqlens + r);
+  const int end = __ldg(a.cu_seqlens + r + 1);
+  x.len = __ldg(a.lengths + r);
+  const long long count = static_cast<long long>(end) - x.t0;
+  const bool bad = x.t0 < 0 || count < 0 || end > a.tokens || count > a.max_row_tokens ||
+                   x.len < 0 || x.len > a.max_blocks * static_cast<long long>(kKv8Page);
+  if (bad && report) atomicOr(a.status, kDevBadIndex);
+  x.count = bad || (count * group >= tile_from) != tiles ? 0 : static_cast<int>(count);
+  if (bad) x.len = 0;
+  x.pages = max(1, (x.len + kKv8Page - 1) / kKv8Page);
+  x.chunks = static_cast<int>((static_cast<long long>(x.count) * group + cols - 1) / cols);
+  return x;
 }
 #endif
 

@@ -41,9 +41,6 @@ namespace hb {
 namespace {
 
 constexpr int kLeast = 4;               // pages of a CTA, where there are so many
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNoReference = -1e30f;  // below every finite score
-constexpr float kLazy = 8.f;            // log2 of the growth that moves a reference
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -57,15 +54,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t o;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(o) : "r"(v));
   return o;
-}
-__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Words (4 codes) of a lane's own slot of the ring.
@@ -136,31 +124,7 @@ struct Shape {
   }
 };
 
-// A row's place in the packed batch and its streams.
-struct RowInfo {
-  int count, len, t0;  // new tokens, keys, first packed token
-  int pages;           // at least 1, so that a row without keys is answered too
-  int chunks;          // streams per kv head
-};
-
-// Rows that this pass does not answer have count 0: rows out of the batch's
-// bounds (reported) and rows long enough for the tile pass.
-__device__ __forceinline__ RowInfo row_info(const Kv8AttnArgs& a, int r, int group, int cols,
-                                            int tile_from, bool report) {
-  RowInfo x;
-  x.t0 = __ldg(a.cu_seqlens + r);
-  const int end = __ldg(a.cu_seqlens + r + 1);
-  x.len = __ldg(a.lengths + r);
-  x.count = end - x.t0;
-  const bool bad = x.t0 < 0 || x.count < 0 || end > a.tokens || x.count > a.max_row_tokens ||
-                   x.len < 0 || x.len > a.max_blocks * static_cast<long long>(kKv8Page);
-  if (bad && report) atomicOr(a.status, kDevBadIndex);
-  if (bad || x.count * static_cast<long long>(group) >= tile_from) x.count = 0;
-  x.pages = max(1, static_cast<int>((static_cast<long long>(x.len) + kKv8Page - 1) / kKv8Page));
-  x.chunks = static_cast<int>((static_cast<long long>(x.count) * group + cols - 1) / cols);
-  return x;
-}
-__device__ __forceinline__ long long row_units(const RowInfo& x, int hkv) {
+__device__ __forceinline__ long long row_units(const Kv8Row& x, int hkv) {
   return static_cast<long long>(x.chunks) * hkv * x.pages;
 }
 
@@ -184,7 +148,7 @@ struct Record {
 
 // The output of one unit of a finished stream: sums of columns 2t, 2t + 1 and
 // of dimensions dim, dim + 1, times the columns' factors.
-__device__ __forceinline__ void store_unit(const Kv8AttnArgs& a, const RowInfo& x, int group,
+__device__ __forceinline__ void store_unit(const Kv8AttnArgs& a, const Kv8Row& x, int group,
                                            int kvh, int col, int dim, const float4& v, float f0,
                                            float f1) {
   const int cols = x.count * group;
@@ -204,14 +168,19 @@ __device__ __forceinline__ void store_unit(const Kv8AttnArgs& a, const RowInfo& 
 
 template <int D, int NT>
 __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
-    kv8_stream_kernel(const Kv8AttnArgs a, int group, int tile_from) {
+    kv8_stream_kernel(const Kv8AttnArgs a, int group, int tile_from, bool beside) {
   using S = Shape<D, NT>;
   constexpr int kCols = S::kCols, kWarps = S::kWarps, ST = S::kStages;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int piece_row[kWarps * 2], piece_stream[kWarps * 2];
   __shared__ bool piece_starts[kWarps * 2], piece_ends[kWarps * 2];
   __shared__ long long units_before;  // units before the row of the CTA's first one
-  griddep_enter();
+  // Launched behind the tile pass this one runs beside it: that pass lets its
+  // successor start once all its CTAs have seen the work before them complete,
+  // and the two share no output.  It then waits before it ends, so that what
+  // follows it follows both.
+  if (!beside) griddep_wait();
+  griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, tq = lane & 3;
   const int hkv = a.cache.hkv;
@@ -223,7 +192,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int r = base + 32 * k + lane;
-      mine[k] = r < a.rows ? row_units(row_info(a, r, group, kCols, tile_from,
+      mine[k] = r < a.rows ? row_units(kv8_row(a, r, group, kCols, tile_from,
                                                 blockIdx.x == 0 && warp == 0), hkv)
                            : 0;
     }
@@ -238,6 +207,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
   Record* records = reinterpret_cast<Record*>(a.workspace);
   if (cut.total == 0 || static_cast<int>(blockIdx.x) >= cut.ctas) {
     if (threadIdx.x == 0) records[blockIdx.x].first = -1;
+    if (beside) griddep_wait();
     return;
   }
   const long long c0 = cut_begin(cut, blockIdx.x), c1 = cut_begin(cut, blockIdx.x + 1);
@@ -258,7 +228,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
         for (int k = 0; k < 4; ++k) {
           const int r = base + 32 * k + lane;
           mine[k] =
-              r < a.rows ? row_units(row_info(a, r, group, kCols, tile_from, false), hkv) : 0;
+              r < a.rows ? row_units(kv8_row(a, r, group, kCols, tile_from, false), hkv) : 0;
         }
       }
 #pragma unroll
@@ -282,22 +252,22 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       }
     }
     if (w0 == c0 && lane == 0) units_before = before;
-    RowInfo x = row_info(a, row, group, kCols, tile_from, false);
+    Kv8Row x = kv8_row(a, row, group, kCols, tile_from, false);
     int stream = static_cast<int>((w0 - before) / x.pages);
     int q = static_cast<int>((w0 - before) % x.pages);
     const float sl2 = a.scale * kLog2e;
 
     // The loader runs ST - 1 units ahead of the arithmetic.
     int lrow = row, lstream = stream, lq = q;
-    RowInfo lx = x;
+    Kv8Row lx = x;
     int tab_row = -1, tab_q0 = 0, tab = -1;  // 32 entries of the block table, one a lane
-    auto advance = [&](int& r, RowInfo& xi, int& st, int& page) {
+    auto advance = [&](int& r, Kv8Row& xi, int& st, int& page) {
       if (++page < xi.pages) return;
       page = 0;
       if (++st < xi.chunks * hkv) return;
       st = 0;
       while (++r < a.rows) {
-        xi = row_info(a, r, group, kCols, tile_from, false);
+        xi = kv8_row(a, r, group, kCols, tile_from, false);
         if (xi.chunks) return;
       }
     };
@@ -574,7 +544,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       j = next_piece(j + 1);
     }
     const bool begins = piece_starts[i], ends = piece_ends[last];
-    const RowInfo x = row_info(a, row, group, kCols, tile_from, false);
+    const Kv8Row x = kv8_row(a, row, group, kCols, tile_from, false);
     const int kvh = stream / x.chunks, x0 = (stream % x.chunks) * kCols;
     float* dst = reinterpret_cast<float*>(records + gridDim.x) +
                  (static_cast<size_t>(blockIdx.x) * 2 + (begins ? 1 : 0)) * S::kPiece;
@@ -632,6 +602,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     i = j;
   }
   if (threadIdx.x == 0) records[blockIdx.x] = rec;
+  if (beside) griddep_wait();
 }
 
 // Joins the pieces of a stream that spans CTAs, in order; one CTA for each CTA
@@ -652,7 +623,7 @@ __global__ void __launch_bounds__(kJoinThreads)
   const Record rec = records[blockIdx.x];
   const int first = rec.first, end = blockIdx.x;
   if (first < 0 || first >= end) return;
-  const RowInfo x = row_info(a, rec.row, group, kCols, tile_from, false);
+  const Kv8Row x = kv8_row(a, rec.row, group, kCols, tile_from, false);
   if (x.chunks == 0) return;
   const int kvh = rec.stream / x.chunks, x0 = (rec.stream % x.chunks) * kCols;
   const int cols = min(kCols, x.count * group - x0);
@@ -721,22 +692,15 @@ __global__ void __launch_bounds__(kJoinThreads)
 int stream_ctas(int sm_count) { return sm_count; }
 
 template <int D, int NT>
-cudaError_t launch_stream(const Kv8AttnArgs& a, int tile_from, cudaStream_t stream) {
+cudaError_t launch_stream(const Kv8AttnArgs& a, int tile_from, bool beside, cudaStream_t stream) {
   using S = Shape<D, NT>;
-  static bool configured[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  static Kv8Configured configured;
+  cudaError_t e = configured.once(kv8_stream_kernel<D, NT>, S::kSmem);
   if (e != cudaSuccess) return e;
-  if (dev >= 64 || !configured[dev]) {
-    e = cudaFuncSetAttribute(kv8_stream_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(S::kSmem));
-    if (e != cudaSuccess) return e;
-    if (dev < 64) configured[dev] = true;
-  }
   const int group = a.hq / a.cache.hkv;
   const int ctas = stream_ctas(a.sm_count);
   e = launch_dependent(kv8_stream_kernel<D, NT>, dim3(ctas), dim3(S::kThreads), S::kSmem, stream, a,
-                       group, tile_from);
+                       group, tile_from, beside);
   if (e != cudaSuccess) return e;
   return launch_dependent(kv8_join_kernel<D, NT>, dim3(ctas), dim3(kJoinThreads),
                           static_cast<size_t>(ctas) * S::kCols * sizeof(float), stream, a, group,
@@ -744,24 +708,51 @@ cudaError_t launch_stream(const Kv8AttnArgs& a, int tile_from, cudaStream_t stre
 }
 
 // Bytes of a piece: Shape<dim, nt>::kPieceBytes.
-size_t piece_bytes(int dim, int nt) { return (static_cast<size_t>(dim) / 16 * nt * 32 * 4 + 8 * nt * 4) * sizeof(float); }
+size_t piece_bytes(int dim, int nt) {
+  return (static_cast<size_t>(dim) / 16 * nt * 32 * 4 + 8 * nt * 4) * sizeof(float);
+}
+
+// Rows with this many columns (new tokens x query heads of a group) go to the
+// tile pass: half a tile of queries, from where its products beat walking the
+// pages once for every 16 columns.
+constexpr int kTileFrom = 64;
+
+bool with_tiles(int max_row_tokens, int hq, int hkv, int dim) {
+  return kv8_tile_supported(dim) &&
+         static_cast<long long>(max_row_tokens) * (hq / hkv) >= kTileFrom;
+}
+size_t stream_workspace(int dim, int sm_count) {
+  return static_cast<size_t>(stream_ctas(sm_count)) *
+         (sizeof(Record) + 2 * piece_bytes(dim, dim <= 128 ? 2 : 1));
+}
 
 }  // namespace
 
-size_t kv8_attention_workspace(int, int, int, int, int, int dim, int sm_count) {
-  return static_cast<size_t>(stream_ctas(sm_count)) * (sizeof(Record) + 2 * piece_bytes(dim, dim <= 128 ? 2 : 1));
+size_t kv8_attention_workspace(int rows, int tokens, int max_row_tokens, int hq, int hkv, int dim,
+                               int sm_count) {
+  return stream_workspace(dim, sm_count) +
+         (with_tiles(max_row_tokens, hq, hkv, dim)
+              ? kv8_tile_workspace(rows, tokens, hq, hkv, dim, sm_count)
+              : 0);
 }
 
 cudaError_t kv8_attention_launch(const Kv8AttnArgs& a, cudaStream_t stream) {
   if (a.rows == 0 || a.tokens == 0) return cudaSuccess;
-  const int tile_from = 0x7fffffff;
-  const int group = a.hq / a.cache.hkv;
-  const bool wide = group > 8 || a.max_row_tokens > 1;
+  const bool tiles = with_tiles(a.max_row_tokens, a.hq, a.cache.hkv, a.cache.dim);
+  const int tile_from = tiles ? kTileFrom : 0x7fffffff;
+  float* partial = a.workspace + stream_workspace(a.cache.dim, a.sm_count) / sizeof(float);
+  cudaError_t e = cudaSuccess;
+  if (tiles) e = kv8_tile_launch(a, tile_from, partial, stream);
+  if (e != cudaSuccess) return e;
+  // 16 columns a stream where the rows have them; one-token rows of a group of
+  // at most 8 heads have not.
+  const bool wide = a.hq / a.cache.hkv > 8 || (a.max_row_tokens > 1 && !tiles);
   switch (a.cache.dim) {
-#define HB_KV8_DIM(D)                                                   \
-  case D:                                                               \
-    return wide && D <= 128 ? launch_stream<D, D <= 128 ? 2 : 1>(a, tile_from, stream) \
-                            : launch_stream<D, 1>(a, tile_from, stream);
+#define HB_KV8_DIM(D)                                                                        \
+  case D:                                                                                    \
+    e = wide && D <= 128 ? launch_stream<D, D <= 128 ? 2 : 1>(a, tile_from, tiles, stream)   \
+                         : launch_stream<D, 1>(a, tile_from, tiles, stream);                 \
+    break;
     HB_KV8_DIM(32)
     HB_KV8_DIM(64)
     HB_KV8_DIM(96)
@@ -773,6 +764,8 @@ cudaError_t kv8_attention_launch(const Kv8AttnArgs& a, cudaStream_t stream) {
 #undef HB_KV8_DIM
     default: return cudaErrorInvalidValue;
   }
+  if (e == cudaSuccess && tiles) e = kv8_tile_join_launch(a, tile_from, partial, stream);
+  return e;
 }
 
 }  // namespace hb

@@ -1,0 +1,743 @@
+// kv8_tile.cu -- prompt chunks over the 8-bit paged KV cache on the
+// 5th-generation tensor cores (head sizes 64 and 128).
+//
+// The rows of a tile are 128 columns (token, query head of the kv head's
+// group) of one batch row; S = Q K^T and O += P V run as tcgen05 products of
+// F16 operands into TMEM, 128 keys at a time.  Tensor-bound: 4 x 128 x 128 x D
+// operations a tile, next to which the codes are few bytes, so the work is to
+// keep the tensor pipe fed while codes become F16 and scores become weights:
+//
+//   warps 8-11  converters: a tile's K and V codes from their pages into
+//               shared memory as swizzled F16 operands.  K rows are code *
+//               2^(e - E) with E the tile's largest exponent, so that F16 holds
+//               rows of any size; what it rounds lies 2^-34 below the largest
+//               row, and E goes into the score scale of the tile.  V rows are
+//               the codes; their scales go into the weights.
+//   warp 12     one thread issues the products.
+//   warps 0-7   two softmax groups of 128 threads, one row (TMEM lane) a
+//               thread.  The weights go back into TMEM over the scores they
+//               came from, as F16, and are the A operand of P V from there.
+//
+// The two groups keep the tensor pipe busy for one another: while one group's
+// scores become weights, the other's products run.  With many tiles (SHARED) a
+// CTA holds two tiles of queries and both groups use each key tile that the
+// converters make.  With few, both groups work on one tile of queries and take
+// the key tiles in turn, the two halves being joined at the end; and the keys
+// of a tile are split over CTAs, joined by a second launch.
+//
+// With s_j the score in log2 and ev_j the exponent of value row j, a row keeps
+// one reference m for  l = sum 2^(s_j - m)  and  O = sum (2^(s_j - m) 2^ev_j) d_j,
+// d_j the codes: the weights in brackets are what F16 has to hold, so m follows
+// max (s_j + ev_j), and o = O / l.  Each group computes a key tile's weights
+// against the reference it has, in one pass over the scores, and only where a
+// weight passes 2^8 (first tiles, mostly) goes back for the maximum.  Every
+// wait is bounded (common.cuh).
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "kv8.cuh"
+
+namespace hb {
+namespace {
+
+constexpr int kKeys = 128;       // keys of a tile
+constexpr int kRows = 128;       // columns of a query tile
+constexpr int kSoftmax = 256;    // threads of the softmax groups
+constexpr int kThreads = kSoftmax + 128 + 128;  // the last warps but one idle: registers go by four warps
+constexpr float kMostWeight = 256.f;              // 2^kLazy
+
+// D[tmem] (+)= A[tmem] * B[smem desc]: A is F16 pairs, a row per lane.
+__device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 32 lanes x 32 bits, 16 consecutive columns a thread, without the wait.
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32"
+      " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+template <int D, bool SHARED>
+struct Tile {
+  static constexpr int kQueries = SHARED ? 2 : 1;           // query tiles of a CTA
+  static constexpr uint32_t kAtom = 128 * 128;              // 128 rows x 64 F16: one swizzle column
+  static constexpr uint32_t kOperand = 128 * D * 2;         // Q, K or V of 128 rows
+  static constexpr uint32_t kQ = 0, kK = kQueries * kOperand, kV = kK + 2 * kOperand;
+  static constexpr uint32_t kEnd = kV + 2 * kOperand;
+  static constexpr uint32_t kSmem = kEnd + 1024;            // 1024-byte alignment slack
+  static constexpr uint32_t kTmemS = 0, kTmemO = 256;       // per group: + 128 g
+  // A partial result: D / 4 x 128 rows x 4 sums, then 128 x (m, l).
+  static constexpr int kPiece = 128 * (D + 2);              // floats
+};
+
+// 2^k as F16 bits, k <= 0 (0 where F16 has no such value).
+__device__ __forceinline__ uint32_t half_power(int k) {
+  return k >= -14 ? static_cast<uint32_t>(k + 15) << 10 : k >= -24 ? 1u << (k + 24) : 0u;
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <int D, bool SHARED>
+__global__ void __launch_bounds__(kThreads, 1)
+    kv8_tile_kernel(const Kv8AttnArgs a, int group, int tile_from, float* partial) {
+  using T = Tile<D, SHARED>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  __shared__ uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2],
+      o_done[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int found[2];             // row, tile in the row
+  // By key tile: E of its K, whether a page is missing, and each key's 2^ev
+  // (0 where there is no key).  A tile's entry is rewritten four tiles later,
+  // when its weights are long done.
+  __shared__ volatile int exps[4][2];
+  __shared__ __align__(16) float value_scale[4][kKeys];
+  __shared__ int warp_exps[2][4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kCta = T::kQueries * kRows;  // columns of a CTA
+
+  griddep_enter();
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, kSoftmax);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], 128);
+      mbar_init(&v_full[s], 128);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_empty[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 128);
+      mbar_init(&o_done[s], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    // The row of this CTA's tile; late tiles, which have the most keys, go first.
+    const int want = static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x);
+    int row = -1, before = 0;
+    for (int base = 0; base < a.rows && row < 0; base += 32) {
+      const int r = base + lane;
+      int incl = r < a.rows
+                     ? kv8_row(a, r, group, kCta, tile_from, blockIdx.x + blockIdx.y + blockIdx.z == 0,
+                               true).chunks
+                     : 0;
+      const int own = incl;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > want);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        row = base + src;
+        before += __shfl_sync(0xffffffffu, incl - own, src);
+      } else {
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+    if (lane == 0) {
+      found[0] = row;
+      found[1] = want - before;
+    }
+  }
+  __syncthreads();
+  const int row = found[0];
+  if (row < 0) return;  // the whole CTA: fewer tiles than the grid has room for
+  if (warp == 12) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  const Kv8Row x = kv8_row(a, row, group, kCta, tile_from, false, true);
+  const int kvh = blockIdx.y, hkv = a.cache.hkv;
+  const int x0 = found[1] * kCta, cols = x.count * group;
+  const int past = x.len - x.count;  // position of the row's first new token
+  // Keys that the CTA's last column sees, and this split's share of their tiles.
+  const int last_token = (min(x0 + kCta, cols) - 1) / group;
+  const int keys = max(0, past + last_token + 1);
+  const int all = (keys + kKeys - 1) / kKeys;
+  const int kt0 = static_cast<int>(static_cast<long long>(all) * blockIdx.z / gridDim.z);
+  const int n = static_cast<int>(static_cast<long long>(all) * (blockIdx.z + 1) / gridDim.z) - kt0;
+
+  // 512 threads x 128 registers: the softmax takes from the other two groups
+  // (256 x 168 + 128 x 120 + 128 x 56 = 65536).
+  if (warp >= 12) {
+    // ---------------------------------------------------------------- products
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 12 && lane == 0 && n > 0) {
+      constexpr uint32_t idesc_s = umma_idesc(kRows, kKeys, 0);
+      constexpr uint32_t idesc_pv = umma_idesc(kRows, D, 0) | (1u << 16);  // V: MN-major
+      const uint32_t base = smem_u32(smem);
+      // A descriptor's address field counts 16 bytes: offsets are added to it.
+      auto scores = [&](int t, int g) {  // S of group g on key tile t
+        const uint64_t qd = sw128_desc(base + T::kQ + (SHARED ? g * T::kOperand : 0u));
+        const uint64_t kd = sw128_desc(base + T::kK + (t & 1) * T::kOperand);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * T::kAtom + (kk & 3) * 32) >> 4;
+          umma_f16(tmem + T::kTmemS + g * 128, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[g]);
+      };
+      auto sums = [&](int t, int g, bool first) {  // O of group g += P V
+        const uint64_t vd = sw128_desc_mn(base + T::kV + (t & 1) * T::kOperand, T::kAtom);
+#pragma unroll
+        for (int ks = 0; ks < kKeys / 16; ++ks)
+          umma_f16_ta(tmem + T::kTmemO + g * 128, tmem + T::kTmemS + g * 128 + ks * 8,
+                      vd + ks * (2048 >> 4), idesc_pv, !first || ks > 0 ? 1u : 0u);
+        umma_commit(&o_done[g]);
+      };
+      auto wait = [&](uint64_t* bar, int use) {
+        const bool ok = mbar_wait(bar, use & 1, a.status);
+        tc_fence_after();
+        return ok;
+      };
+      bool ok = wait(&q_full, 0);
+      if (SHARED) {
+        ok = ok && wait(&k_full[0], 0);
+        if (ok) {
+          scores(0, 0);
+          scores(0, 1);
+          umma_commit(&k_empty[0]);
+        }
+        for (int i = 0; ok && i < n; ++i) {
+          const int u = (i + 1) >> 1;  // use of the stage of key tile i + 1
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            ok = ok && wait(&p_full[g], i);
+            if (g == 0) ok = ok && wait(&v_full[i & 1], i >> 1);
+            if (!ok) break;
+            sums(i, g, i == 0);
+            if (g == 1) umma_commit(&v_empty[i & 1]);
+            if (i + 1 < n) {
+              if (g == 0) ok = wait(&k_full[(i + 1) & 1], u);
+              if (!ok) break;
+              scores(i + 1, g);
+              if (g == 1) umma_commit(&k_empty[(i + 1) & 1]);
+            }
+          }
+        }
+      } else {
+        for (int t = 0; ok && t < 2 && t < n; ++t) {
+          ok = wait(&k_full[t], 0);
+          if (!ok) break;
+          scores(t, t);
+          umma_commit(&k_empty[t]);
+        }
+        for (int t = 0; ok && t < n; ++t) {
+          const int g = t & 1;
+          ok = wait(&p_full[g], t >> 1) && wait(&v_full[g], t >> 1);
+          if (!ok) break;
+          sums(t, g, t < 2);
+          umma_commit(&v_empty[g]);
+          if (t + 2 < n) {
+            ok = wait(&k_full[g], (t + 2) >> 1);
+            if (!ok) break;
+            scores(t + 2, g);
+            umma_commit(&k_empty[g]);
+          }
+        }
+      }
+    }
+  } else if (warp >= 8) {
+    // ---------------------------------------------------------------- converters
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+    constexpr int kChunks = D / 16;           // 16-byte chunks of a row's codes
+    constexpr int kPass = 128 / kChunks;      // rows that the 128 threads take at once
+    constexpr int kPasses = kKeys / kPass;
+    const int tid = threadIdx.x - kSoftmax, cw = warp - 8;
+    const int chunk = tid % kChunks, prow = tid / kChunks;
+    const int32_t* table = a.tables + static_cast<size_t>(row) * a.max_blocks;
+    uint4 kc[kPasses], vc[kPasses];
+    uint32_t scales[kPasses];  // bytes: K's, V's << 8
+    int page[kPasses] = {};    // block of this thread's row of pass p; -1: no key
+    auto codes_of = [&](int p) {  // offset of its codes
+      return ((static_cast<size_t>(page[p]) * hkv + kvh) * kKv8Page + (p * kPass + prow) % kKv8Page);
+    };
+    auto load_k = [&](int t) {
+      const int key0 = (kt0 + t) * kKeys;
+      int id = -1;
+      if (lane < 8 && key0 + lane * kKv8Page < keys) {
+        id = __ldg(table + (key0 / kKv8Page + lane));  // below max_blocks: keys <= its length
+        if (id < 0 || id >= a.cache.blocks) {
+          atomicOr(a.status, kDevBadIndex);
+          id = -1;
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        const int r = p * kPass + prow;
+        const int b = __shfl_sync(0xffffffffu, id, r / kKv8Page);
+        page[p] = key0 + r < keys ? b : -1;
+        kc[p] = make_uint4(0u, 0u, 0u, 0u);
+        scales[p] = 0u;
+        if (page[p] >= 0) {
+          const size_t at = codes_of(p);
+          kc[p] = __ldg(reinterpret_cast<const uint4*>(a.cache.k + at * D + chunk * 16));
+          scales[p] = __ldg(a.cache.k_scale + at) | static_cast<uint32_t>(__ldg(a.cache.v_scale + at)) << 8;
+        }
+      }
+    };
+    // 16 codes, times a factor where they are scaled, as two swizzled 16-byte
+    // chunks of F16.
+    auto store = [&](uint8_t* dst, int p, const uint4& c, auto scaled, uint32_t factor) {
+      const int r = p * kPass + prow;
+      const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+      uint32_t h[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        h[2 * j] = kv8_half2_lo(w[j]);
+        h[2 * j + 1] = kv8_half2_hi(w[j]);
+        if (decltype(scaled)::value) {
+          h[2 * j] = mul2(h[2 * j], factor);
+          h[2 * j + 1] = mul2(h[2 * j + 1], factor);
+        }
+      }
+      // The upper half of a row's lanes stores its second chunk first: eight
+      // lanes then reach eight different groups of banks.
+      const int flip = chunk >> 2 & 1;
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        const int which = o ^ flip;
+        const int c16 = chunk * 2 + which;
+        uint8_t* to = dst + (c16 >> 3) * T::kAtom + r * 128 + (((c16 & 7) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(to) = which ? make_uint4(h[4], h[5], h[6], h[7])
+                                              : make_uint4(h[0], h[1], h[2], h[3]);
+      }
+    };
+    bool ok = true;
+    if (n > 0) load_k(0);
+    for (int t = 0; t <= n; ++t) {
+      if (t < n) {
+        int ek = -128;
+        bool hole = false;
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+          const int r = p * kPass + prow;
+          if (page[p] >= 0) ek = max(ek, static_cast<int>(scales[p] & 255u) - 127);
+          else hole |= (kt0 + t) * kKeys + r < keys;
+          if (chunk == 0) value_scale[t & 3][r] = page[p] >= 0 ? kv8_scale(scales[p] >> 8) : 0.f;
+        }
+        ek = __reduce_max_sync(0xffffffffu, ek);
+        hole = __any_sync(0xffffffffu, hole);
+        if (lane == 0) warp_exps[t & 1][cw] = ek * 2 + (hole ? 1 : 0);
+        named_bar_sync(3, 128);
+        hole = false;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          ek = max(ek, warp_exps[t & 1][w] >> 1);
+          hole |= warp_exps[t & 1][w] & 1;
+        }
+        if (ek == -128) ek = 0;  // no key here
+        if (tid == 0) {
+          exps[t & 3][0] = ek;
+          exps[t & 3][1] = hole;
+        }
+        if (t >= 2) ok = mbar_wait(&k_empty[t & 1], ((t - 2) >> 1) & 1, a.status);
+        if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+          const uint32_t f = half_power(static_cast<int>(scales[p] & 255u) - 127 - ek);
+          store(smem + T::kK + (t & 1) * T::kOperand, p, kc[p], std::true_type{}, f | f << 16);
+        }
+        fence_proxy_async();
+        mbar_arrive(&k_full[t & 1]);
+      }
+      if (t >= 1) {
+        const int v = t - 1;
+        if (v >= 2) ok = mbar_wait(&v_empty[v & 1], ((v - 2) >> 1) & 1, a.status);
+        if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p)
+          store(smem + T::kV + (v & 1) * T::kOperand, p, vc[p], std::false_type{}, 0u);
+        fence_proxy_async();
+        mbar_arrive(&v_full[v & 1]);
+      }
+      if (t < n) {
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+          vc[p] = make_uint4(0u, 0u, 0u, 0u);
+          if (page[p] >= 0)
+            vc[p] = __ldg(reinterpret_cast<const uint4*>(a.cache.v + codes_of(p) * D + chunk * 16));
+        }
+        if (t + 1 < n) load_k(t + 1);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    const int g = warp >> 2, tid = threadIdx.x & 127;  // group, row (TMEM lane)
+    // Queries into shared memory: 16-byte chunks, swizzled.
+    {
+      constexpr int kChunks = D / 8;
+      const int who = SHARED ? tid : threadIdx.x, step = SHARED ? 128 : kSoftmax;
+      const int c0 = x0 + (SHARED ? g * kRows : 0);
+      uint8_t* dst = smem + T::kQ + (SHARED ? g * T::kOperand : 0u);
+      for (int i = who; i < kRows * kChunks; i += step) {
+        const int r = i / kChunks, c = i % kChunks, col = c0 + r;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (col < cols)
+          v = __ldg(reinterpret_cast<const uint4*>(
+              a.q + static_cast<size_t>(x.t0 + col / group) * a.ld_q +
+              static_cast<size_t>(kvh * group + col % group) * D + c * 8));
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * T::kAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+      }
+      fence_proxy_async();
+      mbar_arrive(&q_full);
+    }
+    const int col = x0 + (SHARED ? g * kRows : 0) + tid;
+    const int lim = col < cols ? min(past + col / group, keys - 1) : -1;  // last key seen
+    const float sl2 = a.scale * kLog2e;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t sa = lanes + T::kTmemS + g * 128, oa = lanes + T::kTmemO + g * 128;
+    float m = kNoReference, l = 0.f;
+    bool ok = true;
+    const int mine = SHARED ? n : (n + 1 - g) >> 1;  // key tiles of this group
+    for (int j = 0; j < mine; ++j) {
+      const int t = SHARED ? j : 2 * j + g;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[g], j & 1, a.status));
+      if (!ok) break;
+      tc_fence_after();
+      const float f = sl2 * __uint_as_float(static_cast<uint32_t>(exps[t & 3][0] + 127) << 23);
+      const int seen = lim - (kt0 + t) * kKeys;  // keys 0 .. seen of the tile
+      const bool full = __all_sync(0xffffffffu, seen >= kKeys - 1) && !exps[t & 3][1];
+      const float4* vs = reinterpret_cast<const float4*>(value_scale[t & 3]);
+      float alpha = 1.f;
+      // The largest weight of the row becomes 1.
+      auto raise = [&]() {
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < kKeys; c += 16) {
+          uint32_t v[16];
+          tmem_ld16_nowait(sa + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t b = __float_as_uint(value_scale[t & 3][c + i]);
+            if (c + i <= seen && b)
+              mx = fmaxf(mx, fmaf(__uint_as_float(v[i]), f, static_cast<float>(static_cast<int>(b >> 23) - 127)));
+          }
+        }
+        if (mx > m + kLazy) {
+          alpha *= ex2(m - mx);
+          m = mx;
+        }
+      };
+      uint32_t pk[64];
+      float rs;
+      auto weights = [&](auto masked) {
+        float s0 = 0.f, s1 = 0.f, top = 0.f;
+        uint32_t v[2][16];
+        tmem_ld16_nowait(sa, v[0]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          tmem_ld_wait();
+          if (c < 7) tmem_ld16_nowait(sa + (c + 1) * 16, v[(c + 1) & 1]);
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const float4 sc = vs[c * 4 + (i >> 2)];
+            const float scale[4] = {sc.x, sc.y, sc.z, sc.w};
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float y = fmaf(__uint_as_float(v[c & 1][i + e]), f, -m);
+              if (decltype(masked)::value)
+                if (c * 16 + i + e > seen || scale[e] == 0.f) y = -INFINITY;
+              const float w = ex2(y);
+              if (e & 1) s1 += w;
+              else s0 += w;
+              p[e] = w * scale[e];
+            }
+            top = fmaxf(top, fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])));
+            pk[c * 8 + (i >> 1)] = half2_bits(p[0], p[1]);
+            pk[c * 8 + (i >> 1) + 1] = half2_bits(p[2], p[3]);
+          }
+        }
+        rs = s0 + s1;
+        return top;
+      };
+      if (j == 0) raise();
+      for (bool raised = false;; raised = true) {
+        const float top = full ? weights(std::false_type{}) : weights(std::true_type{});
+        if (raised || !__any_sync(0xffffffffu, top > kMostWeight)) break;
+        raise();
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w[i] = pk[h * 32 + i];
+        tmem_st32(sa + h * 32, w);
+      }
+      l = l * alpha + rs;
+      // O was summed to another reference: bring it to the new one.
+      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[g], (j - 1) & 1, a.status));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32];
+          tmem_ld32_nowait(oa + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+          tmem_st32(oa + c, v);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&p_full[g]);
+    }
+    if (ok && mine > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&o_done[g], (mine - 1) & 1, a.status));
+      tc_fence_after();
+    }
+    // Row sums of O, 32 dimensions at a time; zeros where this group had no key tile.
+    auto load_o = [&](int c, float (&v)[32]) {
+      uint32_t w[32];
+      if (mine > 0) {
+        tmem_ld32_nowait(oa + c, w);
+        tmem_ld_wait();
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = mine > 0 ? __uint_as_float(w[i]) : 0.f;
+    };
+    float4* half = reinterpret_cast<float4*>(smem + T::kK);  // K and V are done with
+    float2* half_ml = reinterpret_cast<float2*>(half + 128 * (D / 4));
+    float wo = 1.f, wh = 0.f;  // weights of this group's sums and of the other's
+    if (!SHARED) {
+      // Group 1's half goes through shared memory to group 0, once both
+      // groups' products are done.
+      if (g == 1 && ok && n > 0)
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[0], (((n + 1) >> 1) - 1) & 1, a.status));
+      if (g == 1 && ok) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float v[32];
+          load_o(c, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            half[(c / 4 + i) * 128 + tid] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+        half_ml[tid] = make_float2(m, l);
+      }
+      ok = named_bar_all(1, kSoftmax, ok);
+      if (g == 0 && ok && n > 1) {
+        const float2 o = half_ml[tid];
+        const float mm = fmaxf(m, o.x);
+        wo = ex2(m - mm);
+        wh = ex2(o.x - mm);
+        l = l * wo + o.y * wh;
+        m = mm;
+      }
+    }
+    if (ok && (SHARED || g == 0)) {
+      const bool split = gridDim.z > 1;
+      const size_t cell = (static_cast<size_t>(gridDim.x - 1 - blockIdx.x) * hkv + kvh) * gridDim.z +
+                          blockIdx.z;
+      float4* piece = reinterpret_cast<float4*>(partial + cell * T::kPiece);
+      const float inv = 1.f / l;
+      __half* out = col < cols ? a.out + static_cast<size_t>(x.t0 + col / group) * a.ld_out +
+                                     static_cast<size_t>(kvh * group + col % group) * D
+                               : nullptr;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        float v[32];
+        load_o(c, v);
+        if (!SHARED && n > 1) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 o = half[(c / 4 + i) * 128 + tid];
+            v[4 * i] = v[4 * i] * wo + o.x * wh;
+            v[4 * i + 1] = v[4 * i + 1] * wo + o.y * wh;
+            v[4 * i + 2] = v[4 * i + 2] * wo + o.z * wh;
+            v[4 * i + 3] = v[4 * i + 3] * wo + o.w * wh;
+          }
+        }
+        if (!SHARED && split) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            piece[(c / 4 + i) * 128 + tid] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        } else if (out) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              h[k] = lim < 0 ? 0u : half2_bits(v[8 * i + 2 * k] * inv, v[8 * i + 2 * k + 1] * inv);
+            *reinterpret_cast<uint4*>(out + c + 8 * i) = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+        }
+      }
+      if (!SHARED && split)
+        reinterpret_cast<float2*>(piece + 128 * (D / 4))[tid] = make_float2(m, l);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// Joins the key splits of a query tile in order: one CTA a tile and kv head.
+template <int D>
+__global__ void __launch_bounds__(256)
+    kv8_tile_join_kernel(const Kv8AttnArgs a, int group, int tile_from, const float* partial, int splits) {
+  using T = Tile<D, false>;
+  __shared__ int found[2];
+  griddep_enter();
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {
+    const int want = blockIdx.x;
+    int row = -1, before = 0;
+    for (int base = 0; base < a.rows && row < 0; base += 32) {
+      const int r = base + lane;
+      int incl = r < a.rows ? kv8_row(a, r, group, kRows, tile_from, false, true).chunks : 0;
+      const int own = incl;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > want);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        row = base + src;
+        before += __shfl_sync(0xffffffffu, incl - own, src);
+      } else {
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+    if (lane == 0) {
+      found[0] = row;
+      found[1] = want - before;
+    }
+  }
+  __syncthreads();
+  if (found[0] < 0) return;
+  const Kv8Row x = kv8_row(a, found[0], group, kRows, tile_from, false, true);
+  const int kvh = blockIdx.y, x0 = found[1] * kRows, cols = x.count * group;
+  const float4* base = reinterpret_cast<const float4*>(
+      partial + (static_cast<size_t>(blockIdx.x) * a.cache.hkv + kvh) * splits * T::kPiece);
+  // A thread takes one row's eight dimensions.
+  for (int u = threadIdx.x; u < kRows * (D / 8); u += 256) {
+    const int r = u % kRows, d8 = u / kRows, col = x0 + r;
+    if (col >= cols) continue;
+    auto ml_of = [&](int s) {
+      return __ldcg(reinterpret_cast<const float2*>(base + static_cast<size_t>(s) * (T::kPiece / 4) +
+                                                    128 * (D / 4)) + r);
+    };
+    float m = kNoReference;
+    for (int s = 0; s < splits; ++s) m = fmaxf(m, ml_of(s).x);
+    float l = 0.f;
+    float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+    for (int s = 0; s < splits; ++s) {
+      const float4* piece = base + static_cast<size_t>(s) * (T::kPiece / 4);
+      const float2 ml = ml_of(s);
+      const float w = ex2(ml.x - m);
+      l += ml.y * w;
+      const float4 v0 = __ldcg(piece + (d8 * 2) * 128 + r), v1 = __ldcg(piece + (d8 * 2 + 1) * 128 + r);
+      lo.x += v0.x * w;
+      lo.y += v0.y * w;
+      lo.z += v0.z * w;
+      lo.w += v0.w * w;
+      hi.x += v1.x * w;
+      hi.y += v1.y * w;
+      hi.z += v1.z * w;
+      hi.w += v1.w * w;
+    }
+    const bool none = x.len - x.count + col / group < 0;
+    const float inv = 1.f / l;
+    uint4 o = make_uint4(0u, 0u, 0u, 0u);
+    if (!none)
+      o = make_uint4(half2_bits(lo.x * inv, lo.y * inv), half2_bits(lo.z * inv, lo.w * inv),
+                     half2_bits(hi.x * inv, hi.y * inv), half2_bits(hi.z * inv, hi.w * inv));
+    *reinterpret_cast<uint4*>(a.out + static_cast<size_t>(x.t0 + col / group) * a.ld_out +
+                              static_cast<size_t>(kvh * group + col % group) * D + d8 * 8) = o;
+  }
+}
+
+// The most query tiles of `columns` columns that the batch's rows can have.
+long long most_tiles(int rows, int tokens, int group, int columns) {
+  return static_cast<long long>(tokens) * group / columns + std::min(rows, tokens);
+}
+
+struct Plan {
+  bool shared;
+  int tiles, splits;
+};
+constexpr int kMostSplits = 8;
+Plan plan_tiles(int rows, int tokens, int hq, int hkv, int sm_count) {
+  const int group = hq / hkv;
+  // Two query tiles a CTA halve the conversions; worth it from two waves on.
+  const long long single = most_tiles(rows, tokens, group, kRows);
+  Plan p{};
+  p.shared = static_cast<long long>(tokens) * group / kRows * hkv >= 2LL * sm_count;
+  p.tiles = static_cast<int>(p.shared ? most_tiles(rows, tokens, group, 2 * kRows) : single);
+  p.splits = p.shared ? 1
+                      : static_cast<int>(std::max(1LL, std::min<long long>(kMostSplits, sm_count / std::max(1LL, single * hkv))));
+  return p;
+}
+
+template <int D, bool SHARED>
+cudaError_t launch_tile(const Kv8AttnArgs& a, const Plan& p, int tile_from, float* partial,
+                        cudaStream_t stream) {
+  using T = Tile<D, SHARED>;
+  static Kv8Configured configured;
+  const cudaError_t e = configured.once(kv8_tile_kernel<D, SHARED>, static_cast<int>(T::kSmem), 128);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(kv8_tile_kernel<D, SHARED>, dim3(p.tiles, a.cache.hkv, p.splits), dim3(kThreads),
+                          T::kSmem, stream, a, a.hq / a.cache.hkv, tile_from, partial);
+}
+
+}  // namespace
+
+bool kv8_tile_supported(int dim) { return dim == 64 || dim == 128; }
+
+size_t kv8_tile_workspace(int rows, int tokens, int hq, int hkv, int dim, int sm_count) {
+  const Plan p = plan_tiles(rows, tokens, hq, hkv, sm_count);
+  return p.splits == 1 ? 0
+                       : static_cast<size_t>(p.tiles) * hkv * p.splits * 128 * (dim + 2) * sizeof(float);
+}
+
+cudaError_t kv8_tile_launch(const Kv8AttnArgs& a, int tile_from, float* partial, cudaStream_t stream) {
+  const Plan p = plan_tiles(a.rows, a.tokens, a.hq, a.cache.hkv, a.sm_count);
+  if (a.cache.dim == 64)
+    return p.shared ? launch_tile<64, true>(a, p, tile_from, partial, stream)
+                    : launch_tile<64, false>(a, p, tile_from, partial, stream);
+  return p.shared ? launch_tile<128, true>(a, p, tile_from, partial, stream)
+                  : launch_tile<128, false>(a, p, tile_from, partial, stream);
+}
+
+cudaError_t kv8_tile_join_launch(const Kv8AttnArgs& a, int tile_from, const float* partial,
+                                 cudaStream_t stream) {
+  const Plan p = plan_tiles(a.rows, a.tokens, a.hq, a.cache.hkv, a.sm_count);
+  if (p.splits == 1) return cudaSuccess;
+  const dim3 grid(p.tiles, a.cache.hkv);
+  const int group = a.hq / a.cache.hkv;
+  return a.cache.dim == 64 ? launch_dependent(kv8_tile_join_kernel<64>, grid, dim3(256), 0, stream, a,
+                                              group, tile_from, partial, p.splits)
+                           : launch_dependent(kv8_tile_join_kernel<128>, grid, dim3(256), 0, stream, a,
+                                              group, tile_from, partial, p.splits);
+}
+
+}  // namespace hb
