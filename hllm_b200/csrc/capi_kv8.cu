@@ -47,8 +47,9 @@ const char* cache_fault(const hllm_b200_kv8* c) {
   if (c->head_dim == 0 || c->head_dim % 32 != 0 || c->head_dim > hb::kKv8MaxDim)
     return "8-bit KV cache: head_dim must be a multiple of 32, at most 256";
   if (c->kv_heads == 0 || c->kv_heads > 65535) return "8-bit KV cache: bad kv_heads";
-  if (c->blocks == 0 || c->blocks > kMaxInt / hb::kKv8Page)
-    return "8-bit KV cache: blocks x 16 must be 1 to 2^31 - 1";
+  if (c->blocks == 0 || c->blocks > kMaxInt / hb::kKv8Page ||
+      c->blocks * c->kv_heads > kMaxInt)
+    return "8-bit KV cache: blocks x 16 and blocks x kv_heads must be 1 to 2^31 - 1";
   return nullptr;
 }
 

@@ -96,21 +96,15 @@ size_t kv8_attention_workspace(int rows, int tokens, int max_row_tokens, int hq,
 cudaError_t kv8_attention_launch(const Kv8AttnArgs& a, cudaStream_t stream);
 
 #ifdef __CUDACC__
-// A kernel's dynamic shared memory limit, raised once a device.  `registers`:
-// refused with fewer registers a thread, for a kernel that moves registers
-// between its warps and would wait for ever for those it was not launched with.
+// A kernel's dynamic shared memory limit, raised once a device.
 struct Kv8Configured {
   std::atomic<bool> done[64] = {};
   template <typename K>
-  cudaError_t once(K kernel, int bytes, int registers = 0) {
+  cudaError_t once(K kernel, int bytes) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 64 && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
-    cudaFuncAttributes f{};
-    e = cudaFuncGetAttributes(&f, kernel);
-    if (e != cudaSuccess) return e;
-    if (f.numRegs < registers) return cudaErrorInvalidConfiguration;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_relaxed);
     return e;

@@ -28,10 +28,7 @@
 // With s_j the score in log2 and ev_j the exponent of value row j, a row keeps
 // one reference m for  l = sum 2^(s_j - m)  and  O = sum (2^(s_j - m) 2^ev_j) d_j,
 // d_j the codes: the weights in brackets are what F16 has to hold, so m follows
-// max (s_j + ev_j), and o = O / l.  Each group computes a key tile's weights
-// against the reference it has, in one pass over the scores, and only where a
-// weight passes 2^8 (first tiles, mostly) goes back for the maximum.  Every
-// wait is bounded (common.cuh).
+// max (s_j + ev_j), lazily, and o = O / l.  Every wait is bounded (common.cuh).
 #include <algorithm>
 #include <type_traits>
 
@@ -44,8 +41,7 @@ namespace {
 constexpr int kKeys = 128;       // keys of a tile
 constexpr int kRows = 128;       // columns of a query tile
 constexpr int kSoftmax = 256;    // threads of the softmax groups
-constexpr int kThreads = kSoftmax + 128 + 128;  // the last warps but one idle: registers go by four warps
-constexpr float kMostWeight = 256.f;              // 2^kLazy
+constexpr int kThreads = kSoftmax + 128 + 32;
 
 // D[tmem] (+)= A[tmem] * B[smem desc]: A is F16 pairs, a row per lane.
 __device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
@@ -57,15 +53,41 @@ __device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, ui
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// 32 lanes x 32 bits, 16 consecutive columns a thread, without the wait.
-__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
+// Two F32 operations an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)),
+        "l"(reinterpret_cast<const unsigned long long&>(b)),
+        "l"(reinterpret_cast<const unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2f(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)),
+        "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add2f(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)),
+        "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return d;
+}
+
+// 16 consecutive columns of a thread's lane.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32"
-      " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+      " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 
 template <int D, bool SHARED>
@@ -81,13 +103,72 @@ struct Tile {
   static constexpr int kPiece = 128 * (D + 2);              // floats
 };
 
-// 2^k as F16 bits, k <= 0 (0 where F16 has no such value).
-__device__ __forceinline__ uint32_t half_power(int k) {
-  return k >= -14 ? static_cast<uint32_t>(k + 15) << 10 : k >= -24 ? 1u << (k + 24) : 0u;
+// Loads that leave zeros where !live, without a branch, so that a run of them
+// is in flight together.
+__device__ __forceinline__ uint2 load8_if(const void* p, bool live) {
+  uint2 v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t"
+      "@p ld.global.nc.v2.u32 {%0, %1}, [%2];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y)
+      : "l"(p), "r"(static_cast<uint32_t>(live)));
+  return v;
+}
+__device__ __forceinline__ uint32_t load_byte_if(const uint8_t* p, bool live) {
+  uint32_t v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t"
+      "@p ld.global.nc.u8 %0, [%1];\n\t}"
+      : "=&r"(v)
+      : "l"(p), "r"(static_cast<uint32_t>(live)));
+  return v;
+}
+
+// 2^(k - 127), at most 1, in both halves of a word (0 where F16 has no such value).
+__device__ __forceinline__ uint32_t half_power2(int k) {
+  const float f = __uint_as_float(static_cast<uint32_t>(max(k, 0)) << 23);
+  return half2_bits(f, f);
 }
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// A converter thread's codes of a tile: eight of each 64 dimensions of its row
+// of each page, `pages` (pool page of this kv head, -1: none) being in the first
+// eight lanes; zeros past the last key.
+template <int D>
+__device__ __forceinline__ void load_codes(uint2 (&c)[kKeys / kKv8Page * (D / 64)], const uint8_t* pool,
+                                           int pages, int left) {
+  constexpr int kPages = kKeys / kKv8Page, kHalves = D / 64;
+  int page[kPages];
+#pragma unroll
+  for (int p = 0; p < kPages; ++p) page[p] = __shfl_sync(0xffffffffu, pages, p);
+#pragma unroll
+  for (int p = 0; p < kPages; ++p) {
+    const bool live = page[p] >= 0 && p * kKv8Page < left;
+    const uint8_t* at = pool + static_cast<uint64_t>(static_cast<uint32_t>(page[p])) * (kKv8Page * D);
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) c[p * kHalves + h] = load8_if(at + h * 64, live);
+  }
+}
+// Eight codes of each 64 dimensions as swizzled 16-byte chunks of F16, times a
+// factor where they are scaled.
+template <int D, bool SCALED>
+__device__ __forceinline__ void store_codes(uint8_t* dst, int r, int chunk, const uint2* c,
+                                            uint32_t factor) {
+#pragma unroll
+  for (int h = 0; h < D / 64; ++h) {
+    uint32_t f[4] = {kv8_half2_lo(c[h].x), kv8_half2_hi(c[h].x), kv8_half2_lo(c[h].y),
+                     kv8_half2_hi(c[h].y)};
+    if (SCALED) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = mul2(f[j], factor);
+    }
+    *reinterpret_cast<uint4*>(dst + h * 128 * 128 + r * 128 + ((chunk ^ (r & 7)) << 4)) =
+        make_uint4(f[0], f[1], f[2], f[3]);
+  }
 }
 
 template <int D, bool SHARED>
@@ -101,12 +182,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       o_done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int found[2];             // row, tile in the row
-  // By key tile: E of its K, whether a page is missing, and each key's 2^ev
+  // By key tile: E + 127 of its K, whether a page is missing, and each key's 2^ev
   // (0 where there is no key).  A tile's entry is rewritten four tiles later,
   // when its weights are long done.
   __shared__ volatile int exps[4][2];
-  __shared__ __align__(16) float value_scale[4][kKeys];
+  __shared__ __align__(16) float value_scale[4][2 * kKeys];  // 2^ev, then ev (-inf: no key)
   __shared__ int warp_exps[2][4];
+  __shared__ uint8_t key_scale[2][kKeys];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kCta = T::kQueries * kRows;  // columns of a CTA
 
@@ -177,12 +259,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int kt0 = static_cast<int>(static_cast<long long>(all) * blockIdx.z / gridDim.z);
   const int n = static_cast<int>(static_cast<long long>(all) * (blockIdx.z + 1) / gridDim.z) - kt0;
 
-  // 512 threads x 128 registers: the softmax takes from the other two groups
-  // (256 x 168 + 128 x 120 + 128 x 56 = 65536).
-  if (warp >= 12) {
+  if (warp == 12) {
     // ---------------------------------------------------------------- products
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 12 && lane == 0 && n > 0) {
+    if (lane == 0 && n > 0) {
       constexpr uint32_t idesc_s = umma_idesc(kRows, kKeys, 0);
       constexpr uint32_t idesc_pv = umma_idesc(kRows, D, 0) | (1u << 16);  // V: MN-major
       const uint32_t base = smem_u32(smem);
@@ -259,131 +338,94 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 8) {
     // ---------------------------------------------------------------- converters
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
-    constexpr int kChunks = D / 16;           // 16-byte chunks of a row's codes
-    constexpr int kPass = 128 / kChunks;      // rows that the 128 threads take at once
-    constexpr int kPasses = kKeys / kPass;
+    // A page at a time: eight threads a row, eight codes of each 64 dimensions a
+    // thread, which are one 16-byte chunk of F16; the eight chunks of a row's 64
+    // dimensions reach eight different groups of banks.
+    constexpr int kPages = kKeys / kKv8Page, kHalves = D / 64;
     const int tid = threadIdx.x - kSoftmax, cw = warp - 8;
-    const int chunk = tid % kChunks, prow = tid / kChunks;
+    const int chunk = tid & 7, prow = tid >> 3;
     const int32_t* table = a.tables + static_cast<size_t>(row) * a.max_blocks;
-    uint4 kc[kPasses], vc[kPasses];
-    uint32_t scales[kPasses];  // bytes: K's, V's << 8
-    int page[kPasses] = {};    // block of this thread's row of pass p; -1: no key
-    auto codes_of = [&](int p) {  // offset of its codes
-      return ((static_cast<size_t>(page[p]) * hkv + kvh) * kKv8Page + (p * kPass + prow) % kKv8Page);
+    const uint32_t code_at = prow * D + chunk * 8;  // in a page's codes
+    uint2 kc[kPages * kHalves], vc[kPages * kHalves];
+    // The tile's pages of this kv head, in the first eight lanes (-1: none).
+    auto load_ids = [&](int t) {
+      const int key = (kt0 + t) * kKeys + lane * kKv8Page;
+      // Below max_blocks: keys is at most the row's length.
+      return t < n && lane < 8 && key < keys ? __ldg(table + key / kKv8Page) : -1;
     };
+    int ids = load_ids(0), kids = -1, vids = -1;  // of the tile to load, and of the loaded K and V
+    uint32_t ks = 0u, vs = 0u;                    // scale bytes of key `tid` of the loaded K
+    bool have = false, hole = false;              // whether that key is there, or should be
+    // This thread's row of page p is a key while 16 p is below this.
+    auto left = [&](int t) { return keys - (kt0 + t) * kKeys - prow; };
     auto load_k = [&](int t) {
       const int key0 = (kt0 + t) * kKeys;
-      int id = -1;
-      if (lane < 8 && key0 + lane * kKv8Page < keys) {
-        id = __ldg(table + (key0 / kKv8Page + lane));  // below max_blocks: keys <= its length
-        if (id < 0 || id >= a.cache.blocks) {
-          atomicOr(a.status, kDevBadIndex);
-          id = -1;
-        }
+      if (lane < 8 && key0 + lane * kKv8Page < keys && (ids < 0 || ids >= a.cache.blocks)) {
+        atomicOr(a.status, kDevBadIndex);
+        ids = -1;
       }
-#pragma unroll
-      for (int p = 0; p < kPasses; ++p) {
-        const int r = p * kPass + prow;
-        const int b = __shfl_sync(0xffffffffu, id, r / kKv8Page);
-        page[p] = key0 + r < keys ? b : -1;
-        kc[p] = make_uint4(0u, 0u, 0u, 0u);
-        scales[p] = 0u;
-        if (page[p] >= 0) {
-          const size_t at = codes_of(p);
-          kc[p] = __ldg(reinterpret_cast<const uint4*>(a.cache.k + at * D + chunk * 16));
-          scales[p] = __ldg(a.cache.k_scale + at) | static_cast<uint32_t>(__ldg(a.cache.v_scale + at)) << 8;
-        }
-      }
+      kids = ids < 0 ? -1 : ids * hkv + kvh;
+      const int page = __shfl_sync(0xffffffffu, kids, tid / kKv8Page);
+      have = page >= 0 && key0 + tid < keys;
+      hole = page < 0 && key0 + tid < keys;
+      const size_t at = static_cast<size_t>(max(page, 0)) * kKv8Page + tid % kKv8Page;
+      ks = load_byte_if(a.cache.k_scale + at, have);
+      vs = load_byte_if(a.cache.v_scale + at, have);
+      load_codes<D>(kc, a.cache.k + code_at, kids, left(t));
+      ids = load_ids(t + 1);  // a tile ahead, so that no load waits for another
     };
-    // 16 codes, times a factor where they are scaled, as two swizzled 16-byte
-    // chunks of F16.
-    auto store = [&](uint8_t* dst, int p, const uint4& c, auto scaled, uint32_t factor) {
-      const int r = p * kPass + prow;
-      const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-      uint32_t h[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        h[2 * j] = kv8_half2_lo(w[j]);
-        h[2 * j + 1] = kv8_half2_hi(w[j]);
-        if (decltype(scaled)::value) {
-          h[2 * j] = mul2(h[2 * j], factor);
-          h[2 * j + 1] = mul2(h[2 * j + 1], factor);
-        }
-      }
-      // The upper half of a row's lanes stores its second chunk first: eight
-      // lanes then reach eight different groups of banks.
-      const int flip = chunk >> 2 & 1;
-#pragma unroll
-      for (int o = 0; o < 2; ++o) {
-        const int which = o ^ flip;
-        const int c16 = chunk * 2 + which;
-        uint8_t* to = dst + (c16 >> 3) * T::kAtom + r * 128 + (((c16 & 7) ^ (r & 7)) << 4);
-        *reinterpret_cast<uint4*>(to) = which ? make_uint4(h[4], h[5], h[6], h[7])
-                                              : make_uint4(h[0], h[1], h[2], h[3]);
-      }
-    };
+    // Codes in flight are the other operand's: K of tile t + 1 is asked for as
+    // soon as K of tile t is stored, and arrives under V of tile t - 1, and so on.
     bool ok = true;
     if (n > 0) load_k(0);
     for (int t = 0; t <= n; ++t) {
       if (t < n) {
-        int ek = -128;
-        bool hole = false;
-#pragma unroll
-        for (int p = 0; p < kPasses; ++p) {
-          const int r = p * kPass + prow;
-          if (page[p] >= 0) ek = max(ek, static_cast<int>(scales[p] & 255u) - 127);
-          else hole |= (kt0 + t) * kKeys + r < keys;
-          if (chunk == 0) value_scale[t & 3][r] = page[p] >= 0 ? kv8_scale(scales[p] >> 8) : 0.f;
-        }
-        ek = __reduce_max_sync(0xffffffffu, ek);
-        hole = __any_sync(0xffffffffu, hole);
-        if (lane == 0) warp_exps[t & 1][cw] = ek * 2 + (hole ? 1 : 0);
+        value_scale[t & 3][tid] = have ? kv8_scale(vs) : 0.f;
+        value_scale[t & 3][kKeys + tid] = have ? static_cast<float>(static_cast<int>(vs) - 127) : -INFINITY;
+        key_scale[t & 1][tid] = static_cast<uint8_t>(ks);
+        // E + 127, so that 0 is no key's.
+        int ek = __reduce_max_sync(0xffffffffu, have ? static_cast<int>(ks) : 0);
+        const bool any_hole = __any_sync(0xffffffffu, hole);
+        if (lane == 0) warp_exps[t & 1][cw] = ek * 2 + (any_hole ? 1 : 0);
         named_bar_sync(3, 128);
-        hole = false;
+        int holes = 0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           ek = max(ek, warp_exps[t & 1][w] >> 1);
-          hole |= warp_exps[t & 1][w] & 1;
+          holes |= warp_exps[t & 1][w] & 1;
         }
-        if (ek == -128) ek = 0;  // no key here
         if (tid == 0) {
-          exps[t & 3][0] = ek;
-          exps[t & 3][1] = hole;
+          exps[t & 3][0] = ek > 0 ? ek : 127;
+          exps[t & 3][1] = holes;
         }
         if (t >= 2) ok = mbar_wait(&k_empty[t & 1], ((t - 2) >> 1) & 1, a.status);
         if (!__all_sync(0xffffffffu, ok)) break;
+        uint32_t factor[kPages];
 #pragma unroll
-        for (int p = 0; p < kPasses; ++p) {
-          const uint32_t f = half_power(static_cast<int>(scales[p] & 255u) - 127 - ek);
-          store(smem + T::kK + (t & 1) * T::kOperand, p, kc[p], std::true_type{}, f | f << 16);
-        }
+        for (int p = 0; p < kPages; ++p)
+          factor[p] = half_power2(static_cast<int>(key_scale[t & 1][p * kKv8Page + prow]) - ek + 127);
+        uint8_t* dst = smem + T::kK + (t & 1) * T::kOperand;
+#pragma unroll
+        for (int p = 0; p < kPages; ++p) store_codes<D, true>(dst, p * kKv8Page + prow, chunk, kc + p * kHalves, factor[p]);
         fence_proxy_async();
         mbar_arrive(&k_full[t & 1]);
       }
+      vids = kids;
+      if (t + 1 < n) load_k(t + 1);
       if (t >= 1) {
         const int v = t - 1;
         if (v >= 2) ok = mbar_wait(&v_empty[v & 1], ((v - 2) >> 1) & 1, a.status);
         if (!__all_sync(0xffffffffu, ok)) break;
+        uint8_t* dst = smem + T::kV + (v & 1) * T::kOperand;
 #pragma unroll
-        for (int p = 0; p < kPasses; ++p)
-          store(smem + T::kV + (v & 1) * T::kOperand, p, vc[p], std::false_type{}, 0u);
+        for (int p = 0; p < kPages; ++p) store_codes<D, false>(dst, p * kKv8Page + prow, chunk, vc + p * kHalves, 0u);
         fence_proxy_async();
         mbar_arrive(&v_full[v & 1]);
       }
-      if (t < n) {
-#pragma unroll
-        for (int p = 0; p < kPasses; ++p) {
-          vc[p] = make_uint4(0u, 0u, 0u, 0u);
-          if (page[p] >= 0)
-            vc[p] = __ldg(reinterpret_cast<const uint4*>(a.cache.v + codes_of(p) * D + chunk * 16));
-        }
-        if (t + 1 < n) load_k(t + 1);
-      }
+      if (t < n) load_codes<D>(vc, a.cache.v + code_at, vids, left(t));
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int g = warp >> 2, tid = threadIdx.x & 127;  // group, row (TMEM lane)
     // Queries into shared memory: 16-byte chunks, swizzled.
     {
@@ -416,77 +458,77 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[g], j & 1, a.status));
       if (!ok) break;
       tc_fence_after();
-      const float f = sl2 * __uint_as_float(static_cast<uint32_t>(exps[t & 3][0] + 127) << 23);
+      const float f = sl2 * __uint_as_float(static_cast<uint32_t>(exps[t & 3][0]) << 23);
       const int seen = lim - (kt0 + t) * kKeys;  // keys 0 .. seen of the tile
       const bool full = __all_sync(0xffffffffu, seen >= kKeys - 1) && !exps[t & 3][1];
       const float4* vs = reinterpret_cast<const float4*>(value_scale[t & 3]);
+      const float2 f2 = make_float2(f, f);
+      auto pair_of = [](uint32_t lo, uint32_t hi) {
+        return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+      };
       float alpha = 1.f;
-      // The largest weight of the row becomes 1.
-      auto raise = [&]() {
-        float mx = -INFINITY;
+      // Two passes over the scores, 32 at a time in a rolled loop: the code of
+      // all roles has to stay in the instruction cache, or the products wait
+      // for their instructions.
+      auto pass = [&](auto masked) {
+        float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll 1
-        for (int c = 0; c < kKeys; c += 16) {
-          uint32_t v[16];
-          tmem_ld16_nowait(sa + c, v);
+        for (int c = 0; c < kKeys; c += 32) {
+          uint32_t v[32];
+          tmem_ld32_nowait(sa + c, v);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint32_t b = __float_as_uint(value_scale[t & 3][c + i]);
-            if (c + i <= seen && b)
-              mx = fmaxf(mx, fmaf(__uint_as_float(v[i]), f, static_cast<float>(static_cast<int>(b >> 23) - 127)));
+          for (int i = 0; i < 32; i += 4) {
+            const float4 ev = vs[kKeys / 4 + (c + i) / 4];
+            float2 y0 = fma2(pair_of(v[i], v[i + 1]), f2, make_float2(ev.x, ev.y));
+            float2 y1 = fma2(pair_of(v[i + 2], v[i + 3]), f2, make_float2(ev.z, ev.w));
+            if (decltype(masked)::value) {
+              if (c + i > seen) y0.x = -INFINITY;
+              if (c + i + 1 > seen) y0.y = -INFINITY;
+              if (c + i + 2 > seen) y1.x = -INFINITY;
+              if (c + i + 3 > seen) y1.y = -INFINITY;
+            }
+            m0 = fmaxf(m0, fmaxf(y0.x, y0.y));
+            m1 = fmaxf(m1, fmaxf(y1.x, y1.y));
           }
         }
+        const float mx = fmaxf(m0, m1);
+        // A reference moves only when a weight would pass 2^8: it becomes the
+        // row's largest so far.
         if (mx > m + kLazy) {
-          alpha *= ex2(m - mx);
+          alpha = ex2(m - mx);
           m = mx;
         }
-      };
-      uint32_t pk[64];
-      float rs;
-      auto weights = [&](auto masked) {
-        float s0 = 0.f, s1 = 0.f, top = 0.f;
-        uint32_t v[2][16];
-        tmem_ld16_nowait(sa, v[0]);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        float2 sum = make_float2(0.f, 0.f);
+        const float2 minus = make_float2(-m, -m);
+#pragma unroll 1
+        for (int c = 0; c < kKeys; c += 32) {
+          uint32_t v[32], pk[16];
+          tmem_ld32_nowait(sa + c, v);
           tmem_ld_wait();
-          if (c < 7) tmem_ld16_nowait(sa + (c + 1) * 16, v[(c + 1) & 1]);
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const float4 sc = vs[c * 4 + (i >> 2)];
-            const float scale[4] = {sc.x, sc.y, sc.z, sc.w};
-            float p[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float y = fmaf(__uint_as_float(v[c & 1][i + e]), f, -m);
-              if (decltype(masked)::value)
-                if (c * 16 + i + e > seen || scale[e] == 0.f) y = -INFINITY;
-              const float w = ex2(y);
-              if (e & 1) s1 += w;
-              else s0 += w;
-              p[e] = w * scale[e];
+          for (int i = 0; i < 32; i += 4) {
+            const float4 sc = vs[(c + i) / 4];
+            float2 y0 = fma2(pair_of(v[i], v[i + 1]), f2, minus);
+            float2 y1 = fma2(pair_of(v[i + 2], v[i + 3]), f2, minus);
+            if (decltype(masked)::value) {
+              if (c + i > seen || sc.x == 0.f) y0.x = -INFINITY;
+              if (c + i + 1 > seen || sc.y == 0.f) y0.y = -INFINITY;
+              if (c + i + 2 > seen || sc.z == 0.f) y1.x = -INFINITY;
+              if (c + i + 3 > seen || sc.w == 0.f) y1.y = -INFINITY;
             }
-            top = fmaxf(top, fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])));
-            pk[c * 8 + (i >> 1)] = half2_bits(p[0], p[1]);
-            pk[c * 8 + (i >> 1) + 1] = half2_bits(p[2], p[3]);
+            const float2 w0 = make_float2(ex2(y0.x), ex2(y0.y)), w1 = make_float2(ex2(y1.x), ex2(y1.y));
+            sum = add2f(sum, add2f(w0, w1));
+            const float2 p0 = mul2f(w0, make_float2(sc.x, sc.y)), p1 = mul2f(w1, make_float2(sc.z, sc.w));
+            pk[i >> 1] = half2_bits(p0.x, p0.y);
+            pk[(i >> 1) + 1] = half2_bits(p1.x, p1.y);
           }
+          // The weights of these 32 keys go over scores that are read already.
+          tmem_st16(sa + c / 2, pk);
         }
-        rs = s0 + s1;
-        return top;
+        return sum.x + sum.y;
       };
-      if (j == 0) raise();
-      for (bool raised = false;; raised = true) {
-        const float top = full ? weights(std::false_type{}) : weights(std::true_type{});
-        if (raised || !__any_sync(0xffffffffu, top > kMostWeight)) break;
-        raise();
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) w[i] = pk[h * 32 + i];
-        tmem_st32(sa + h * 32, w);
-      }
+      const float rs = full ? pass(std::false_type{}) : pass(std::true_type{});
       l = l * alpha + rs;
       // O was summed to another reference: bring it to the new one.
       if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
@@ -703,7 +745,7 @@ cudaError_t launch_tile(const Kv8AttnArgs& a, const Plan& p, int tile_from, floa
                         cudaStream_t stream) {
   using T = Tile<D, SHARED>;
   static Kv8Configured configured;
-  const cudaError_t e = configured.once(kv8_tile_kernel<D, SHARED>, static_cast<int>(T::kSmem), 128);
+  const cudaError_t e = configured.once(kv8_tile_kernel<D, SHARED>, static_cast<int>(T::kSmem));
   if (e != cudaSuccess) return e;
   return launch_dependent(kv8_tile_kernel<D, SHARED>, dim3(p.tiles, a.cache.hkv, p.splits), dim3(kThreads),
                           T::kSmem, stream, a, a.hq / a.cache.hkv, tile_from, partial);
