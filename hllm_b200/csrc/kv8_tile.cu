@@ -7,13 +7,14 @@
 // operations a tile, next to which the codes are few bytes, so the work is to
 // keep the tensor pipe fed while codes become F16 and scores become weights:
 //
-//   warps 8-11  converters: a tile's K and V codes from their pages into
-//               shared memory as swizzled F16 operands.  K rows are code *
-//               2^(e - E) with E the tile's largest exponent, so that F16 holds
-//               rows of any size; what it rounds lies 2^-34 below the largest
-//               row, and E goes into the score scale of the tile.  V rows are
-//               the codes; their scales go into the weights.
-//   warp 12     one thread issues the products.
+//   warps 8-11  converters of K, warps 12-15 of V: a tile's codes from their
+//               pages into shared memory as swizzled F16 operands, the next
+//               tile's loads going out as the registers become free.  K rows
+//               are code * 2^(e - E) with E the tile's largest exponent, so that
+//               F16 holds rows of any size; what it rounds lies 2^-34 below the
+//               largest row, and E goes into the score scale of the tile.  V
+//               rows are the codes; their scales go into the weights.
+//   warp 16     one thread issues the products.
 //   warps 0-7   two softmax groups of 128 threads, one row (TMEM lane) a
 //               thread.  The weights go back into TMEM over the scores they
 //               came from, as F16, and are the A operand of P V from there.
@@ -41,7 +42,7 @@ namespace {
 constexpr int kKeys = 128;       // keys of a tile
 constexpr int kRows = 128;       // columns of a query tile
 constexpr int kSoftmax = 256;    // threads of the softmax groups
-constexpr int kThreads = kSoftmax + 128 + 32;
+constexpr int kThreads = kSoftmax + 256 + 32;
 
 // D[tmem] (+)= A[tmem] * B[smem desc]: A is F16 pairs, a row per lane.
 __device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
@@ -80,14 +81,20 @@ __device__ __forceinline__ float2 add2f(float2 a, float2 b) {
   return d;
 }
 
-// 16 consecutive columns of a thread's lane.
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+// Consecutive columns of a thread's lane: 16 read without the wait, 8 written.
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
-      " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32"
+      " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 template <int D, bool SHARED>
@@ -135,23 +142,16 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// A converter thread's codes of a tile: eight of each 64 dimensions of its row
-// of each page, `pages` (pool page of this kv head, -1: none) being in the first
-// eight lanes; zeros past the last key.
+// A converter thread's codes of one page of a tile, eight of each 64 dimensions
+// of its row; `pages` (pool page of this kv head, -1: none) is in the first
+// lanes; zeros past the last key.
 template <int D>
-__device__ __forceinline__ void load_codes(uint2 (&c)[kKeys / kKv8Page * (D / 64)], const uint8_t* pool,
-                                           int pages, int left) {
-  constexpr int kPages = kKeys / kKv8Page, kHalves = D / 64;
-  int page[kPages];
+__device__ __forceinline__ void load_codes(uint2* c, const uint8_t* pool, int pages, int p, int left) {
+  const int page = __shfl_sync(0xffffffffu, pages, p);
+  const bool live = page >= 0 && p * kKv8Page < left;
+  const uint8_t* at = pool + static_cast<uint64_t>(static_cast<uint32_t>(page)) * (kKv8Page * D);
 #pragma unroll
-  for (int p = 0; p < kPages; ++p) page[p] = __shfl_sync(0xffffffffu, pages, p);
-#pragma unroll
-  for (int p = 0; p < kPages; ++p) {
-    const bool live = page[p] >= 0 && p * kKv8Page < left;
-    const uint8_t* at = pool + static_cast<uint64_t>(static_cast<uint32_t>(page[p])) * (kKv8Page * D);
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) c[p * kHalves + h] = load8_if(at + h * 64, live);
-  }
+  for (int h = 0; h < D / 64; ++h) c[h] = load8_if(at + h * 64, live);
 }
 // Eight codes of each 64 dimensions as swizzled 16-byte chunks of F16, times a
 // factor where they are scaled.
@@ -183,8 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ int found[2];             // row, tile in the row
   // By key tile: E + 127 of its K, whether a page is missing, and each key's 2^ev
-  // (0 where there is no key).  A tile's entry is rewritten four tiles later,
-  // when its weights are long done.
+  // (0 where there is no key).
   __shared__ volatile int exps[4][2];
   __shared__ __align__(16) float value_scale[4][2 * kKeys];  // 2^ev, then ev (-inf: no key)
   __shared__ int warp_exps[2][4];
@@ -206,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == 16) {
     // The row of this CTA's tile; late tiles, which have the most keys, go first.
     const int want = static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x);
     int row = -1, before = 0;
@@ -239,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   const int row = found[0];
   if (row < 0) return;  // the whole CTA: fewer tiles than the grid has room for
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
   }
@@ -259,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int kt0 = static_cast<int>(static_cast<long long>(all) * blockIdx.z / gridDim.z);
   const int n = static_cast<int>(static_cast<long long>(all) * (blockIdx.z + 1) / gridDim.z) - kt0;
 
-  if (warp == 12) {
+  if (warp == 16) {
     // ---------------------------------------------------------------- products
     if (lane == 0 && n > 0) {
       constexpr uint32_t idesc_s = umma_idesc(kRows, kKeys, 0);
@@ -294,7 +293,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = ok && wait(&k_full[0], 0);
         if (ok) {
           scores(0, 0);
-          scores(0, 1);
+          // Half a period behind: one group's weights then run under the
+          // other's products, and neither waits for the exponentials of both.
+          ok = wait(&p_full[0], 0);
+          if (ok) scores(0, 1);
           umma_commit(&k_empty[0]);
         }
         for (int i = 0; ok && i < n; ++i) {
@@ -342,51 +344,70 @@ __global__ void __launch_bounds__(kThreads, 1)
     // thread, which are one 16-byte chunk of F16; the eight chunks of a row's 64
     // dimensions reach eight different groups of banks.
     constexpr int kPages = kKeys / kKv8Page, kHalves = D / 64;
-    const int tid = threadIdx.x - kSoftmax, cw = warp - 8;
+    const bool values = warp >= 12;
+    const int tid = (threadIdx.x - kSoftmax) & 127, cw = warp & 3;
     const int chunk = tid & 7, prow = tid >> 3;
     const int32_t* table = a.tables + static_cast<size_t>(row) * a.max_blocks;
-    const uint32_t code_at = prow * D + chunk * 8;  // in a page's codes
-    uint2 kc[kPages * kHalves], vc[kPages * kHalves];
+    uint2 c[kPages * kHalves];
     // The tile's pages of this kv head, in the first eight lanes (-1: none).
     auto load_ids = [&](int t) {
       const int key = (kt0 + t) * kKeys + lane * kKv8Page;
       // Below max_blocks: keys is at most the row's length.
       return t < n && lane < 8 && key < keys ? __ldg(table + key / kKv8Page) : -1;
     };
-    int ids = load_ids(0), kids = -1, vids = -1;  // of the tile to load, and of the loaded K and V
-    uint32_t ks = 0u, vs = 0u;                    // scale bytes of key `tid` of the loaded K
-    bool have = false, hole = false;              // whether that key is there, or should be
+    auto pages_of = [&](int id) { return id >= 0 && id < a.cache.blocks ? id * hkv + kvh : -1; };
     // This thread's row of page p is a key while 16 p is below this.
     auto left = [&](int t) { return keys - (kt0 + t) * kKeys - prow; };
-    auto load_k = [&](int t) {
-      const int key0 = (kt0 + t) * kKeys;
-      if (lane < 8 && key0 + lane * kKv8Page < keys && (ids < 0 || ids >= a.cache.blocks)) {
-        atomicOr(a.status, kDevBadIndex);
-        ids = -1;
-      }
-      kids = ids < 0 ? -1 : ids * hkv + kvh;
-      const int page = __shfl_sync(0xffffffffu, kids, tid / kKv8Page);
-      have = page >= 0 && key0 + tid < keys;
-      hole = page < 0 && key0 + tid < keys;
-      const size_t at = static_cast<size_t>(max(page, 0)) * kKv8Page + tid % kKv8Page;
-      ks = load_byte_if(a.cache.k_scale + at, have);
-      vs = load_byte_if(a.cache.v_scale + at, have);
-      load_codes<D>(kc, a.cache.k + code_at, kids, left(t));
-      ids = load_ids(t + 1);  // a tile ahead, so that no load waits for another
-    };
-    // Codes in flight are the other operand's: K of tile t + 1 is asked for as
-    // soon as K of tile t is stored, and arrives under V of tile t - 1, and so on.
+    const uint8_t* pool = (values ? a.cache.v : a.cache.k) + prow * D + chunk * 8;
     bool ok = true;
-    if (n > 0) load_k(0);
-    for (int t = 0; t <= n; ++t) {
-      if (t < n) {
-        value_scale[t & 3][tid] = have ? kv8_scale(vs) : 0.f;
-        value_scale[t & 3][kKeys + tid] = have ? static_cast<float>(static_cast<int>(vs) - 127) : -INFINITY;
+    int pages = pages_of(load_ids(0));
+    int ids = load_ids(1);  // a tile ahead, so that no load waits for another
+    if (n > 0) {
+#pragma unroll
+      for (int p = 0; p < kPages; ++p) load_codes<D>(c + p * kHalves, pool, pages, p, left(0));
+    }
+    if (values) {
+#pragma unroll 1
+      for (int t = 0; t < n; ++t) {
+        if (t >= 2) ok = mbar_wait(&v_empty[t & 1], ((t - 2) >> 1) & 1, a.status);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        uint8_t* dst = smem + T::kV + (t & 1) * T::kOperand;
+        pages = pages_of(ids);  // -1 everywhere past the last tile
+        ids = load_ids(t + 2);
+#pragma unroll
+        for (int p = 0; p < kPages; ++p) {
+          store_codes<D, false>(dst, p * kKv8Page + prow, chunk, c + p * kHalves, 0u);
+          load_codes<D>(c + p * kHalves, pool, pages, p, left(t + 1));
+        }
+        fence_proxy_async();
+        mbar_arrive(&v_full[t & 1]);
+      }
+    } else {
+      uint32_t ks = 0u, vs = 0u;        // scale bytes of key `tid` of the tile
+      bool have = false, hole = false;  // whether that key is there, or should be
+      auto load_scales = [&](int t) {
+        const int page = __shfl_sync(0xffffffffu, pages, tid / kKv8Page);
+        const bool key = (kt0 + t) * kKeys + tid < keys;
+        have = page >= 0 && key;
+        hole = page < 0 && key;
+        const size_t at = static_cast<size_t>(max(page, 0)) * kKv8Page + tid % kKv8Page;
+        ks = load_byte_if(a.cache.k_scale + at, have);
+        vs = load_byte_if(a.cache.v_scale + at, have);
+      };
+      if (n > 0) load_scales(0);
+#pragma unroll 1
+      for (int t = 0; t < n; ++t) {
+        if (hole) atomicOr(a.status, kDevBadIndex);
+        const float ev = have ? static_cast<float>(static_cast<int>(vs) - 127) : -INFINITY;
+        const float scale = have ? kv8_scale(vs) : 0.f;
         key_scale[t & 1][tid] = static_cast<uint8_t>(ks);
         // E + 127, so that 0 is no key's.
         int ek = __reduce_max_sync(0xffffffffu, have ? static_cast<int>(ks) : 0);
         const bool any_hole = __any_sync(0xffffffffu, hole);
         if (lane == 0) warp_exps[t & 1][cw] = ek * 2 + (any_hole ? 1 : 0);
+        pages = pages_of(ids);
+        ids = load_ids(t + 2);
+        load_scales(t + 1);
         named_bar_sync(3, 128);
         int holes = 0;
 #pragma unroll
@@ -394,35 +415,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           ek = max(ek, warp_exps[t & 1][w] >> 1);
           holes |= warp_exps[t & 1][w] & 1;
         }
+        if (t >= 2) ok = mbar_wait(&k_empty[t & 1], ((t - 2) >> 1) & 1, a.status);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        // The scores of tile t - 2 followed the sums of tile t - 4, so that
+        // tile's entry is read by nobody any more.
         if (tid == 0) {
           exps[t & 3][0] = ek > 0 ? ek : 127;
           exps[t & 3][1] = holes;
         }
-        if (t >= 2) ok = mbar_wait(&k_empty[t & 1], ((t - 2) >> 1) & 1, a.status);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        value_scale[t & 3][tid] = scale;
+        value_scale[t & 3][kKeys + tid] = ev;
         uint32_t factor[kPages];
 #pragma unroll
         for (int p = 0; p < kPages; ++p)
           factor[p] = half_power2(static_cast<int>(key_scale[t & 1][p * kKv8Page + prow]) - ek + 127);
         uint8_t* dst = smem + T::kK + (t & 1) * T::kOperand;
 #pragma unroll
-        for (int p = 0; p < kPages; ++p) store_codes<D, true>(dst, p * kKv8Page + prow, chunk, kc + p * kHalves, factor[p]);
+        for (int p = 0; p < kPages; ++p) {
+          store_codes<D, true>(dst, p * kKv8Page + prow, chunk, c + p * kHalves, factor[p]);
+          load_codes<D>(c + p * kHalves, pool, pages, p, left(t + 1));
+        }
         fence_proxy_async();
         mbar_arrive(&k_full[t & 1]);
       }
-      vids = kids;
-      if (t + 1 < n) load_k(t + 1);
-      if (t >= 1) {
-        const int v = t - 1;
-        if (v >= 2) ok = mbar_wait(&v_empty[v & 1], ((v - 2) >> 1) & 1, a.status);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        uint8_t* dst = smem + T::kV + (v & 1) * T::kOperand;
-#pragma unroll
-        for (int p = 0; p < kPages; ++p) store_codes<D, false>(dst, p * kKv8Page + prow, chunk, vc + p * kHalves, 0u);
-        fence_proxy_async();
-        mbar_arrive(&v_full[v & 1]);
-      }
-      if (t < n) load_codes<D>(vc, a.cache.v + code_at, vids, left(t));
     }
   } else {
     // ---------------------------------------------------------------- softmax
@@ -467,21 +482,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         return make_float2(__uint_as_float(lo), __uint_as_float(hi));
       };
       float alpha = 1.f;
-      // Two passes over the scores, 32 at a time in a rolled loop: the code of
-      // all roles has to stay in the instruction cache, or the products wait
-      // for their instructions.
+      // Two passes over the scores in rolled loops: the code of all roles has to
+      // stay in the instruction cache, or the products wait for their
+      // instructions.  16 scores are on their way while 16 are worked on.
       auto pass = [&](auto masked) {
         float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < kKeys; c += 32) {
-          uint32_t v[32];
-          tmem_ld32_nowait(sa + c, v);
-          tmem_ld_wait();
+        uint32_t v[2][16];
+        auto largest = [&](const uint32_t (&x)[16], int c) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 ev = vs[kKeys / 4 + (c + i) / 4];
-            float2 y0 = fma2(pair_of(v[i], v[i + 1]), f2, make_float2(ev.x, ev.y));
-            float2 y1 = fma2(pair_of(v[i + 2], v[i + 3]), f2, make_float2(ev.z, ev.w));
+          for (int i = 0; i < 16; i += 4) {
+            const float4 ev = vs[(kKeys + c + i) / 4];
+            float2 y0 = fma2(pair_of(x[i], x[i + 1]), f2, make_float2(ev.x, ev.y));
+            float2 y1 = fma2(pair_of(x[i + 2], x[i + 3]), f2, make_float2(ev.z, ev.w));
             if (decltype(masked)::value) {
               if (c + i > seen) y0.x = -INFINITY;
               if (c + i + 1 > seen) y0.y = -INFINITY;
@@ -491,6 +503,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             m0 = fmaxf(m0, fmaxf(y0.x, y0.y));
             m1 = fmaxf(m1, fmaxf(y1.x, y1.y));
           }
+        };
+        tmem_ld16_nowait(sa, v[0]);
+#pragma unroll 1
+        for (int c = 0; c < kKeys; c += 32) {
+          tmem_ld_wait();
+          tmem_ld16_nowait(sa + c + 16, v[1]);
+          largest(v[0], c);
+          tmem_ld_wait();
+          tmem_ld16_nowait(sa + (c + 32) % kKeys, v[0]);  // at the end: the second pass's first
+          largest(v[1], c + 16);
         }
         const float mx = fmaxf(m0, m1);
         // A reference moves only when a weight would pass 2^8: it becomes the
@@ -501,16 +523,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float2 sum = make_float2(0.f, 0.f);
         const float2 minus = make_float2(-m, -m);
-#pragma unroll 1
-        for (int c = 0; c < kKeys; c += 32) {
-          uint32_t v[32], pk[16];
-          tmem_ld32_nowait(sa + c, v);
-          tmem_ld_wait();
+        // The weights of 16 keys go over scores that are read already.
+        auto weigh = [&](const uint32_t (&x)[16], int c) {
+          uint32_t pk[8];
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
+          for (int i = 0; i < 16; i += 4) {
             const float4 sc = vs[(c + i) / 4];
-            float2 y0 = fma2(pair_of(v[i], v[i + 1]), f2, minus);
-            float2 y1 = fma2(pair_of(v[i + 2], v[i + 3]), f2, minus);
+            float2 y0 = fma2(pair_of(x[i], x[i + 1]), f2, minus);
+            float2 y1 = fma2(pair_of(x[i + 2], x[i + 3]), f2, minus);
             if (decltype(masked)::value) {
               if (c + i > seen || sc.x == 0.f) y0.x = -INFINITY;
               if (c + i + 1 > seen || sc.y == 0.f) y0.y = -INFINITY;
@@ -523,8 +543,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             pk[i >> 1] = half2_bits(p0.x, p0.y);
             pk[(i >> 1) + 1] = half2_bits(p1.x, p1.y);
           }
-          // The weights of these 32 keys go over scores that are read already.
-          tmem_st16(sa + c / 2, pk);
+          tmem_st8(sa + c / 2, pk);
+        };
+#pragma unroll 1
+        for (int c = 0; c < kKeys; c += 32) {
+          tmem_ld_wait();
+          tmem_ld16_nowait(sa + c + 16, v[1]);
+          weigh(v[0], c);
+          tmem_ld_wait();
+          if (c + 32 < kKeys) tmem_ld16_nowait(sa + c + 32, v[0]);
+          weigh(v[1], c + 16);
         }
         return sum.x + sum.y;
       };
@@ -637,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
 // Joins the key splits of a query tile in order: one CTA a tile and kv head.
