@@ -13,7 +13,10 @@
 //               are code * 2^(e - E) with E the tile's largest exponent, so that
 //               F16 holds rows of any size; what it rounds lies 2^-34 below the
 //               largest row, and E goes into the score scale of the tile.  V
-//               rows are the codes; their scales go into the weights.
+//               rows likewise where the tile's exponents lie within 2^8 of their
+//               largest E' (exact then), which goes into the weights' exponent;
+//               else they are the codes, and each key's scale goes into its
+//               weights.
 //   warp 16     one thread issues the products.
 //   warps 0-7   two softmax groups of 128 threads, one row (TMEM lane) a
 //               thread.  The weights go back into TMEM over the scores they
@@ -29,7 +32,8 @@
 // With s_j the score in log2 and ev_j the exponent of value row j, a row keeps
 // one reference m for  l = sum 2^(s_j - m)  and  O = sum (2^(s_j - m) 2^ev_j) d_j,
 // d_j the codes: the weights in brackets are what F16 has to hold, so m follows
-// max (s_j + ev_j), lazily, and o = O / l.  Every wait is bounded (common.cuh).
+// max (s_j + ev_j), lazily, and o = O / l.  (2^(s_j - m + E') 2^(ev_j - E') d_j
+// where E' is taken out: the weights are then the exponentials themselves.)  Every wait is bounded (common.cuh).
 #include <algorithm>
 #include <type_traits>
 
@@ -43,6 +47,8 @@ constexpr int kKeys = 128;       // keys of a tile
 constexpr int kRows = 128;       // columns of a query tile
 constexpr int kSoftmax = 256;    // threads of the softmax groups
 constexpr int kThreads = kSoftmax + 256 + 32;
+constexpr int kSpread = 8;        // V exponents this near their tile's largest are taken out of the weights
+constexpr int kApart = 1000;      // others
 
 // D[tmem] (+)= A[tmem] * B[smem desc]: A is F16 pairs, a row per lane.
 __device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
@@ -112,13 +118,13 @@ struct Tile {
 
 // Loads that leave zeros where !live, without a branch, so that a run of them
 // is in flight together.
-__device__ __forceinline__ uint2 load8_if(const void* p, bool live) {
-  uint2 v;
+__device__ __forceinline__ uint4 load16_if(const void* p, bool live) {
+  uint4 v;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t"
-      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t"
-      "@p ld.global.nc.v2.u32 {%0, %1}, [%2];\n\t}"
-      : "=&r"(v.x), "=&r"(v.y)
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
       : "l"(p), "r"(static_cast<uint32_t>(live)));
   return v;
 }
@@ -142,32 +148,49 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// A converter thread's codes of one page of a tile, eight of each 64 dimensions
-// of its row; `pages` (pool page of this kv head, -1: none) is in the first
-// lanes; zeros past the last key.
+// How the 128 threads of a converter group share a tile: 16 codes of a key a
+// thread, kRows keys a pass.  Of eight lanes in a row four hold one key's codes
+// and four its neighbour's: their 16-byte chunks of F16, every second one of a
+// key, then reach eight different groups of banks under the swizzle.
 template <int D>
-__device__ __forceinline__ void load_codes(uint2* c, const uint8_t* pool, int pages, int p, int left) {
-  const int page = __shfl_sync(0xffffffffu, pages, p);
-  const bool live = page >= 0 && p * kKv8Page < left;
-  const uint8_t* at = pool + static_cast<uint64_t>(static_cast<uint32_t>(page)) * (kKv8Page * D);
-#pragma unroll
-  for (int h = 0; h < D / 64; ++h) c[h] = load8_if(at + h * 64, live);
-}
-// Eight codes of each 64 dimensions as swizzled 16-byte chunks of F16, times a
-// factor where they are scaled.
-template <int D, bool SCALED>
-__device__ __forceinline__ void store_codes(uint8_t* dst, int r, int chunk, const uint2* c,
-                                            uint32_t factor) {
-#pragma unroll
-  for (int h = 0; h < D / 64; ++h) {
-    uint32_t f[4] = {kv8_half2_lo(c[h].x), kv8_half2_hi(c[h].x), kv8_half2_lo(c[h].y),
-                     kv8_half2_hi(c[h].y)};
-    if (SCALED) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] = mul2(f[j], factor);
+struct Share {
+  static constexpr int kLanes = D / 16;             // threads of a key
+  static constexpr int kRows = 128 / kLanes;        // keys of a pass
+  static constexpr int kPasses = kKeys / kRows;
+  int chunk, row;                                   // codes 16 chunk ..., key row of a pass
+  __device__ explicit Share(int tid) {
+    const int lane = tid & 31, warp = tid >> 5;
+    if (D == 128) {
+      chunk = (lane & 3) | (lane >> 1 & 4);
+      row = warp * 4 + (lane >> 4) * 2 + (lane >> 2 & 1);
+    } else {
+      chunk = lane & 3;
+      row = warp * 8 + (lane >> 2);
     }
-    *reinterpret_cast<uint4*>(dst + h * 128 * 128 + r * 128 + ((chunk ^ (r & 7)) << 4)) =
-        make_uint4(f[0], f[1], f[2], f[3]);
+  }
+};
+// The codes of pass p; `pages` (pool page of this kv head, -1: none) is in the
+// first lanes; zeros from key `left` on.
+template <int D>
+__device__ __forceinline__ uint4 load_codes(const Share<D>& h, const uint8_t* pool, int pages, int p,
+                                            int left) {
+  const int key = p * Share<D>::kRows + h.row;
+  const int page = __shfl_sync(0xffffffffu, pages, key / kKv8Page);
+  const uint8_t* at = pool + static_cast<uint64_t>(static_cast<uint32_t>(page)) * (kKv8Page * D);
+  return load16_if(at, page >= 0 && key < left);
+}
+// Times 2^k (a factor for both halves of a word) as two swizzled chunks of F16.
+template <int D>
+__device__ __forceinline__ void store_codes(uint8_t* dst, const Share<D>& h, int p, const uint4& c,
+                                            uint32_t factor) {
+  const int r = p * Share<D>::kRows + h.row;
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int c16 = h.chunk * 2 + k;
+    *reinterpret_cast<uint4*>(dst + (c16 >> 3) * (128 * 128) + r * 128 + (((c16 & 7) ^ (r & 7)) << 4)) =
+        make_uint4(mul2(kv8_half2_lo(w[2 * k]), factor), mul2(kv8_half2_hi(w[2 * k]), factor),
+                   mul2(kv8_half2_lo(w[2 * k + 1]), factor), mul2(kv8_half2_hi(w[2 * k + 1]), factor));
   }
 }
 
@@ -182,12 +205,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       o_done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int found[2];             // row, tile in the row
-  // By key tile: E + 127 of its K, whether a page is missing, and each key's 2^ev
-  // (0 where there is no key).
+  // By key tile: E + 127 of its K; E' of its V, or kApart; and then each key's
+  // 2^ev (0 where there is no key) and ev (-inf).
   __shared__ volatile int exps[4][2];
-  __shared__ __align__(16) float value_scale[4][2 * kKeys];  // 2^ev, then ev (-inf: no key)
-  __shared__ int warp_exps[2][4];
-  __shared__ uint8_t key_scale[2][kKeys];
+  __shared__ __align__(16) float value_scale[4][2 * kKeys];
+  __shared__ int extremes[2][2][4][3];          // by group, tile and warp: E, E' + 127, least ev + 127
+  __shared__ uint8_t scale_byte[2][2][kKeys];   // by group and tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kCta = T::kQueries * kRows;  // columns of a CTA
 
@@ -340,15 +363,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 8) {
     // ---------------------------------------------------------------- converters
-    // A page at a time: eight threads a row, eight codes of each 64 dimensions a
-    // thread, which are one 16-byte chunk of F16; the eight chunks of a row's 64
-    // dimensions reach eight different groups of banks.
-    constexpr int kPages = kKeys / kKv8Page, kHalves = D / 64;
     const bool values = warp >= 12;
     const int tid = (threadIdx.x - kSoftmax) & 127, cw = warp & 3;
-    const int chunk = tid & 7, prow = tid >> 3;
+    const Share<D> share(tid);
+    constexpr int kPasses = Share<D>::kPasses;
     const int32_t* table = a.tables + static_cast<size_t>(row) * a.max_blocks;
-    uint2 c[kPages * kHalves];
     // The tile's pages of this kv head, in the first eight lanes (-1: none).
     auto load_ids = [&](int t) {
       const int key = (kt0 + t) * kKeys + lane * kKv8Page;
@@ -356,88 +375,86 @@ __global__ void __launch_bounds__(kThreads, 1)
       return t < n && lane < 8 && key < keys ? __ldg(table + key / kKv8Page) : -1;
     };
     auto pages_of = [&](int id) { return id >= 0 && id < a.cache.blocks ? id * hkv + kvh : -1; };
-    // This thread's row of page p is a key while 16 p is below this.
-    auto left = [&](int t) { return keys - (kt0 + t) * kKeys - prow; };
-    const uint8_t* pool = (values ? a.cache.v : a.cache.k) + prow * D + chunk * 8;
-    bool ok = true;
+    const uint8_t* pool = (values ? a.cache.v : a.cache.k) + (share.row % kKv8Page) * D + share.chunk * 16;
+    uint4 c[kPasses];
     int pages = pages_of(load_ids(0));
     int ids = load_ids(1);  // a tile ahead, so that no load waits for another
+    uint32_t ks = 0u, vs = 0u;        // scale bytes of key `tid` of the tile
+    bool have = false, hole = false;  // whether that key is there, or should be
+    auto load_scales = [&](int t) {
+      const int page = __shfl_sync(0xffffffffu, pages, tid / kKv8Page);
+      const bool key = (kt0 + t) * kKeys + tid < keys;
+      have = page >= 0 && key;
+      hole = page < 0 && key;
+      const size_t at = static_cast<size_t>(max(page, 0)) * kKv8Page + tid % kKv8Page;
+      ks = load_byte_if(a.cache.k_scale + at, have);
+      vs = load_byte_if(a.cache.v_scale + at, have);
+    };
     if (n > 0) {
+      load_scales(0);
 #pragma unroll
-      for (int p = 0; p < kPages; ++p) load_codes<D>(c + p * kHalves, pool, pages, p, left(0));
+      for (int p = 0; p < kPasses; ++p) c[p] = load_codes<D>(share, pool, pages, p, keys - kt0 * kKeys);
     }
-    if (values) {
+    const int group_of = values ? 1 : 0;
+    uint64_t* const full = values ? v_full : k_full;
+    uint64_t* const empty = values ? v_empty : k_empty;
+    uint8_t* const operand = smem + (values ? T::kV : T::kK);
 #pragma unroll 1
-      for (int t = 0; t < n; ++t) {
-        if (t >= 2) ok = mbar_wait(&v_empty[t & 1], ((t - 2) >> 1) & 1, a.status);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        uint8_t* dst = smem + T::kV + (t & 1) * T::kOperand;
-        pages = pages_of(ids);  // -1 everywhere past the last tile
-        ids = load_ids(t + 2);
-#pragma unroll
-        for (int p = 0; p < kPages; ++p) {
-          store_codes<D, false>(dst, p * kKv8Page + prow, chunk, c + p * kHalves, 0u);
-          load_codes<D>(c + p * kHalves, pool, pages, p, left(t + 1));
-        }
-        fence_proxy_async();
-        mbar_arrive(&v_full[t & 1]);
+    for (int t = 0; t < n; ++t) {
+      // The tile's exponents; bytes are e + 127, and 0 is no key's.
+      if (hole && !values) atomicOr(a.status, kDevBadIndex);
+      const int mine = static_cast<int>(values ? vs : ks);
+      scale_byte[group_of][t & 1][tid] = static_cast<uint8_t>(mine);
+      const int ek = __reduce_max_sync(0xffffffffu, have ? static_cast<int>(ks) : 0);
+      const int ev = __reduce_max_sync(0xffffffffu, have ? static_cast<int>(vs) : 0);
+      // A missing page takes the path that looks at each key.
+      const int least = __reduce_min_sync(0xffffffffu, have ? static_cast<int>(vs) : hole ? -1000 : 1000);
+      if (lane == 0) {
+        extremes[group_of][t & 1][cw][0] = ek;
+        extremes[group_of][t & 1][cw][1] = ev;
+        extremes[group_of][t & 1][cw][2] = least;
       }
-    } else {
-      uint32_t ks = 0u, vs = 0u;        // scale bytes of key `tid` of the tile
-      bool have = false, hole = false;  // whether that key is there, or should be
-      auto load_scales = [&](int t) {
-        const int page = __shfl_sync(0xffffffffu, pages, tid / kKv8Page);
-        const bool key = (kt0 + t) * kKeys + tid < keys;
-        have = page >= 0 && key;
-        hole = page < 0 && key;
-        const size_t at = static_cast<size_t>(max(page, 0)) * kKv8Page + tid % kKv8Page;
-        ks = load_byte_if(a.cache.k_scale + at, have);
-        vs = load_byte_if(a.cache.v_scale + at, have);
-      };
-      if (n > 0) load_scales(0);
-#pragma unroll 1
-      for (int t = 0; t < n; ++t) {
-        if (hole) atomicOr(a.status, kDevBadIndex);
-        const float ev = have ? static_cast<float>(static_cast<int>(vs) - 127) : -INFINITY;
-        const float scale = have ? kv8_scale(vs) : 0.f;
-        key_scale[t & 1][tid] = static_cast<uint8_t>(ks);
-        // E + 127, so that 0 is no key's.
-        int ek = __reduce_max_sync(0xffffffffu, have ? static_cast<int>(ks) : 0);
-        const bool any_hole = __any_sync(0xffffffffu, hole);
-        if (lane == 0) warp_exps[t & 1][cw] = ek * 2 + (any_hole ? 1 : 0);
-        pages = pages_of(ids);
-        ids = load_ids(t + 2);
-        load_scales(t + 1);
-        named_bar_sync(3, 128);
-        int holes = 0;
+      const float scale = have ? kv8_scale(vs) : 0.f;
+      const float exponent = have ? static_cast<float>(static_cast<int>(vs) - 127) : -INFINITY;
+      pages = pages_of(ids);  // -1 everywhere past the last tile
+      ids = load_ids(t + 2);
+      load_scales(t + 1);
+      named_bar_sync(3 + group_of, 128);
+      int e_k = 0, e_v = 0, low = 1000;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          ek = max(ek, warp_exps[t & 1][w] >> 1);
-          holes |= warp_exps[t & 1][w] & 1;
-        }
-        if (t >= 2) ok = mbar_wait(&k_empty[t & 1], ((t - 2) >> 1) & 1, a.status);
-        if (!__all_sync(0xffffffffu, ok)) break;
+      for (int w = 0; w < 4; ++w) {
+        e_k = max(e_k, extremes[group_of][t & 1][w][0]);
+        e_v = max(e_v, extremes[group_of][t & 1][w][1]);
+        low = min(low, extremes[group_of][t & 1][w][2]);
+      }
+      // (max (s f) is max (s) f for a scale >= 0 only.)
+      const bool apart = e_v - low > kSpread || !(a.scale >= 0.f);
+      const bool ok = t < 2 || mbar_wait(&empty[t & 1], ((t - 2) >> 1) & 1, a.status);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (!values) {
         // The scores of tile t - 2 followed the sums of tile t - 4, so that
         // tile's entry is read by nobody any more.
         if (tid == 0) {
-          exps[t & 3][0] = ek > 0 ? ek : 127;
-          exps[t & 3][1] = holes;
+          exps[t & 3][0] = e_k > 0 ? e_k : 127;
+          exps[t & 3][1] = apart ? kApart : e_v - 127;
         }
-        value_scale[t & 3][tid] = scale;
-        value_scale[t & 3][kKeys + tid] = ev;
-        uint32_t factor[kPages];
-#pragma unroll
-        for (int p = 0; p < kPages; ++p)
-          factor[p] = half_power2(static_cast<int>(key_scale[t & 1][p * kKv8Page + prow]) - ek + 127);
-        uint8_t* dst = smem + T::kK + (t & 1) * T::kOperand;
-#pragma unroll
-        for (int p = 0; p < kPages; ++p) {
-          store_codes<D, true>(dst, p * kKv8Page + prow, chunk, c + p * kHalves, factor[p]);
-          load_codes<D>(c + p * kHalves, pool, pages, p, left(t + 1));
+        if (apart) {
+          value_scale[t & 3][tid] = scale;
+          value_scale[t & 3][kKeys + tid] = exponent;
         }
-        fence_proxy_async();
-        mbar_arrive(&k_full[t & 1]);
       }
+      uint8_t* dst = operand + (t & 1) * T::kOperand;
+      const int top = values ? e_v : e_k;
+      const int left = keys - (kt0 + t + 1) * kKeys;
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        const int byte = scale_byte[group_of][t & 1][p * Share<D>::kRows + share.row];
+        const uint32_t factor = values && apart ? 0x3c003c00u : half_power2(byte - top + 127);
+        store_codes<D>(dst, share, p, c[p], factor);
+        c[p] = load_codes<D>(share, pool, pages, p, left);
+      }
+      fence_proxy_async();
+      mbar_arrive(&full[t & 1]);
     }
   } else {
     // ---------------------------------------------------------------- softmax
@@ -474,8 +491,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       tc_fence_after();
       const float f = sl2 * __uint_as_float(static_cast<uint32_t>(exps[t & 3][0]) << 23);
+      const int e_v = exps[t & 3][1];
       const int seen = lim - (kt0 + t) * kKeys;  // keys 0 .. seen of the tile
-      const bool full = __all_sync(0xffffffffu, seen >= kKeys - 1) && !exps[t & 3][1];
       const float4* vs = reinterpret_cast<const float4*>(value_scale[t & 3]);
       const float2 f2 = make_float2(f, f);
       auto pair_of = [](uint32_t lo, uint32_t hi) {
@@ -485,16 +502,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Two passes over the scores in rolled loops: the code of all roles has to
       // stay in the instruction cache, or the products wait for their
       // instructions.  16 scores are on their way while 16 are worked on.
-      auto pass = [&](auto masked) {
+      auto pass = [&](auto kind) {
+        constexpr bool kMasked = decltype(kind)::value >= 1, kEach = decltype(kind)::value == 2;
         float m0 = -INFINITY, m1 = -INFINITY;
         uint32_t v[2][16];
         auto largest = [&](const uint32_t (&x)[16], int c) {
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
-            const float4 ev = vs[(kKeys + c + i) / 4];
-            float2 y0 = fma2(pair_of(x[i], x[i + 1]), f2, make_float2(ev.x, ev.y));
-            float2 y1 = fma2(pair_of(x[i + 2], x[i + 3]), f2, make_float2(ev.z, ev.w));
-            if (decltype(masked)::value) {
+            float2 y0 = pair_of(x[i], x[i + 1]), y1 = pair_of(x[i + 2], x[i + 3]);
+            if (kEach) {
+              const float4 ev = vs[(kKeys + c + i) / 4];
+              y0 = fma2(y0, f2, make_float2(ev.x, ev.y));
+              y1 = fma2(y1, f2, make_float2(ev.z, ev.w));
+            }
+            if (kMasked) {
               if (c + i > seen) y0.x = -INFINITY;
               if (c + i + 1 > seen) y0.y = -INFINITY;
               if (c + i + 2 > seen) y1.x = -INFINITY;
@@ -514,7 +535,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld16_nowait(sa + (c + 32) % kKeys, v[0]);  // at the end: the second pass's first
           largest(v[1], c + 16);
         }
-        const float mx = fmaxf(m0, m1);
+        const float offset = kEach ? 0.f : static_cast<float>(e_v);
+        const float mx = kEach ? fmaxf(m0, m1) : fmaf(fmaxf(m0, m1), f, offset);
         // A reference moves only when a weight would pass 2^8: it becomes the
         // row's largest so far.
         if (mx > m + kLazy) {
@@ -522,26 +544,35 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = mx;
         }
         float2 sum = make_float2(0.f, 0.f);
-        const float2 minus = make_float2(-m, -m);
+        const float2 minus = make_float2(offset - m, offset - m);
         // The weights of 16 keys go over scores that are read already.
         auto weigh = [&](const uint32_t (&x)[16], int c) {
           uint32_t pk[8];
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
-            const float4 sc = vs[(c + i) / 4];
             float2 y0 = fma2(pair_of(x[i], x[i + 1]), f2, minus);
             float2 y1 = fma2(pair_of(x[i + 2], x[i + 3]), f2, minus);
-            if (decltype(masked)::value) {
-              if (c + i > seen || sc.x == 0.f) y0.x = -INFINITY;
-              if (c + i + 1 > seen || sc.y == 0.f) y0.y = -INFINITY;
-              if (c + i + 2 > seen || sc.z == 0.f) y1.x = -INFINITY;
-              if (c + i + 3 > seen || sc.w == 0.f) y1.y = -INFINITY;
+            if (kMasked) {
+              if (c + i > seen) y0.x = -INFINITY;
+              if (c + i + 1 > seen) y0.y = -INFINITY;
+              if (c + i + 2 > seen) y1.x = -INFINITY;
+              if (c + i + 3 > seen) y1.y = -INFINITY;
             }
-            const float2 w0 = make_float2(ex2(y0.x), ex2(y0.y)), w1 = make_float2(ex2(y1.x), ex2(y1.y));
-            sum = add2f(sum, add2f(w0, w1));
-            const float2 p0 = mul2f(w0, make_float2(sc.x, sc.y)), p1 = mul2f(w1, make_float2(sc.z, sc.w));
-            pk[i >> 1] = half2_bits(p0.x, p0.y);
-            pk[(i >> 1) + 1] = half2_bits(p1.x, p1.y);
+            float2 w0, w1;
+            if (kEach) {
+              const float4 sc = vs[(c + i) / 4];
+              w0 = make_float2(sc.x == 0.f ? 0.f : ex2(y0.x), sc.y == 0.f ? 0.f : ex2(y0.y));
+              w1 = make_float2(sc.z == 0.f ? 0.f : ex2(y1.x), sc.w == 0.f ? 0.f : ex2(y1.y));
+              sum = add2f(sum, add2f(w0, w1));
+              w0 = mul2f(w0, make_float2(sc.x, sc.y));
+              w1 = mul2f(w1, make_float2(sc.z, sc.w));
+            } else {
+              w0 = make_float2(ex2(y0.x), ex2(y0.y));
+              w1 = make_float2(ex2(y1.x), ex2(y1.y));
+              sum = add2f(sum, add2f(w0, w1));
+            }
+            pk[i >> 1] = half2_bits(w0.x, w0.y);
+            pk[(i >> 1) + 1] = half2_bits(w1.x, w1.y);
           }
           tmem_st8(sa + c / 2, pk);
         };
@@ -554,9 +585,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (c + 32 < kKeys) tmem_ld16_nowait(sa + c + 32, v[0]);
           weigh(v[1], c + 16);
         }
-        return sum.x + sum.y;
+        return kEach ? sum.x + sum.y : (sum.x + sum.y) * ex2(-offset);
       };
-      const float rs = full ? pass(std::false_type{}) : pass(std::true_type{});
+      const bool full = __all_sync(0xffffffffu, seen >= kKeys - 1);
+      const float rs = e_v == kApart ? pass(std::integral_constant<int, 2>{})
+                       : full ? pass(std::integral_constant<int, 0>{})
+                              : pass(std::integral_constant<int, 1>{});
       l = l * alpha + rs;
       // O was summed to another reference: bring it to the new one.
       if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
