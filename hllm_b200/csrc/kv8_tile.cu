@@ -169,15 +169,13 @@ struct Share {
     }
   }
 };
-// The codes of pass p; `pages` (pool page of this kv head, -1: none) is in the
-// first lanes; zeros from key `left` on.
+// The codes of pass p from `page` (pool page of this kv head, -1: none); zeros
+// from key `left` on.
 template <int D>
-__device__ __forceinline__ uint4 load_codes(const Share<D>& h, const uint8_t* pool, int pages, int p,
+__device__ __forceinline__ uint4 load_codes(const Share<D>& h, const uint8_t* pool, int page, int p,
                                             int left) {
-  const int key = p * Share<D>::kRows + h.row;
-  const int page = __shfl_sync(0xffffffffu, pages, key / kKv8Page);
   const uint8_t* at = pool + static_cast<uint64_t>(static_cast<uint32_t>(page)) * (kKv8Page * D);
-  return load16_if(at, page >= 0 && key < left);
+  return load16_if(at, page >= 0 && p * Share<D>::kRows + h.row < left);
 }
 // Times 2^k (a factor for both halves of a word) as two swizzled chunks of F16.
 template <int D>
@@ -378,6 +376,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint8_t* pool = (values ? a.cache.v : a.cache.k) + (share.row % kKv8Page) * D + share.chunk * 16;
     uint4 c[kPasses];
     int pages = pages_of(load_ids(0));
+    auto page_of = [&](int p) {
+      return __shfl_sync(0xffffffffu, pages, (p * Share<D>::kRows + share.row) / kKv8Page);
+    };
     int ids = load_ids(1);  // a tile ahead, so that no load waits for another
     uint32_t ks = 0u, vs = 0u;        // scale bytes of key `tid` of the tile
     bool have = false, hole = false;  // whether that key is there, or should be
@@ -393,7 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (n > 0) {
       load_scales(0);
 #pragma unroll
-      for (int p = 0; p < kPasses; ++p) c[p] = load_codes<D>(share, pool, pages, p, keys - kt0 * kKeys);
+      for (int p = 0; p < kPasses; ++p)
+        c[p] = load_codes<D>(share, pool, page_of(p), p, keys - kt0 * kKeys);
     }
     const int group_of = values ? 1 : 0;
     uint64_t* const full = values ? v_full : k_full;
@@ -446,12 +448,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint8_t* dst = operand + (t & 1) * T::kOperand;
       const int top = values ? e_v : e_k;
       const int left = keys - (kt0 + t + 1) * kKeys;
+      // All passes' factors and pages first: nothing then waits between stores.
+      uint32_t factor[kPasses];
+      int page[kPasses];
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
+        page[p] = page_of(p);
         const int byte = scale_byte[group_of][t & 1][p * Share<D>::kRows + share.row];
-        const uint32_t factor = values && apart ? 0x3c003c00u : half_power2(byte - top + 127);
-        store_codes<D>(dst, share, p, c[p], factor);
-        c[p] = load_codes<D>(share, pool, pages, p, left);
+        factor[p] = values && apart ? 0x3c003c00u : half_power2(byte - top + 127);
+      }
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        store_codes<D>(dst, share, p, c[p], factor[p]);
+        c[p] = load_codes<D>(share, pool, page[p], p, left);
       }
       fence_proxy_async();
       mbar_arrive(&full[t & 1]);
