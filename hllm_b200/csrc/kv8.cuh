@@ -115,6 +115,7 @@ struct Kv8Configured {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoReference = -1e30f;  // below every finite score
 constexpr float kLazy = 8.f;            // log2 of the growth that moves a softmax reference
+constexpr float kMostWeight = 256.f;    // 2^kLazy
 
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -124,6 +125,14 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// The scale exponent of a row whose largest magnitude is `top` (finite, at
+// most kKv8Limit): the least e in [-24, 39] with top <= 448 * 2^e.  With
+// top = 1.f * 2^k, 448 = 1.75 * 2^8: e = k - 8, one more where 1.f > 1.75.
+__device__ __forceinline__ int kv8_exponent(float top) {
+  const uint32_t b = __float_as_uint(top);
+  const int e = static_cast<int>(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return min(max(e, kKv8ExpMin), kKv8ExpMax);
 }
 // The value of a scale byte.
 __device__ __forceinline__ float kv8_scale(uint32_t byte) {

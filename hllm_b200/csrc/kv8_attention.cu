@@ -4,13 +4,18 @@
 //
 // o = sum_j softmax_j(scale q.k_j) v_j over the keys j <= the query's position.
 // With k_j = 2^ek_j c_j and v_j = 2^ev_j d_j (codes c, d) and s_j = scale
-// log2(e) 2^ek_j (q.c_j):
-//   l = sum 2^(s_j - m),   O = sum 2^(s_j + ev_j - m') d_j,   o = O / l * 2^(m' - m)
-// for any references m, m'.  The value scales are added to the weights'
-// exponents, so the weights that the tensor cores multiply (F16, rounded by
-// 2^-11) have their own reference m' and keep their precision whatever the
-// sizes of the value rows.  A reference is raised only when a score passes it
-// by 2^8: most pages rescale nothing.
+// log2(e) 2^ek_j (q.c_j), one reference m serves
+//   l = sum 2^(s_j - m),   O = sum (2^(s_j - m) 2^ev_j) d_j,   o = O / l.
+// The weights in brackets are what the products round (F16, by 2^-11), so m
+// follows max (s_j + ev_j): they keep their precision whatever the sizes of the
+// value rows.  It is raised only when a weight passes 2^8: most pages rescale
+// nothing.
+//
+// q.c_j is a product of e4m3 operands: q is the sum of three e4m3 vectors at
+// scales 2^e, 2^(e-4) and 2^(e-8), each the rounding of what the former left.
+// Three times four bits hold the 11 of F16, so nothing of q is lost (but 2^-26
+// of a head's largest element in its small ones), the codes go into the product
+// as they are, and it runs four times faster than one of F16 operands.
 //
 // Work.  A row's new tokens and the query heads of one kv head form columns
 // (token, head), 8 NT of them a stream; a stream walks the row's pages.  The
@@ -21,18 +26,18 @@
 // joined first in the CTA (shared memory), then, where a stream spans CTAs, by
 // a second small launch, in order: results do not depend on timing.
 //
-// Per page a warp computes S^T = K Q^T and O^T = V^T P^T with m16n8k16 F16
-// products: the 16 keys, then 16 value dimensions, are the M side, so that the
-// columns are the 8-wide N side and one decode row wastes half of a tile, not
-// three quarters.  Codes go from global memory straight into the registers of
-// the fragments: the order of the products' inner dimension is free, so a lane
-// takes 16 consecutive bytes of a key for four steps of QK, and for PV the
-// bytes of four keys, paired by byte permutes.  No shared memory, no barrier,
-// no transpose is in the stream; the next page's loads are in flight while one
-// is multiplied.
+// Per page a warp computes S^T = K Q^T (m16n8k32, e4m3) and O^T = V^T P^T
+// (m16n8k16, F16): the 16 keys, then 16 value dimensions, are the M side, so
+// that the columns are the 8-wide N side and one decode row wastes half of a
+// tile, not three quarters.  The order of the products' inner dimension is
+// free, so a lane takes 16 consecutive bytes of a key for the steps of QK, and
+// for PV the bytes of four keys, paired by byte permutes: what a lane copies
+// into shared memory, ahead of time (cp.async), it alone reads back.  No
+// barrier and no transpose is in the stream.
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kv8.cuh"
@@ -49,6 +54,37 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, "
+      "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two F16 values as e4m3 codes (low half), and back.
+__device__ __forceinline__ uint32_t codes_of_half2(uint32_t h) {
+  uint32_t w;
+  asm("{\n\t.reg .b16 c;\n\tcvt.rn.satfinite.e4m3x2.f16x2 c, %1;\n\tcvt.u32.u16 %0, c;\n\t}"
+      : "=r"(w)
+      : "r"(h));
+  return w;
+}
+// Takes the e4m3 rounding of x (four F16 values) out of it: the codes, and what
+// is left times 16.
+__device__ __forceinline__ uint32_t take_codes(uint32_t (&x)[2]) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t c = codes_of_half2(x[i]);
+    const uint32_t v = kv8_half2_lo(c);
+    const __half2 left = __hsub2(*reinterpret_cast<const __half2*>(&x[i]), *reinterpret_cast<const __half2*>(&v));
+    const __half2 r = __hmul2(left, __floats2half2_rn(16.f, 16.f));
+    x[i] = *reinterpret_cast<const uint32_t*>(&r);
+    w |= c << (16 * i);
+  }
+  return w;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t o;
@@ -73,15 +109,22 @@ __device__ __forceinline__ void read_words(uint32_t (&w)[W], const uint8_t* p) {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
-// BYTES from global to shared memory, asynchronously; zeros where !live.
-template <int BYTES>
+// BYTES from global to shared memory, asynchronously; zeros where !live (WHOLE:
+// it always is).
+template <int BYTES, bool WHOLE>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {
-  const int n = live ? BYTES : 0;
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(BYTES)
+  if constexpr (WHOLE && BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  } else if constexpr (WHOLE) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+  } else if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0)
                  : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src),
+                 "r"(live ? BYTES : 0), "n"(BYTES)
+                 : "memory");
+  }
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -102,9 +145,9 @@ struct Shape {
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kStage = 32 * D + 32;  // a page's codes, each lane's own, and its scales
   static constexpr int kVAt = 16 * D, kScalesAt = 32 * D;
-  // A piece: D / 16 x NT fragments of 32 lanes x 4 sums, then cols x (m, m', l, 0).
+  // A piece: D / 16 x NT fragments of 32 lanes x 4 sums, then cols x (m, l).
   static constexpr int kUnits = D / 16 * NT * 32;
-  static constexpr int kPiece = kUnits * 4 + kCols * 4;  // floats
+  static constexpr int kPiece = kUnits * 4 + kCols * 2;  // floats
   // A warp's shared memory: its ring, whose place the piece it leaves open
   // takes at the end, and the piece it continues, which may be done earlier.
   static constexpr int kPieceBytes = kPiece * static_cast<int>(sizeof(float));
@@ -215,7 +258,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
   const int n = static_cast<int>(w1 - w0);
 
   float o[NT][D / 16][4];
-  float m[NT][2], mo[NT][2], l[NT][2];
+  float m[NT][2], l[NT][2];
   if (lane < 2) piece_row[warp * 2 + lane] = -1;
   __syncwarp();
 
@@ -233,6 +276,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
+        if (base + 32 * k >= a.rows || row >= 0) continue;
         long long incl = mine[k];
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -240,94 +284,114 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
           if (lane >= off) incl += v;
         }
         const unsigned hit = __ballot_sync(0xffffffffu, before + incl > w0);
-        if (row < 0) {
-          if (hit) {
-            const int src = __ffs(hit) - 1;
-            row = base + 32 * k + src;
-            before += __shfl_sync(0xffffffffu, incl - mine[k], src);
-          } else {
-            before += __shfl_sync(0xffffffffu, incl, 31);
-          }
+        if (hit) {
+          const int src = __ffs(hit) - 1;
+          row = base + 32 * k + src;
+          before += __shfl_sync(0xffffffffu, incl - mine[k], src);
+        } else {
+          before += __shfl_sync(0xffffffffu, incl, 31);
         }
       }
     }
     if (w0 == c0 && lane == 0) units_before = before;
     Kv8Row x = kv8_row(a, row, group, kCols, tile_from, false);
-    int stream = static_cast<int>((w0 - before) / x.pages);
-    int q = static_cast<int>((w0 - before) % x.pages);
     const float sl2 = a.scale * kLog2e;
-
-    // The loader runs ST - 1 units ahead of the arithmetic.
-    int lrow = row, lstream = stream, lq = q;
-    Kv8Row lx = x;
-    int tab_row = -1, tab_q0 = 0, tab = -1;  // 32 entries of the block table, one a lane
-    auto advance = [&](int& r, Kv8Row& xi, int& st, int& page) {
-      if (++page < xi.pages) return;
-      page = 0;
-      if (++st < xi.chunks * hkv) return;
-      st = 0;
-      while (++r < a.rows) {
-        xi = kv8_row(a, r, group, kCols, tile_from, false);
-        if (xi.chunks) return;
+    // Where the arithmetic is, and the loader, ST - 1 units ahead of it.
+    struct Cursor {
+      int row, kvh, chunk, page;
+      Kv8Row x;
+    };
+    Cursor at;
+    at.row = row;
+    at.x = kv8_row(a, row, group, kCols, tile_from, false);
+    at.page = static_cast<int>((w0 - before) % at.x.pages);
+    {
+      const int stream = static_cast<int>((w0 - before) / at.x.pages);
+      at.kvh = stream / at.x.chunks;
+      at.chunk = stream % at.x.chunks;
+    }
+    Cursor ahead = at;
+    auto advance = [&](Cursor& c) {
+      if (++c.page < c.x.pages) return;
+      c.page = 0;
+      if (++c.chunk < c.x.chunks) return;
+      c.chunk = 0;
+      if (++c.kvh < hkv) return;
+      c.kvh = 0;
+      while (++c.row < a.rows) {
+        c.x = kv8_row(a, c.row, group, kCols, tile_from, false);
+        if (c.x.chunks) return;
       }
     };
+    int tab_row = -1, tab_q0 = 0, tab = -1;  // 32 entries of the block table, one a lane
     uint8_t* ring = smem + warp * S::kWarpBytes;
     unsigned have = 0;  // bit s: stage s holds a page
+    const uint8_t* const kbase = a.cache.k + g * D + tq * S::KW * 4;
+    const uint8_t* const vbase = a.cache.v + 2 * tq * D + g * S::VW * 4;
+    const uint8_t* const sbase = (lane < 4 ? a.cache.k_scale : a.cache.v_scale) + (lane & 3) * 4;
+    const uint32_t kring = smem_u32(ring) + lane * S::KW * 4;
+    const uint32_t vring = smem_u32(ring) + S::kVAt + lane * S::VW * 4;
+    const uint32_t sring = smem_u32(ring) + S::kScalesAt + lane * 4;
+    auto copy_page = [&](int stage, int page, int valid, auto whole) {
+      const uint64_t off = static_cast<uint64_t>(static_cast<uint32_t>(page)) * (kKv8Page * D);
+      const uint8_t *kp = kbase + off, *vp = vbase + off;
+      const uint32_t kd = kring + stage * S::kStage, vd = vring + stage * S::kStage;
+      // Rows past the last key may hold anything: they are not read.
+#pragma unroll
+      for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          copy_async<S::KW * 4, decltype(whole)::value>(kd + (s * 2 + h) * S::KW * 128,
+                                                        kp + 8 * h * D + s * S::KW * 16, g + 8 * h < valid);
+#pragma unroll
+      for (int s = 0; s < S::VS; ++s)
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int key = (h & 1) + (h >> 1) * 8;
+          copy_async<S::VW * 4, decltype(whole)::value>(vd + (s * 4 + h) * S::VW * 128,
+                                                        vp + key * D + s * S::VW * 32, 2 * tq + key < valid);
+        }
+      if (lane < 8) copy_async<4, true>(sring + stage * S::kStage, sbase + static_cast<size_t>(page) * kKv8Page, true);
+    };
     auto fetch = [&](int stage) {
-      if (lrow != tab_row || lq < tab_q0 || lq >= tab_q0 + 32) {
-        tab_row = lrow;
-        tab_q0 = lq;
-        const int i = lq + lane;
-        tab = i < lx.pages && i < a.max_blocks
-                  ? __ldg(a.tables + static_cast<size_t>(lrow) * a.max_blocks + i)
+      if (ahead.row != tab_row || ahead.page < tab_q0 || ahead.page >= tab_q0 + 32) {
+        tab_row = ahead.row;
+        tab_q0 = ahead.page;
+        const int i = ahead.page + lane;
+        tab = i < ahead.x.pages && i < a.max_blocks
+                  ? __ldg(a.tables + static_cast<size_t>(ahead.row) * a.max_blocks + i)
                   : -1;
       }
-      const int b = __shfl_sync(0xffffffffu, tab, lq - tab_q0);
-      const int valid = lx.len - lq * kKv8Page;  // keys of the page
+      const int b = __shfl_sync(0xffffffffu, tab, ahead.page - tab_q0);
+      const int valid = ahead.x.len - ahead.page * kKv8Page;  // keys of the page
       const bool ok = valid > 0 && b >= 0 && b < a.cache.blocks;
       have = (have & ~(1u << stage)) | (ok ? 1u << stage : 0u);
       if (ok) {
-        const size_t at = (static_cast<size_t>(b) * hkv + lstream / lx.chunks) * kKv8Page;
-        const uint8_t* kp = a.cache.k + at * D + g * D + tq * S::KW * 4;
-        const uint8_t* vp = a.cache.v + at * D + 2 * tq * D + g * S::VW * 4;
-        const uint32_t base = smem_u32(ring + stage * S::kStage);
-        const uint32_t kd = base + lane * S::KW * 4, vd = base + S::kVAt + lane * S::VW * 4;
-        // Rows past the last key may hold anything: they are not read.
-#pragma unroll
-        for (int s = 0; s < S::KS; ++s)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            copy_async<S::KW * 4>(kd + (s * 2 + h) * S::KW * 128, kp + 8 * h * D + s * S::KW * 16,
-                                  g + 8 * h < valid);
-#pragma unroll
-        for (int s = 0; s < S::VS; ++s)
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const int key = (h & 1) + (h >> 1) * 8;
-            copy_async<S::VW * 4>(vd + (s * 4 + h) * S::VW * 128, vp + key * D + s * S::VW * 32,
-                                  2 * tq + key < valid);
-          }
-        if (lane < 8)
-          copy_async<4>(base + S::kScalesAt + lane * 4,
-                        (lane < 4 ? a.cache.k_scale : a.cache.v_scale) + at + (lane & 3) * 4, true);
+        const int page = b * hkv + ahead.kvh;
+        if (valid >= kKv8Page) copy_page(stage, page, valid, std::true_type{});
+        else copy_page(stage, page, valid, std::false_type{});
       } else if (valid > 0 && lane == 0) {
         atomicOr(a.status, kDevBadIndex);
       }
-      advance(lrow, lx, lstream, lq);
+      advance(ahead);
     };
 
-    uint32_t qb[NT][D / 16][2];
-    int lim[NT][2];  // last key that columns 2t, 2t + 1 see; -1: none
+    uint32_t qb[NT][3][D / 16];  // e4m3 parts of the queries: words of four, as the keys'
+    float qs[NT];                // 2^e of column g of an n-tile
+    float cs[NT][2];             // score scale of columns 2t, 2t + 1
+    int lim[NT][2];              // last key that these columns see
+    int edge;                    // least of them over the stream's columns
 
     auto open = [&]() {
-      const int kvh = stream / x.chunks, x0 = (stream % x.chunks) * kCols;
-      const int cols = x.count * group;
+      const int x0 = at.chunk * kCols, cols = at.x.count * group;
+      edge = 0x7fffffff;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int c = x0 + nt * 8 + g;
         const bool live = c < cols;
-        const __half* src = a.q + static_cast<size_t>(x.t0 + (live ? c / group : 0)) * a.ld_q +
-                            static_cast<size_t>(kvh * group + (live ? c % group : 0)) * D;
+        const __half* src = a.q + static_cast<size_t>(at.x.t0 + (live ? c / group : 0)) * a.ld_q +
+                            static_cast<size_t>(at.kvh * group + (live ? c % group : 0)) * D;
+        uint32_t h[D / 16][2];
 #pragma unroll
         for (int s = 0; s < S::KS; ++s)
 #pragma unroll
@@ -335,95 +399,149 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
             const uint2 v =
                 live ? __ldg(reinterpret_cast<const uint2*>(src + ((s * 4 + tq) * S::KW + w) * 4))
                      : make_uint2(0u, 0u);
-            qb[nt][s * S::KW + w][0] = v.x;
-            qb[nt][s * S::KW + w][1] = v.y;
+            h[s * S::KW + w][0] = v.x;
+            h[s * S::KW + w][1] = v.y;
+          }
+        // The head's largest element goes to 224 .. 448.
+        __half2 top = __floats2half2_rn(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<const __half2*>(&h[i][e])));
+        float mx = fmaxf(__low2float(top), __high2float(top));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const int e = max(kv8_exponent(mx), -14);
+        // A query that is not finite gives NaN.
+        const float f = mx <= 65504.f ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23)
+                                      : __uint_as_float(0x7fffffffu);
+        qs[nt] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        const __half2 f2 = __floats2half2_rn(f, f);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h[i][k]), f2);
+            h[i][k] = *reinterpret_cast<const uint32_t*>(&r);
           }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int cc = x0 + nt * 8 + 2 * tq + e;
-          lim[nt][e] = cc < cols ? max(-1, x.len - x.count + cc / group) : -1;
-          m[nt][e] = mo[nt][e] = kNoReference;
-          l[nt][e] = 0.f;
+          for (int part = 0; part < 3; ++part) qb[nt][part][i] = take_codes(h[i]);
+        }
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2) {
+          const int cc = x0 + nt * 8 + 2 * tq + e2;
+          // Columns beyond the stream's see everything; nothing of them is stored.
+          lim[nt][e2] = cc < cols ? max(-1, at.x.len - at.x.count + cc / group) : 0x7fffffff;
+          edge = min(edge, lim[nt][e2]);
+          cs[nt][e2] = __shfl_sync(0xffffffffu, qs[nt], (2 * tq + e2) * 4) * sl2;
+          m[nt][e2] = kNoReference;
+          l[nt][e2] = 0.f;
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+          for (int e2 = 0; e2 < 4; ++e2) o[nt][i][e2] = 0.f;
       }
+      edge = __reduce_min_sync(0xffffffffu, edge);
     };
 
     auto multiply = [&](const uint8_t* page, bool ok) {
       if (!ok) return;  // no keys here
-      float s[NT][2][4];
+      float s[NT][3][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][0][e] = s[nt][1][e] = 0.f;
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][part][e] = 0.f;
 #pragma unroll
       for (int st = 0; st < S::KS; ++st) {
         uint32_t k0[S::KW], k1[S::KW];
         read_words<S::KW>(k0, page + (st * 2) * S::KW * 128 + lane * S::KW * 4);
         read_words<S::KW>(k1, page + (st * 2 + 1) * S::KW * 128 + lane * S::KW * 4);
 #pragma unroll
-        for (int w = 0; w < S::KW; ++w) {
+        for (int w = 0; w < S::KW; w += 2) {
           const int i = st * S::KW + w;
-          const uint32_t a0 = kv8_half2_lo(k0[w]), a2 = kv8_half2_hi(k0[w]);
-          const uint32_t a1 = kv8_half2_lo(k1[w]), a3 = kv8_half2_hi(k1[w]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            mma16816(s[nt][i & 1], a0, a1, a2, a3, qb[nt][i][0], qb[nt][i][1]);
+#pragma unroll
+            for (int part = 0; part < 3; ++part)
+              mma16832(s[nt][part], k0[w], k1[w], k0[w + 1], k1[w + 1], qb[nt][part][i],
+                       qb[nt][part][i + 1]);
         }
       }
-      const int key = q * kKv8Page + g;
       const uint8_t* sc = page + S::kScalesAt + g;
-      const float ks0 = kv8_scale(sc[0]) * sl2, ks1 = kv8_scale(sc[8]) * sl2;
-      const float ev0 = static_cast<float>(static_cast<int>(sc[16]) - 127);
-      const float ev1 = static_cast<float>(static_cast<int>(sc[24]) - 127);
-      bool grown = false;
+      const float ks[2] = {__uint_as_float(static_cast<uint32_t>(sc[0]) << 23),
+                           __uint_as_float(static_cast<uint32_t>(sc[8]) << 23)};
+      // (A byte 0, which no write leaves, counts as the least normal number.)
+      uint32_t vb[2] = {max(static_cast<uint32_t>(sc[16]), 1u), max(static_cast<uint32_t>(sc[24]), 1u)};
+      float p[NT][4];
+      float top = 0.f;
+      const int key = at.page * kKv8Page + g;
+      if ((at.page + 1) * kKv8Page - 1 > edge) {
+        // A page that ends past the last key, or some column's.
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int h = 0; h < 2; ++h)
+          if (key + 8 * h >= at.x.len) vb[h] = 127u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool seen = key + (e >> 1) * 8 <= lim[nt][e & 1];
-          const float v = (s[nt][0][e] + s[nt][1][e]) * (e >> 1 ? ks1 : ks0);
-          s[nt][0][e] = seen ? v : -INFINITY;
-          s[nt][1][e] = s[nt][0][e] + (e >> 1 ? ev1 : ev0);
-          grown |= s[nt][0][e] > m[nt][e & 1] + kLazy || s[nt][1][e] > mo[nt][e & 1] + kLazy;
-        }
-      if (__any_sync(0xffffffffu, grown)) {
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = fmaf(fmaf(s[nt][2][e], 0.0625f, s[nt][1][e]), 0.0625f, s[nt][0][e]) *
+                            (ks[e >> 1] * cs[nt][e & 1]);
+            s[nt][0][e] = key + (e >> 1) * 8 <= lim[nt][e & 1] ? v : -INFINITY;
+          }
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[nt][0][e] = fmaf(fmaf(s[nt][2][e], 0.0625f, s[nt][1][e]), 0.0625f, s[nt][0][e]) *
+                          (ks[e >> 1] * cs[nt][e & 1]);
+      }
+      const float vs[2] = {__uint_as_float(vb[0] << 23), __uint_as_float(vb[1] << 23)};
+      auto weigh = [&]() {
+        top = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[nt][1][e] = ex2(s[nt][0][e] - m[nt][e & 1]);
+            p[nt][e] = s[nt][1][e] * vs[e >> 1];
+            top = fmaxf(top, p[nt][e]);
+          }
+      };
+      weigh();
+      if (__any_sync(0xffffffffu, top > kMostWeight)) {
+        const float ev[2] = {static_cast<float>(static_cast<int>(vb[0]) - 127),
+                             static_cast<float>(static_cast<int>(vb[1]) - 127)};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float a0 = fmaxf(s[nt][0][e], s[nt][0][e + 2]), a1 = fmaxf(s[nt][1][e], s[nt][1][e + 2]);
+            float mx = fmaxf(s[nt][0][e] + ev[0], s[nt][0][e + 2] + ev[1]);
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) {
-              a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, off));
-              a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, off));
-            }
-            const float m1 = fmaxf(m[nt][e], a0), mo1 = fmaxf(mo[nt][e], a1);
-            l[nt][e] *= ex2(m[nt][e] - m1);
-            const float f = ex2(mo[nt][e] - mo1);
-            m[nt][e] = m1;
-            mo[nt][e] = mo1;
+            for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            if (mx > m[nt][e]) {
+              const float f = ex2(m[nt][e] - mx);
+              m[nt][e] = mx;
+              l[nt][e] *= f;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              o[nt][i][e] *= f;
-              o[nt][i][e + 2] *= f;
+              for (int i = 0; i < D / 16; ++i) {
+                o[nt][i][e] *= f;
+                o[nt][i][e + 2] *= f;
+              }
             }
           }
+        weigh();
       }
       uint32_t pb[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float p2[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          l[nt][e & 1] += ex2(s[nt][0][e] - m[nt][e & 1]);
-          p2[e] = ex2(s[nt][1][e] - mo[nt][e & 1]);
-        }
-        pb[nt][0] = transpose8x8(half2_bits(p2[0], p2[1]));
-        pb[nt][1] = transpose8x8(half2_bits(p2[2], p2[3]));
+        l[nt][0] += s[nt][1][0] + s[nt][1][2];
+        l[nt][1] += s[nt][1][1] + s[nt][1][3];
+        pb[nt][0] = transpose8x8(half2_bits(p[nt][0], p[nt][1]));
+        pb[nt][1] = transpose8x8(half2_bits(p[nt][2], p[nt][3]));
       }
 #pragma unroll
       for (int st = 0; st < S::VS; ++st) {
@@ -457,19 +575,17 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
             l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
     };
 
-    bool starts = q == 0;
+    bool starts = at.page == 0;
     // The stream's sums so far: its output where this warp had it whole, else a piece.
     auto close = [&](bool ends) {
       sum_l();
       if (starts && ends) {
-        const int kvh = stream / x.chunks, x0 = (stream % x.chunks) * kCols;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float f0 = ex2(mo[nt][0] - m[nt][0]) / l[nt][0];
-          const float f1 = ex2(mo[nt][1] - m[nt][1]) / l[nt][1];
+          const float f0 = 1.f / l[nt][0], f1 = 1.f / l[nt][1];
 #pragma unroll
           for (int i = 0; i < D / 16; ++i)
-            store_unit(a, x, group, kvh, x0 + nt * 8 + 2 * tq, S::dim_of(i, g),
+            store_unit(a, at.x, group, at.kvh, at.chunk * kCols + nt * 8 + 2 * tq, S::dim_of(i, g),
                        make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]), f0, f1);
         }
         return;
@@ -482,16 +598,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
         for (int i = 0; i < D / 16; ++i)
           *reinterpret_cast<float4*>(piece + ((nt * (D / 16) + i) * 32 + lane) * 4) =
               make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]);
-        if (g == 0) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<float4*>(piece + S::kUnits * 4 + (nt * 8 + 2 * tq + e) * 4) =
-                make_float4(m[nt][e], mo[nt][e], l[nt][e], 0.f);
-        }
+        if (g == 0)
+          *reinterpret_cast<float4*>(piece + S::kUnits * 4 + (nt * 8 + 2 * tq) * 2) =
+              make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]);
       }
       if (lane == 0) {
-        piece_row[p] = row;
-        piece_stream[p] = stream;
+        piece_row[p] = at.row;
+        piece_stream[p] = at.kvh * at.x.chunks + at.chunk;
         piece_starts[p] = starts;
         piece_ends[p] = ends;
       }
@@ -503,28 +616,28 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       copy_commit();
     }
     open();
-    int stage = 0, ahead = ST - 1;  // of the page at hand, and of the one to fetch
+    int stage = 0, next = ST - 1;  // of the page at hand, and of the one to fetch
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
       copy_wait<ST - 2>();
       __syncwarp();  // the scales are other lanes' copies; the stage to fill is read by none
-      if (i + ST - 1 < n) fetch(ahead);
+      if (i + ST - 1 < n) fetch(next);
       copy_commit();
       multiply(ring + stage * S::kStage, (have >> stage) & 1u);
-      const bool ends = q == x.pages - 1;
+      const bool ends = at.page == at.x.pages - 1;
       if (ends || i + 1 == n) {
         __syncwarp();  // an open piece takes the ring's place
         close(ends);
       }
       if (i + 1 < n) {
-        advance(row, x, stream, q);
-        if (q == 0) {
+        advance(at);
+        if (at.page == 0) {
           starts = true;
           open();
         }
       }
       stage = stage + 1 == ST ? 0 : stage + 1;
-      ahead = ahead + 1 == ST ? 0 : ahead + 1;
+      next = next + 1 == ST ? 0 : next + 1;
     }
   }
   __syncthreads();
@@ -551,45 +664,35 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     for (int u = threadIdx.x; u < S::kUnits; u += S::kThreads) {
       const int nt = u / (D / 16 * 32), col = nt * 8 + 2 * (u & 3);
       if (x0 + col >= x.count * group) continue;
-      float M[2] = {kNoReference, kNoReference}, MO[2] = {kNoReference, kNoReference};
+      auto ml_of = [&](int k) {  // (m, l) of the unit's two columns
+        return *reinterpret_cast<const float4*>(S::piece(smem, k) + S::kUnits * 4 + col * 2);
+      };
+      float2 M = make_float2(kNoReference, kNoReference), L = make_float2(0.f, 0.f);
       for (int k = i; k <= last; ++k)
         if (piece_row[k] >= 0) {
-          const float4* ml = reinterpret_cast<const float4*>(S::piece(smem, k) + S::kUnits * 4) + col;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            M[e] = fmaxf(M[e], ml[e].x);
-            MO[e] = fmaxf(MO[e], ml[e].y);
-          }
+          const float4 ml = ml_of(k);
+          M = make_float2(fmaxf(M.x, ml.x), fmaxf(M.y, ml.z));
         }
-      float L[2] = {0.f, 0.f};
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k = i; k <= last; ++k)
         if (piece_row[k] >= 0) {
-          const float* piece = S::piece(smem, k);
-          const float4* ml = reinterpret_cast<const float4*>(piece + S::kUnits * 4) + col;
-          float f[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            L[e] += ml[e].z * ex2(ml[e].x - M[e]);
-            f[e] = ex2(ml[e].y - MO[e]);
-          }
-          const float4 v = *reinterpret_cast<const float4*>(piece + u * 4);
-          acc.x += v.x * f[0];
-          acc.y += v.y * f[1];
-          acc.z += v.z * f[0];
-          acc.w += v.w * f[1];
+          const float4 ml = ml_of(k);
+          const float f0 = ex2(ml.x - M.x), f1 = ex2(ml.z - M.y);
+          L.x += ml.y * f0;
+          L.y += ml.w * f1;
+          const float4 v = *reinterpret_cast<const float4*>(S::piece(smem, k) + u * 4);
+          acc.x += v.x * f0;
+          acc.y += v.y * f1;
+          acc.z += v.z * f0;
+          acc.w += v.w * f1;
         }
       if (begins && ends) {
         store_unit(a, x, group, kvh, x0 + col, S::dim_of((u >> 5) % (D / 16), (u >> 2) & 7), acc,
-                   ex2(MO[0] - M[0]) / L[0], ex2(MO[1] - M[1]) / L[1]);
+                   1.f / L.x, 1.f / L.y);
       } else {
         *reinterpret_cast<float4*>(dst + u * 4) = acc;
-        if (u % (D / 16 * 32) < 4) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<float4*>(dst + S::kUnits * 4 + (col + e) * 4) =
-                make_float4(M[e], MO[e], L[e], 0.f);
-        }
+        if (u % (D / 16 * 32) < 4)
+          *reinterpret_cast<float4*>(dst + S::kUnits * 4 + col * 2) = make_float4(M.x, L.x, M.y, L.y);
       }
     }
     if (!begins && ends) {
@@ -634,22 +737,21 @@ __global__ void __launch_bounds__(kJoinThreads)
   };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp < cols) {
-    float M = kNoReference, MO = kNoReference;
-    for (int k = first + lane; k <= end; k += 32) {
-      const float4 ml = __ldcg(reinterpret_cast<const float4*>(piece(k) + S::kUnits * 4) + warp);
-      M = fmaxf(M, ml.x);
-      MO = fmaxf(MO, ml.y);
-    }
+    auto ml_of = [&](int k) {
+      return __ldcg(reinterpret_cast<const float2*>(piece(k) + S::kUnits * 4) + warp);
+    };
+    float M = kNoReference;
+    for (int k = first + lane; k <= end; k += 32) M = fmaxf(M, ml_of(k).x);
     M = warp_max(M);
-    MO = warp_max(MO);
     float L = 0.f;
     for (int k = first + lane; k <= end; k += 32) {
-      const float4 ml = __ldcg(reinterpret_cast<const float4*>(piece(k) + S::kUnits * 4) + warp);
-      L += ml.z * ex2(ml.x - M);
-      weight[(k - first) * kCols + warp] = ex2(ml.y - MO);
+      const float2 ml = ml_of(k);
+      const float f = ex2(ml.x - M);
+      L += ml.y * f;
+      weight[(k - first) * kCols + warp] = f;
     }
     L = warp_sum(L);
-    if (lane == 0) factor[warp] = ex2(MO - M) / L;
+    if (lane == 0) factor[warp] = 1.f / L;
   }
   __syncthreads();
   constexpr int kAtOnce = kJoinThreads / kJoinGroups;
@@ -709,7 +811,7 @@ cudaError_t launch_stream(const Kv8AttnArgs& a, int tile_from, bool beside, cuda
 
 // Bytes of a piece: Shape<dim, nt>::kPieceBytes.
 size_t piece_bytes(int dim, int nt) {
-  return (static_cast<size_t>(dim) / 16 * nt * 32 * 4 + 8 * nt * 4) * sizeof(float);
+  return (static_cast<size_t>(dim) / 16 * nt * 32 * 4 + 8 * nt * 2) * sizeof(float);
 }
 
 // Rows with this many columns (new tokens x query heads of a group) go to the

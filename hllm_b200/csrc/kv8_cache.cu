@@ -30,15 +30,6 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
                      __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
 }
 
-// The scale exponent of a row whose largest magnitude is `top` (finite, at
-// most kKv8Limit): the least e in [-24, 39] with top <= 448 * 2^e.  With
-// top = 1.f * 2^k, 448 = 1.75 * 2^8: e = k - 8, one more where 1.f > 1.75.
-__device__ __forceinline__ int scale_exponent(float top) {
-  const uint32_t b = __float_as_uint(top);
-  const int e = static_cast<int>(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return min(max(e, kKv8ExpMin), kKv8ExpMax);
-}
-
 // ---------------------------------------------------------------- write
 // Per token t and head h of qkv: y = x * (1 / sqrt(mean x^2 + eps)) * w for q
 // and k where weights are given; then for i < rotary / 2 the pair (i, i +
@@ -198,7 +189,7 @@ __global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(const Kv8Write
       }
     top = max_lanes(top);
     if (!is_q && live && stored) {
-      const int e = scale_exponent(top);
+      const int e = kv8_exponent(top);
       const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
       const int kvh = is_v ? h - hq - hkv : h - hq;
       const size_t at = (static_cast<size_t>(slot / kKv8Page) * hkv + kvh) * kKv8Page + slot % kKv8Page;
