@@ -31,13 +31,14 @@
 // that the columns are the 8-wide N side and one decode row wastes half of a
 // tile, not three quarters.  The order of the products' inner dimension is
 // free, so a lane takes 16 consecutive bytes of a key for the steps of QK, and
-// for PV the bytes of four keys, paired by byte permutes: what a lane copies
-// into shared memory, ahead of time (cp.async), it alone reads back.  No
-// barrier and no transpose is in the stream.
+// for PV the bytes of four keys, paired by byte permutes.  Pages arrive by TMA,
+// one lane of a warp asking for its warp's, in boxes whose swizzle spreads each
+// read over all banks (rows and the order of reads are chosen for that).
+#include <cudaTypedefs.h>
 #include <math.h>
 
 #include <algorithm>
-#include <type_traits>
+#include <mutex>
 
 #include "common.cuh"
 #include "kv8.cuh"
@@ -109,55 +110,70 @@ __device__ __forceinline__ void read_words(uint32_t (&w)[W], const uint8_t* p) {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
-// BYTES from global to shared memory, asynchronously; zeros where !live (WHOLE:
-// it always is).
-template <int BYTES, bool WHOLE>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool live) {
-  if constexpr (WHOLE && BYTES == 16) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  } else if constexpr (WHOLE) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
-  } else if constexpr (BYTES == 16) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0)
-                 : "memory");
-  } else {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src),
-                 "r"(live ? BYTES : 0), "n"(BYTES)
-                 : "memory");
-  }
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-template <int D, int NT>
-struct Shape {
-  // K: four lanes share a key row, KW words (of four codes) each, KS steps.
-  // V: eight lanes share a value row, VW words each, VS steps.
+// How a page of 16 keys x D codes lies in shared memory: boxes of BOX bytes of
+// every key, 16-byte chunks swizzled within 128 bytes by the key's line, and who
+// reads what.  K: four lanes (t) share a key row, KW words of four codes each,
+// KS steps.  V: eight lanes (g) share a value row, VW words each, VS steps.
+template <int D>
+struct Layout {
+  static constexpr int BOX = D % 128 == 0 ? 128 : D % 64 == 0 ? 64 : 32;
   static constexpr int KW = D % 64 == 0 ? 4 : 2, KS = D / (16 * KW);
   static constexpr int VW = D % 128 == 0 ? 4 : D % 64 == 0 ? 2 : 1, VS = D / (32 * VW);
+  __device__ static int swizzle(int row) {
+    return BOX == 128 ? row & 7 : BOX == 64 ? row >> 1 & 3 : row >> 2 & 1;
+  }
+  // Key of row g of the score product (and + 8 of row g + 8): with 128-byte
+  // boxes two neighbouring g take rows whose swizzles differ in bit 2.
+  __device__ static int key_of(int g) { return BOX == 128 ? (g >> 1) | (g & 1) << 2 : g; }
+  // Byte of lane (g, t)'s words of step s, key row g.
+  __device__ static int k_at(int g, int t, int s) {
+    const int row = key_of(g), byte = (s * 4 + t) * KW * 4;
+    return byte / BOX * (16 * BOX) + row * BOX + ((byte % BOX / 16 ^ swizzle(row)) << 4) + byte % 16;
+  }
+  // Value rows of lane t: keys value_key(t, 0 .. 3), in the order of the
+  // weights' fragment.  Some lanes read the first two, and the last two, in
+  // the other order, which makes eight reads reach all banks.
+  __device__ static int value_key(int t, int h) {
+    return (BOX == 128 ? t + 4 * (h & 1) : 2 * t + (h & 1)) + 8 * (h >> 1);
+  }
+  __device__ static bool swapped(int g, int t) {
+    return BOX == 128 ? g & 1 : BOX == 64 ? g >> 1 & 1 : t >> 1;
+  }
+  __device__ static int v_at(int g, int t, int h, int s) {
+    const int row = value_key(t, h), byte = (s * 8 + g) * VW * 4;
+    return byte / BOX * (16 * BOX) + row * BOX + ((byte % BOX / 16 ^ swizzle(row)) << 4) + byte % 16;
+  }
+};
+
+template <int D, int NT>
+struct Shape : Layout<D> {
+  using Layout<D>::VW;
   static constexpr int kCols = 8 * NT;
-  // 16 warps hide the latency of one page's chain of products; where the sums
-  // and the queries take more than half of 128 registers, 8 warps.
-  static constexpr int kWarps = D * NT <= 128 ? 16 : 8;
+  // Enough warps to hide the latency of one page's chain of products, with the
+  // registers for the sums and the queries.
+  static constexpr int kWarps = D * NT <= 128 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kStage = 32 * D + 32;  // a page's codes, each lane's own, and its scales
-  static constexpr int kVAt = 16 * D, kScalesAt = 32 * D;
   // A piece: D / 16 x NT fragments of 32 lanes x 4 sums, then cols x (m, l).
   static constexpr int kUnits = D / 16 * NT * 32;
   static constexpr int kPiece = kUnits * 4 + kCols * 2;  // floats
-  // A warp's shared memory: its ring, whose place the piece it leaves open
-  // takes at the end, and the piece it continues, which may be done earlier.
+  // A warp's shared memory: its ring of pages, whose place the piece it leaves
+  // open takes at the end; the piece it continues, which may be done earlier;
+  // the pages' scales and the ring's barriers.
+  static constexpr int kStage = 32 * D;  // codes of K, then of V
   static constexpr int kPieceBytes = kPiece * static_cast<int>(sizeof(float));
-  static constexpr int kRoom = 220 * 1024 / kWarps;
-  static constexpr int kStages = 3 * kStage + kPieceBytes <= kRoom ? 3 : 2;
-  static constexpr int kWarpBytes = kStages * kStage + kPieceBytes;
-  static constexpr int kSmem = kWarps * kWarpBytes;
-  static_assert(kStages * kStage >= kPieceBytes && kWarpBytes <= kRoom, "shared memory of a warp");
+  static constexpr int kRoom = 224 * 1024 / kWarps / 1024 * 1024;
+  __host__ __device__ static constexpr int bytes(int stages) {
+    return (stages * (kStage + 32 + 8) + kPieceBytes + 1023) / 1024 * 1024;
+  }
+  static constexpr int kStages = bytes(4) <= kRoom ? 4 : bytes(3) <= kRoom ? 3 : 2;
+  static constexpr int kWarpBytes = bytes(kStages);
+  static constexpr int kPieceAt = kStages * kStage, kScalesAt = kPieceAt + kPieceBytes;
+  static constexpr int kBarsAt = kScalesAt + kStages * 32;
+  static constexpr int kSmem = kWarps * kWarpBytes + 1024;  // 1024-byte alignment slack
+  static_assert(kPieceAt >= kPieceBytes && kWarpBytes <= kRoom, "shared memory of a warp");
+  static_assert(kScalesAt % 16 == 0 && kBarsAt % 8 == 0, "alignment");
   __device__ static float* piece(uint8_t* smem, int p) {
-    return reinterpret_cast<float*>(smem + (p >> 1) * kWarpBytes + (p & 1 ? 0 : kStages * kStage));
+    return reinterpret_cast<float*>(smem + (p >> 1) * kWarpBytes + (p & 1 ? 0 : kPieceAt));
   }
   // Value dimension of unit (i, lane): rows g and g + 8 of product i are
   // consecutive dimensions.
@@ -165,6 +181,11 @@ struct Shape {
     const int st = i / (2 * VW), rest = i % (2 * VW);
     return (st * 8 + g) * VW * 4 + rest * 2;
   }
+};
+
+// The code pools as boxes of BOX codes x one page: [page of a kv head][16][D].
+struct PoolMaps {
+  CUtensorMap k, v;
 };
 
 __device__ __forceinline__ long long row_units(const Kv8Row& x, int hkv) {
@@ -183,10 +204,13 @@ __device__ __forceinline__ int cut_owner(const Cut& c, long long unit) {
 }
 
 // The workspace: per CTA a record and two pieces (the stream it continues, the
-// stream it leaves open).
+// stream it leaves open).  The record is of a stream that earlier CTAs began
+// and this one ended: the CTA that began it (-1: there is none), and what its
+// output needs.
 struct Record {
-  int row, stream, first;  // first: the CTA that holds the stream's first unit; -1: nothing to join
-  int pad;
+  int first, kvh, x0;      // the stream's first column
+  int count, len, t0;      // of its row
+  int pad[2];
 };
 
 // The output of one unit of a finished stream: sums of columns 2t, 2t + 1 and
@@ -211,12 +235,17 @@ __device__ __forceinline__ void store_unit(const Kv8AttnArgs& a, const Kv8Row& x
 
 template <int D, int NT>
 __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
-    kv8_stream_kernel(const Kv8AttnArgs a, int group, int tile_from, bool beside) {
+    kv8_stream_kernel(const __grid_constant__ PoolMaps maps, const Kv8AttnArgs a, int group,
+                      int tile_from, bool beside) {
   using S = Shape<D, NT>;
   constexpr int kCols = S::kCols, kWarps = S::kWarps, ST = S::kStages;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int piece_row[kWarps * 2], piece_stream[kWarps * 2];
-  __shared__ bool piece_starts[kWarps * 2], piece_ends[kWarps * 2];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  // Pieces that warps leave: the row (-1: none), kv head, chunk, and whether the
+  // piece has the stream's first (1) and last (2) page.
+  __shared__ int4 left[kWarps * 2];
+  __shared__ int order[kWarps * 2 + 1], chains[kWarps * 2 + 1], chain_count;
   __shared__ long long units_before;  // units before the row of the CTA's first one
   // Launched behind the tile pass this one runs beside it: that pass lets its
   // successor start once all its CTAs have seen the work before them complete,
@@ -259,7 +288,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
 
   float o[NT][D / 16][4];
   float m[NT][2], l[NT][2];
-  if (lane < 2) piece_row[warp * 2 + lane] = -1;
+  uint8_t* const ring = smem + warp * S::kWarpBytes;
+  uint64_t* const full = reinterpret_cast<uint64_t*>(ring + S::kBarsAt);
+  if (lane < 2) left[warp * 2 + lane].x = -1;
+  if (lane == 0) {
+    for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+  }
   __syncwarp();
 
   if (n > 0) {
@@ -324,35 +359,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       }
     };
     int tab_row = -1, tab_q0 = 0, tab = -1;  // 32 entries of the block table, one a lane
-    uint8_t* ring = smem + warp * S::kWarpBytes;
     unsigned have = 0;  // bit s: stage s holds a page
-    const uint8_t* const kbase = a.cache.k + g * D + tq * S::KW * 4;
-    const uint8_t* const vbase = a.cache.v + 2 * tq * D + g * S::VW * 4;
-    const uint8_t* const sbase = (lane < 4 ? a.cache.k_scale : a.cache.v_scale) + (lane & 3) * 4;
-    const uint32_t kring = smem_u32(ring) + lane * S::KW * 4;
-    const uint32_t vring = smem_u32(ring) + S::kVAt + lane * S::VW * 4;
-    const uint32_t sring = smem_u32(ring) + S::kScalesAt + lane * 4;
-    auto copy_page = [&](int stage, int page, int valid, auto whole) {
-      const uint64_t off = static_cast<uint64_t>(static_cast<uint32_t>(page)) * (kKv8Page * D);
-      const uint8_t *kp = kbase + off, *vp = vbase + off;
-      const uint32_t kd = kring + stage * S::kStage, vd = vring + stage * S::kStage;
-      // Rows past the last key may hold anything: they are not read.
-#pragma unroll
-      for (int s = 0; s < S::KS; ++s)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          copy_async<S::KW * 4, decltype(whole)::value>(kd + (s * 2 + h) * S::KW * 128,
-                                                        kp + 8 * h * D + s * S::KW * 16, g + 8 * h < valid);
-#pragma unroll
-      for (int s = 0; s < S::VS; ++s)
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int key = (h & 1) + (h >> 1) * 8;
-          copy_async<S::VW * 4, decltype(whole)::value>(vd + (s * 4 + h) * S::VW * 128,
-                                                        vp + key * D + s * S::VW * 32, 2 * tq + key < valid);
-        }
-      if (lane < 8) copy_async<4, true>(sring + stage * S::kStage, sbase + static_cast<size_t>(page) * kKv8Page, true);
-    };
     auto fetch = [&](int stage) {
       if (ahead.row != tab_row || ahead.page < tab_q0 || ahead.page >= tab_q0 + 32) {
         tab_row = ahead.row;
@@ -363,15 +370,27 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
                   : -1;
       }
       const int b = __shfl_sync(0xffffffffu, tab, ahead.page - tab_q0);
-      const int valid = ahead.x.len - ahead.page * kKv8Page;  // keys of the page
-      const bool ok = valid > 0 && b >= 0 && b < a.cache.blocks;
+      const bool some = ahead.page * kKv8Page < ahead.x.len;
+      const bool ok = some && b >= 0 && b < a.cache.blocks;
       have = (have & ~(1u << stage)) | (ok ? 1u << stage : 0u);
-      if (ok) {
-        const int page = b * hkv + ahead.kvh;
-        if (valid >= kKv8Page) copy_page(stage, page, valid, std::true_type{});
-        else copy_page(stage, page, valid, std::false_type{});
-      } else if (valid > 0 && lane == 0) {
-        atomicOr(a.status, kDevBadIndex);
+      if (lane == 0) {
+        if (ok) {
+          const int page = b * hkv + ahead.kvh;
+          uint8_t* to = ring + stage * S::kStage;
+          uint8_t* scales = ring + S::kScalesAt + stage * 32;
+          uint64_t* bar = &full[stage];
+          mbar_arrive_expect_tx(bar, S::kStage + 32);
+#pragma unroll
+          for (int box = 0; box < D / S::BOX; ++box)
+            tma_load_3d(to + box * (16 * S::BOX), &maps.k, bar, box * S::BOX, 0, page);
+          bulk_load(scales, a.cache.k_scale + static_cast<size_t>(page) * kKv8Page, 16, bar);
+#pragma unroll
+          for (int box = 0; box < D / S::BOX; ++box)
+            tma_load_3d(to + 16 * D + box * (16 * S::BOX), &maps.v, bar, box * S::BOX, 0, page);
+          bulk_load(scales + 16, a.cache.v_scale + static_cast<size_t>(page) * kKv8Page, 16, bar);
+        } else if (some) {
+          atomicOr(a.status, kDevBadIndex);
+        }
       }
       advance(ahead);
     };
@@ -445,8 +464,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       edge = __reduce_min_sync(0xffffffffu, edge);
     };
 
-    auto multiply = [&](const uint8_t* page, bool ok) {
-      if (!ok) return;  // no keys here
+    // Swapped value rows (Layout) are put right by the permutes that pair them.
+    const bool swap = S::swapped(g, tq);
+    const uint32_t pair_lo = swap ? 0x1504u : 0x5140u, pair_hi = swap ? 0x3726u : 0x7362u;
+    const int mine = S::key_of(g);  // key of score row g
+    auto multiply = [&](const uint8_t* page, const uint8_t* scales) {
       float s[NT][3][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -457,8 +479,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
 #pragma unroll
       for (int st = 0; st < S::KS; ++st) {
         uint32_t k0[S::KW], k1[S::KW];
-        read_words<S::KW>(k0, page + (st * 2) * S::KW * 128 + lane * S::KW * 4);
-        read_words<S::KW>(k1, page + (st * 2 + 1) * S::KW * 128 + lane * S::KW * 4);
+        read_words<S::KW>(k0, page + S::k_at(g, tq, st));
+        read_words<S::KW>(k1, page + S::k_at(g, tq, st) + 8 * S::BOX);
 #pragma unroll
         for (int w = 0; w < S::KW; w += 2) {
           const int i = st * S::KW + w;
@@ -470,15 +492,16 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
                        qb[nt][part][i + 1]);
         }
       }
-      const uint8_t* sc = page + S::kScalesAt + g;
+      const uint8_t* sc = scales + mine;
       const float ks[2] = {__uint_as_float(static_cast<uint32_t>(sc[0]) << 23),
                            __uint_as_float(static_cast<uint32_t>(sc[8]) << 23)};
       // (A byte 0, which no write leaves, counts as the least normal number.)
       uint32_t vb[2] = {max(static_cast<uint32_t>(sc[16]), 1u), max(static_cast<uint32_t>(sc[24]), 1u)};
       float p[NT][4];
       float top = 0.f;
-      const int key = at.page * kKv8Page + g;
-      if ((at.page + 1) * kKv8Page - 1 > edge) {
+      const int key = at.page * kKv8Page + mine;
+      const bool at_edge = (at.page + 1) * kKv8Page - 1 > edge;
+      if (at_edge) {
         // A page that ends past the last key, or some column's.
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -548,12 +571,21 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
         uint32_t v[4][S::VW];
 #pragma unroll
         for (int h = 0; h < 4; ++h)
-          read_words<S::VW>(v[h], page + S::kVAt + (st * 4 + h) * S::VW * 128 + lane * S::VW * 4);
+          read_words<S::VW>(v[h], page + 16 * D + S::v_at(g, tq, h ^ (swap ? 1 : 0), st));
+        if (at_edge) {
+          // Rows past the last key may hold anything, NaN among it.
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            if (at.page * kKv8Page + S::value_key(tq, h ^ (swap ? 1 : 0)) >= at.x.len) {
+#pragma unroll
+              for (int w = 0; w < S::VW; ++w) v[h][w] = 0u;
+            }
+        }
 #pragma unroll
         for (int w = 0; w < S::VW; ++w)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t sel = h ? 0x7362u : 0x5140u;
+            const uint32_t sel = h ? pair_hi : pair_lo;
             const uint32_t lo = __byte_perm(v[0][w], v[1][w], sel);
             const uint32_t hi = __byte_perm(v[2][w], v[3][w], sel);
             const uint32_t a0 = kv8_half2_lo(lo), a1 = kv8_half2_hi(lo);
@@ -602,33 +634,27 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
           *reinterpret_cast<float4*>(piece + S::kUnits * 4 + (nt * 8 + 2 * tq) * 2) =
               make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]);
       }
-      if (lane == 0) {
-        piece_row[p] = at.row;
-        piece_stream[p] = at.kvh * at.x.chunks + at.chunk;
-        piece_starts[p] = starts;
-        piece_ends[p] = ends;
-      }
+      if (lane == 0) left[p] = make_int4(at.row, at.kvh, at.chunk, (starts ? 1 : 0) | (ends ? 2 : 0));
     };
 
 #pragma unroll
-    for (int i = 0; i < ST - 1; ++i) {
+    for (int i = 0; i < ST - 1; ++i)
       if (i < n) fetch(i);
-      copy_commit();
-    }
     open();
     int stage = 0, next = ST - 1;  // of the page at hand, and of the one to fetch
-#pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-      copy_wait<ST - 2>();
-      __syncwarp();  // the scales are other lanes' copies; the stage to fill is read by none
-      if (i + ST - 1 < n) fetch(next);
-      copy_commit();
-      multiply(ring + stage * S::kStage, (have >> stage) & 1u);
-      const bool ends = at.page == at.x.pages - 1;
-      if (ends || i + 1 == n) {
-        __syncwarp();  // an open piece takes the ring's place
-        close(ends);
+    unsigned phases = 0;           // bit s: parity of stage s's next page
+    int i = 0;
+    for (; i < n; ++i) {
+      const bool ok = have >> stage & 1u;
+      if (ok) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phases >> stage & 1u, a.status))) break;
+        phases ^= 1u << stage;
       }
+      if (i + ST - 1 < n) fetch(next);  // the stage that every lane has left behind
+      if (ok) multiply(ring + stage * S::kStage, ring + S::kScalesAt + stage * 32);
+      __syncwarp();
+      const bool ends = at.page == at.x.pages - 1;
+      if (ends || i + 1 == n) close(ends);
       if (i + 1 < n) {
         advance(at);
         if (at.page == 0) {
@@ -639,53 +665,67 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       stage = stage + 1 == ST ? 0 : stage + 1;
       next = next + 1 == ST ? 0 : next + 1;
     }
+    // After a wait that ran out: pages in flight land before the warp goes on (bounded too).
+    for (int k = 0; i < n && k < ST - 1 && i + k < n; ++k) {
+      const int f = (stage + k) % ST;
+      if (have >> f & 1u) mbar_wait(&full[f], phases >> f & 1u, a.status);
+    }
   }
   __syncthreads();
 
-  // Join the warps' pieces: a chain is a run of pieces of one stream.
-  Record rec{0, 0, -1, 0};
-  auto next_piece = [&](int from) {
-    while (from < kWarps * 2 && piece_row[from] < 0) ++from;
-    return from;
-  };
-  int i = next_piece(0);
-  while (i < kWarps * 2) {
-    const int row = piece_row[i], stream = piece_stream[i];
-    int last = i, j = next_piece(i + 1);
-    while (j < kWarps * 2 && piece_row[j] == row && piece_stream[j] == stream) {
-      last = j;
-      j = next_piece(j + 1);
+  // Join the warps' pieces: a chain is a run of pieces of one stream.  One warp
+  // lists the pieces that there are and where chains begin.
+  if (warp == 0) {
+    const int4 p = lane < kWarps * 2 ? left[lane] : make_int4(-1, 0, 0, 0);
+    const unsigned live = __ballot_sync(0xffffffffu, p.x >= 0);
+    const unsigned before = live & ((1u << lane) - 1u);
+    const int prev = before ? 31 - __clz(before) : lane;
+    const int row = __shfl_sync(0xffffffffu, p.x, prev), kvh = __shfl_sync(0xffffffffu, p.y, prev),
+              chunk = __shfl_sync(0xffffffffu, p.z, prev);
+    const bool begin = p.x >= 0 && (!before || row != p.x || kvh != p.y || chunk != p.z);
+    const unsigned begins = __ballot_sync(0xffffffffu, begin);
+    if (p.x >= 0) order[__popc(before)] = lane;
+    if (begin) chains[__popc(begins & ((1u << lane) - 1u))] = __popc(before);
+    if (lane == 0) {
+      chain_count = __popc(begins);
+      chains[__popc(begins)] = __popc(live);
     }
-    const bool begins = piece_starts[i], ends = piece_ends[last];
-    const Kv8Row x = kv8_row(a, row, group, kCols, tile_from, false);
-    const int kvh = stream / x.chunks, x0 = (stream % x.chunks) * kCols;
+  }
+  __syncthreads();
+  Record rec{-1, 0, 0, 0, 0, 0, {0, 0}};
+  for (int ch = 0; ch < chain_count; ++ch) {
+    const int k0 = chains[ch], k1 = chains[ch + 1];
+    const int4 p = left[order[k0]];
+    const bool begins = p.w & 1, ends = left[order[k1 - 1]].w & 2;
+    const Kv8Row x = kv8_row(a, p.x, group, kCols, tile_from, false);
+    const int kvh = p.y, x0 = p.z * kCols;
     float* dst = reinterpret_cast<float*>(records + gridDim.x) +
                  (static_cast<size_t>(blockIdx.x) * 2 + (begins ? 1 : 0)) * S::kPiece;
     for (int u = threadIdx.x; u < S::kUnits; u += S::kThreads) {
       const int nt = u / (D / 16 * 32), col = nt * 8 + 2 * (u & 3);
       if (x0 + col >= x.count * group) continue;
       auto ml_of = [&](int k) {  // (m, l) of the unit's two columns
-        return *reinterpret_cast<const float4*>(S::piece(smem, k) + S::kUnits * 4 + col * 2);
+        return *reinterpret_cast<const float4*>(S::piece(smem, order[k]) + S::kUnits * 4 + col * 2);
       };
       float2 M = make_float2(kNoReference, kNoReference), L = make_float2(0.f, 0.f);
-      for (int k = i; k <= last; ++k)
-        if (piece_row[k] >= 0) {
-          const float4 ml = ml_of(k);
-          M = make_float2(fmaxf(M.x, ml.x), fmaxf(M.y, ml.z));
-        }
+#pragma unroll 4
+      for (int k = k0; k < k1; ++k) {
+        const float4 ml = ml_of(k);
+        M = make_float2(fmaxf(M.x, ml.x), fmaxf(M.y, ml.z));
+      }
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = i; k <= last; ++k)
-        if (piece_row[k] >= 0) {
-          const float4 ml = ml_of(k);
-          const float f0 = ex2(ml.x - M.x), f1 = ex2(ml.z - M.y);
-          L.x += ml.y * f0;
-          L.y += ml.w * f1;
-          const float4 v = *reinterpret_cast<const float4*>(S::piece(smem, k) + u * 4);
-          acc.x += v.x * f0;
-          acc.y += v.y * f1;
-          acc.z += v.z * f0;
-          acc.w += v.w * f1;
-        }
+#pragma unroll 4
+      for (int k = k0; k < k1; ++k) {
+        const float4 ml = ml_of(k);
+        const float f0 = ex2(ml.x - M.x), f1 = ex2(ml.z - M.y);
+        L.x += ml.y * f0;
+        L.y += ml.w * f1;
+        const float4 v = *reinterpret_cast<const float4*>(S::piece(smem, order[k]) + u * 4);
+        acc.x += v.x * f0;
+        acc.y += v.y * f1;
+        acc.z += v.z * f0;
+        acc.w += v.w * f1;
+      }
       if (begins && ends) {
         store_unit(a, x, group, kvh, x0 + col, S::dim_of((u >> 5) % (D / 16), (u >> 2) & 7), acc,
                    1.f / L.x, 1.f / L.y);
@@ -698,97 +738,118 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     if (!begins && ends) {
       // The stream that earlier CTAs began ends here: the join pass takes it.
       // It is the CTA's first chain, so its row is the CTA's first.
-      rec.row = row;
-      rec.stream = stream;
-      rec.first = cut_owner(cut, units_before + static_cast<long long>(stream) * x.pages);
+      const long long stream = static_cast<long long>(kvh) * x.chunks + p.z;
+      rec = Record{cut_owner(cut, units_before + stream * x.pages), kvh, x0, x.count, x.len, x.t0, {0, 0}};
     }
-    i = j;
   }
   if (threadIdx.x == 0) records[blockIdx.x] = rec;
   if (beside) griddep_wait();
 }
 
 // Joins the pieces of a stream that spans CTAs, in order; one CTA for each CTA
-// of the stream pass, with work where that one ended such a stream.  A warp a
-// column finds the references and the pieces' weights; then the units are
-// summed, kJoinGroups shares of the pieces at a time.
-constexpr int kJoinThreads = 512, kJoinGroups = 4;
+// of the stream pass, with work where that one ended such a stream.  A thread
+// sums a unit over a share of the pieces; the shares meet in shared memory.
 template <int D, int NT>
-__global__ void __launch_bounds__(kJoinThreads)
-    kv8_join_kernel(const Kv8AttnArgs a, int group, int tile_from) {
+struct Join {
+  static constexpr int kUnits = Shape<D, NT>::kUnits;
+  static constexpr int kShares = kUnits <= 128 ? 4 : kUnits <= 256 ? 2 : 1;
+  static constexpr int kThreads = kUnits * kShares;
+};
+template <int D, int NT>
+__global__ void __launch_bounds__(Join<D, NT>::kThreads) kv8_join_kernel(const Kv8AttnArgs a, int group) {
   using S = Shape<D, NT>;
-  constexpr int kCols = S::kCols;
-  extern __shared__ __align__(16) float weight[];  // [pieces][kCols]
-  __shared__ float factor[kCols];
-  __shared__ float4 share[kJoinGroups - 1][kJoinThreads / kJoinGroups];
+  constexpr int kShares = Join<D, NT>::kShares;
+  __shared__ float4 sums[kShares > 1 ? kShares - 1 : 1][S::kUnits];
+  __shared__ float4 refs[kShares > 1 ? kShares - 1 : 1][S::kUnits];
   griddep_enter();
   const Record* records = reinterpret_cast<const Record*>(a.workspace);
   const Record rec = records[blockIdx.x];
   const int first = rec.first, end = blockIdx.x;
   if (first < 0 || first >= end) return;
-  const Kv8Row x = kv8_row(a, rec.row, group, kCols, tile_from, false);
-  if (x.chunks == 0) return;
-  const int kvh = rec.stream / x.chunks, x0 = (rec.stream % x.chunks) * kCols;
-  const int cols = min(kCols, x.count * group - x0);
   const float* base = reinterpret_cast<const float*>(records + gridDim.x);
+  const int u = threadIdx.x % S::kUnits, share = threadIdx.x / S::kUnits;
+  const int col = u / (D / 16 * 32) * 8 + 2 * (u & 3);
+  const bool live = rec.x0 + col < rec.count * group;
   // Piece of CTA c: the one it left open for the first, else the one it continued.
   auto piece = [&](int c) {
     return base + (static_cast<size_t>(c) * 2 + (c == first ? 1 : 0)) * S::kPiece;
   };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp < cols) {
-    auto ml_of = [&](int k) {
-      return __ldcg(reinterpret_cast<const float2*>(piece(k) + S::kUnits * 4) + warp);
-    };
-    float M = kNoReference;
-    for (int k = first + lane; k <= end; k += 32) M = fmaxf(M, ml_of(k).x);
-    M = warp_max(M);
-    float L = 0.f;
-    for (int k = first + lane; k <= end; k += 32) {
-      const float2 ml = ml_of(k);
-      const float f = ex2(ml.x - M);
-      L += ml.y * f;
-      weight[(k - first) * kCols + warp] = f;
-    }
-    L = warp_sum(L);
-    if (lane == 0) factor[warp] = 1.f / L;
-  }
-  __syncthreads();
-  constexpr int kAtOnce = kJoinThreads / kJoinGroups;
-  const int part = threadIdx.x / kAtOnce, mine = threadIdx.x % kAtOnce;
-  for (int u0 = 0; u0 < S::kUnits; u0 += kAtOnce) {
-    const int u = u0 + mine;
-    const int col = u / (D / 16 * 32) * 8 + 2 * (u & 3);
-    const bool live = u < S::kUnits && col < cols;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live) {
+  auto ml_of = [&](int c) {
+    return __ldcg(reinterpret_cast<const float4*>(piece(c) + S::kUnits * 4 + col * 2));
+  };
+  float2 M = make_float2(kNoReference, kNoReference), L = make_float2(0.f, 0.f);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
 #pragma unroll 8
-      for (int k = first + part; k <= end; k += kJoinGroups) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(k) + u * 4));
-        const float f0 = weight[(k - first) * kCols + col];
-        const float f1 = col + 1 < cols ? weight[(k - first) * kCols + col + 1] : 0.f;
-        acc.x += v.x * f0;
-        acc.y += v.y * f1;
-        acc.z += v.z * f0;
-        acc.w += v.w * f1;
-      }
+    for (int k = first + share; k <= end; k += kShares) {
+      const float4 ml = ml_of(k);
+      M = make_float2(fmaxf(M.x, ml.x), fmaxf(M.y, ml.z));
     }
-    if (part > 0) share[part - 1][mine] = acc;
-    __syncthreads();
-    if (part == 0 && live) {
-#pragma unroll
-      for (int p = 0; p < kJoinGroups - 1; ++p) {
-        const float4 v = share[p][mine];
-        acc.x += v.x;
-        acc.y += v.y;
-        acc.z += v.z;
-        acc.w += v.w;
-      }
-      store_unit(a, x, group, kvh, x0 + col, S::dim_of((u >> 5) % (D / 16), (u >> 2) & 7), acc,
-                 factor[col], col + 1 < cols ? factor[col + 1] : 0.f);
+#pragma unroll 8
+    for (int k = first + share; k <= end; k += kShares) {
+      const float4 ml = ml_of(k);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(k) + u * 4));
+      const float f0 = ex2(ml.x - M.x), f1 = ex2(ml.z - M.y);
+      L.x += ml.y * f0;
+      L.y += ml.w * f1;
+      acc.x += v.x * f0;
+      acc.y += v.y * f1;
+      acc.z += v.z * f0;
+      acc.w += v.w * f1;
+    }
+  }
+  if (kShares > 1) {
+    if (share > 0) {
+      sums[share - 1][u] = acc;
+      refs[share - 1][u] = make_float4(M.x, L.x, M.y, L.y);
     }
     __syncthreads();
   }
+  if (share > 0 || !live) return;
+#pragma unroll
+  for (int p = 0; p < kShares - 1; ++p) {
+    const float4 ml = refs[p][u], v = sums[p][u];
+    const float m0 = fmaxf(M.x, ml.x), m1 = fmaxf(M.y, ml.z);
+    const float f0 = ex2(M.x - m0), f1 = ex2(M.y - m1), g0 = ex2(ml.x - m0), g1 = ex2(ml.z - m1);
+    M = make_float2(m0, m1);
+    L = make_float2(L.x * f0 + ml.y * g0, L.y * f1 + ml.w * g1);
+    acc = make_float4(acc.x * f0 + v.x * g0, acc.y * f1 + v.y * g1, acc.z * f0 + v.z * g0,
+                      acc.w * f1 + v.w * g1);
+  }
+  const Kv8Row x{rec.count, rec.len, rec.t0, 0, 0};
+  store_unit(a, x, group, rec.kvh, rec.x0 + col, S::dim_of((u >> 5) % (D / 16), (u >> 2) & 7), acc,
+             1.f / L.x, 1.f / L.y);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+bool make_maps(PoolMaps* maps, const Kv8Cache& c, int box) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(c.dim), kKv8Page,
+                              static_cast<cuuint64_t>(c.blocks) * c.hkv};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(c.dim), static_cast<cuuint64_t>(c.dim) * kKv8Page};
+  const cuuint32_t boxes[3] = {static_cast<cuuint32_t>(box), kKv8Page, 1}, ones[3] = {1, 1, 1};
+  const CUtensorMapSwizzle swizzle = box == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : box == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                 : CU_TENSOR_MAP_SWIZZLE_32B;
+  for (int v = 0; v < 2; ++v)
+    if (fn(v ? &maps->v : &maps->k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, v ? c.v : c.k, dims, strides, boxes,
+           ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+  return true;
 }
 
 int stream_ctas(int sm_count) { return sm_count; }
@@ -796,17 +857,18 @@ int stream_ctas(int sm_count) { return sm_count; }
 template <int D, int NT>
 cudaError_t launch_stream(const Kv8AttnArgs& a, int tile_from, bool beside, cudaStream_t stream) {
   using S = Shape<D, NT>;
+  PoolMaps maps;
+  if (!make_maps(&maps, a.cache, S::BOX)) return cudaErrorUnknown;
   static Kv8Configured configured;
   cudaError_t e = configured.once(kv8_stream_kernel<D, NT>, S::kSmem);
   if (e != cudaSuccess) return e;
   const int group = a.hq / a.cache.hkv;
   const int ctas = stream_ctas(a.sm_count);
-  e = launch_dependent(kv8_stream_kernel<D, NT>, dim3(ctas), dim3(S::kThreads), S::kSmem, stream, a,
-                       group, tile_from, beside);
+  e = launch_dependent(kv8_stream_kernel<D, NT>, dim3(ctas), dim3(S::kThreads), S::kSmem, stream,
+                       maps, a, group, tile_from, beside);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kv8_join_kernel<D, NT>, dim3(ctas), dim3(kJoinThreads),
-                          static_cast<size_t>(ctas) * S::kCols * sizeof(float), stream, a, group,
-                          tile_from);
+  return launch_dependent(kv8_join_kernel<D, NT>, dim3(ctas), dim3(Join<D, NT>::kThreads), 0, stream, a,
+                          group);
 }
 
 // Bytes of a piece: Shape<dim, nt>::kPieceBytes.
