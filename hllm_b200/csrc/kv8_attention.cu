@@ -11,26 +11,22 @@
 // value rows.  It is raised only when a weight passes 2^8: most pages rescale
 // nothing.
 //
-// q.c_j is a product of e4m3 operands: q is the sum of three e4m3 vectors at
-// scales 2^e, 2^(e-4) and 2^(e-8), each the rounding of what the former left.
-// Three times four bits hold the 11 of F16, so nothing of q is lost (but 2^-26
-// of a head's largest element in its small ones), the codes go into the product
-// as they are, and it runs four times faster than one of F16 operands.
-//
 // Work.  A row's new tokens and the query heads of one kv head form columns
-// (token, head), 8 NT of them a stream; a stream walks the row's pages.  The
-// batch's (row, stream, page) units in order are one sequence, cut evenly over
+// (token, head), 8 NT of them a stream; a stream walks the row's pages, two at a
+// time (a unit).  The batch's units in order are one sequence, cut evenly over
 // the CTAs of one wave and, within a CTA, over its warps, whatever the rows'
 // lengths.  Everything about the cut follows from the lengths on the device:
 // a captured launch serves any lengths.  What a cut leaves of a stream is
 // joined first in the CTA (shared memory), then, where a stream spans CTAs, by
 // a second small launch, in order: results do not depend on timing.
 //
-// Per page a warp computes S^T = K Q^T (m16n8k32, e4m3) and O^T = V^T P^T
-// (m16n8k16, F16): the 16 keys, then 16 value dimensions, are the M side, so
-// that the columns are the 8-wide N side and one decode row wastes half of a
+// Per page a warp computes S^T = K Q^T and O^T = V^T P^T with m16n8k16 F16
+// products, codes becoming F16 in registers (exactly; a product of e4m3 operands
+// would not be faster: mma.sync runs it as F16 products after converting both).
+// The 16 keys, then 16 value dimensions, are the M side, so that the columns are
+// the 8-wide N side and one decode row wastes half of a
 // tile, not three quarters.  The order of the products' inner dimension is
-// free, so a lane takes 16 consecutive bytes of a key for the steps of QK, and
+// free, so a lane takes 16 consecutive bytes of a key for four steps of QK, and
 // for PV the bytes of four keys, paired by byte permutes.  Pages arrive by TMA,
 // one lane of a warp asking for its warp's, in boxes whose swizzle spreads each
 // read over all banks (rows and the order of reads are chosen for that).
@@ -46,7 +42,7 @@
 namespace hb {
 namespace {
 
-constexpr int kLeast = 4;               // pages of a CTA, where there are so many
+constexpr int kLeast = 2;               // units of a CTA, where there are so many
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -55,37 +51,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, "
-      "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// Two F16 values as e4m3 codes (low half), and back.
-__device__ __forceinline__ uint32_t codes_of_half2(uint32_t h) {
-  uint32_t w;
-  asm("{\n\t.reg .b16 c;\n\tcvt.rn.satfinite.e4m3x2.f16x2 c, %1;\n\tcvt.u32.u16 %0, c;\n\t}"
-      : "=r"(w)
-      : "r"(h));
-  return w;
-}
-// Takes the e4m3 rounding of x (four F16 values) out of it: the codes, and what
-// is left times 16.
-__device__ __forceinline__ uint32_t take_codes(uint32_t (&x)[2]) {
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t c = codes_of_half2(x[i]);
-    const uint32_t v = kv8_half2_lo(c);
-    const __half2 left = __hsub2(*reinterpret_cast<const __half2*>(&x[i]), *reinterpret_cast<const __half2*>(&v));
-    const __half2 r = __hmul2(left, __floats2half2_rn(16.f, 16.f));
-    x[i] = *reinterpret_cast<const uint32_t*>(&r);
-    w |= c << (16 * i);
-  }
-  return w;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t o;
@@ -145,13 +110,24 @@ struct Layout {
   }
 };
 
+// Four bytes from global to shared memory, asynchronously (zeros where !live),
+// and the arrival on a barrier once a lane's copies have landed.
+__device__ __forceinline__ void copy4_async(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 template <int D, int NT>
 struct Shape : Layout<D> {
   using Layout<D>::VW;
   static constexpr int kCols = 8 * NT;
   // Enough warps to hide the latency of one page's chain of products, with the
   // registers for the sums and the queries.
-  static constexpr int kWarps = D * NT <= 128 ? 12 : 8;
+  static constexpr int KP = D <= 128 && NT == 1 ? 2 : 1;  // pages of a unit: two chains of products in flight
+  static constexpr int kWarps = D * NT > 128 ? 8 : KP == 2 && D > 64 ? 10 : 12;
   static constexpr int kThreads = kWarps * 32;
   // A piece: D / 16 x NT fragments of 32 lanes x 4 sums, then cols x (m, l).
   static constexpr int kUnits = D / 16 * NT * 32;
@@ -159,16 +135,17 @@ struct Shape : Layout<D> {
   // A warp's shared memory: its ring of pages, whose place the piece it leaves
   // open takes at the end; the piece it continues, which may be done earlier;
   // the pages' scales and the ring's barriers.
-  static constexpr int kStage = 32 * D;  // codes of K, then of V
+  static constexpr int kPage = 32 * D;  // codes of K, then of V
+  static constexpr int kStage = KP * kPage;
   static constexpr int kPieceBytes = kPiece * static_cast<int>(sizeof(float));
   static constexpr int kRoom = 224 * 1024 / kWarps / 1024 * 1024;
   __host__ __device__ static constexpr int bytes(int stages) {
-    return (stages * (kStage + 32 + 8) + kPieceBytes + 1023) / 1024 * 1024;
+    return (stages * (kStage + 32 * KP + 8) + kPieceBytes + 1023) / 1024 * 1024;
   }
   static constexpr int kStages = bytes(4) <= kRoom ? 4 : bytes(3) <= kRoom ? 3 : 2;
   static constexpr int kWarpBytes = bytes(kStages);
   static constexpr int kPieceAt = kStages * kStage, kScalesAt = kPieceAt + kPieceBytes;
-  static constexpr int kBarsAt = kScalesAt + kStages * 32;
+  static constexpr int kBarsAt = kScalesAt + kStages * 32 * KP;
   static constexpr int kSmem = kWarps * kWarpBytes + 1024;  // 1024-byte alignment slack
   static_assert(kPieceAt >= kPieceBytes && kWarpBytes <= kRoom, "shared memory of a warp");
   static_assert(kScalesAt % 16 == 0 && kBarsAt % 8 == 0, "alignment");
@@ -188,8 +165,14 @@ struct PoolMaps {
   CUtensorMap k, v;
 };
 
+// Units of one stream of a row, of KP pages, and of all its streams.
+template <int KP>
+__device__ __forceinline__ int stream_units(const Kv8Row& x) {
+  return (x.pages + KP - 1) / KP;
+}
+template <int KP>
 __device__ __forceinline__ long long row_units(const Kv8Row& x, int hkv) {
-  return static_cast<long long>(x.chunks) * hkv * x.pages;
+  return static_cast<long long>(x.chunks) * hkv * stream_units<KP>(x);
 }
 
 struct Cut {
@@ -238,7 +221,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     kv8_stream_kernel(const __grid_constant__ PoolMaps maps, const Kv8AttnArgs a, int group,
                       int tile_from, bool beside) {
   using S = Shape<D, NT>;
-  constexpr int kCols = S::kCols, kWarps = S::kWarps, ST = S::kStages;
+  constexpr int kCols = S::kCols, kWarps = S::kWarps, ST = S::kStages, KP = S::KP;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -264,7 +247,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int r = base + 32 * k + lane;
-      mine[k] = r < a.rows ? row_units(kv8_row(a, r, group, kCols, tile_from,
+      mine[k] = r < a.rows ? row_units<KP>(kv8_row(a, r, group, kCols, tile_from,
                                                 blockIdx.x == 0 && warp == 0), hkv)
                            : 0;
     }
@@ -273,7 +256,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     cut.total += n;
   }
-  // A CTA takes kLeast pages at least, where there are so many.
+  // A CTA takes kLeast units at least, where there are so many.
   cut.ctas = static_cast<int>(
       min(static_cast<long long>(gridDim.x), max(1LL, (cut.total + kLeast - 1) / kLeast)));
   Record* records = reinterpret_cast<Record*>(a.workspace);
@@ -292,7 +275,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
   uint64_t* const full = reinterpret_cast<uint64_t*>(ring + S::kBarsAt);
   if (lane < 2) left[warp * 2 + lane].x = -1;
   if (lane == 0) {
-    for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1);
+    for (int i = 0; i < ST; ++i) mbar_init(&full[i], 33);  // the boxes, and every lane's scales
     fence_mbar_init();
   }
   __syncwarp();
@@ -306,7 +289,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
         for (int k = 0; k < 4; ++k) {
           const int r = base + 32 * k + lane;
           mine[k] =
-              r < a.rows ? row_units(kv8_row(a, r, group, kCols, tile_from, false), hkv) : 0;
+              r < a.rows ? row_units<KP>(kv8_row(a, r, group, kCols, tile_from, false), hkv) : 0;
         }
       }
 #pragma unroll
@@ -329,76 +312,93 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       }
     }
     if (w0 == c0 && lane == 0) units_before = before;
-    Kv8Row x = kv8_row(a, row, group, kCols, tile_from, false);
     const float sl2 = a.scale * kLog2e;
     // Where the arithmetic is, and the loader, ST - 1 units ahead of it.
     struct Cursor {
-      int row, kvh, chunk, page;
+      int row, kvh, chunk, unit, units;  // units: of the stream
       Kv8Row x;
     };
     Cursor at;
     at.row = row;
     at.x = kv8_row(a, row, group, kCols, tile_from, false);
-    at.page = static_cast<int>((w0 - before) % at.x.pages);
+    at.units = stream_units<KP>(at.x);
     {
-      const int stream = static_cast<int>((w0 - before) / at.x.pages);
+      at.unit = static_cast<int>((w0 - before) % at.units);
+      const int stream = static_cast<int>((w0 - before) / at.units);
       at.kvh = stream / at.x.chunks;
       at.chunk = stream % at.x.chunks;
     }
     Cursor ahead = at;
     auto advance = [&](Cursor& c) {
-      if (++c.page < c.x.pages) return;
-      c.page = 0;
+      if (++c.unit < c.units) return;
+      c.unit = 0;
       if (++c.chunk < c.x.chunks) return;
       c.chunk = 0;
       if (++c.kvh < hkv) return;
       c.kvh = 0;
       while (++c.row < a.rows) {
         c.x = kv8_row(a, c.row, group, kCols, tile_from, false);
+        c.units = stream_units<KP>(c.x);
         if (c.x.chunks) return;
       }
     };
     int tab_row = -1, tab_q0 = 0, tab = -1;  // 32 entries of the block table, one a lane
-    unsigned have = 0;  // bit s: stage s holds a page
+    unsigned have = 0;                       // bit stage * KP + j: page j of the stage is there
     auto fetch = [&](int stage) {
-      if (ahead.row != tab_row || ahead.page < tab_q0 || ahead.page >= tab_q0 + 32) {
+      const int q0 = ahead.unit * KP;
+      if (ahead.row != tab_row || q0 < tab_q0 || q0 + KP > tab_q0 + 32) {
         tab_row = ahead.row;
-        tab_q0 = ahead.page;
-        const int i = ahead.page + lane;
-        tab = i < ahead.x.pages && i < a.max_blocks
+        tab_q0 = q0;
+        const int i = q0 + lane;
+        // Entries past the last key's page may hold anything.
+        tab = i < a.max_blocks && i * kKv8Page < ahead.x.len
                   ? __ldg(a.tables + static_cast<size_t>(ahead.row) * a.max_blocks + i)
-                  : -1;
+                  : -2;
+        if (tab != -2 && (tab < 0 || tab >= a.cache.blocks)) tab = -1;
       }
-      const int b = __shfl_sync(0xffffffffu, tab, ahead.page - tab_q0);
-      const bool some = ahead.page * kKv8Page < ahead.x.len;
-      const bool ok = some && b >= 0 && b < a.cache.blocks;
-      have = (have & ~(1u << stage)) | (ok ? 1u << stage : 0u);
+      uint64_t* const bar = &full[stage];
+      const uint32_t scales = smem_u32(ring + S::kScalesAt + stage * (32 * KP));
+      // Scales: eight words a page, four of K and four of V.
+      {
+        const int b = __shfl_sync(0xffffffffu, tab, q0 - tab_q0 + (lane >> 3 & (KP - 1)));
+        if (lane < 8 * KP) {
+          const size_t page = static_cast<size_t>(max(b, 0)) * hkv + ahead.kvh;
+          copy4_async(scales + lane * 4,
+                      (lane & 4 ? a.cache.v_scale : a.cache.k_scale) + page * kKv8Page + (lane & 3) * 4,
+                      b >= 0);
+        }
+        copy_arrive(bar);
+      }
+      int b[KP], there = 0;
+#pragma unroll
+      for (int j = 0; j < KP; ++j) {
+        b[j] = __shfl_sync(0xffffffffu, tab, q0 - tab_q0 + j);
+        there |= b[j] >= 0 ? 1 << j : 0;
+      }
+      have = (have & ~(((1u << KP) - 1u) << (stage * KP))) | static_cast<unsigned>(there) << (stage * KP);
       if (lane == 0) {
-        if (ok) {
-          const int page = b * hkv + ahead.kvh;
-          uint8_t* to = ring + stage * S::kStage;
-          uint8_t* scales = ring + S::kScalesAt + stage * 32;
-          uint64_t* bar = &full[stage];
-          mbar_arrive_expect_tx(bar, S::kStage + 32);
+        mbar_arrive_expect_tx(bar, __popc(there) * S::kPage);
+        uint8_t* to = ring + stage * S::kStage;
 #pragma unroll
-          for (int box = 0; box < D / S::BOX; ++box)
-            tma_load_3d(to + box * (16 * S::BOX), &maps.k, bar, box * S::BOX, 0, page);
-          bulk_load(scales, a.cache.k_scale + static_cast<size_t>(page) * kKv8Page, 16, bar);
+        for (int j = 0; j < KP; ++j) {
+          if (b[j] >= 0) {
+            const int page = b[j] * hkv + ahead.kvh;
 #pragma unroll
-          for (int box = 0; box < D / S::BOX; ++box)
-            tma_load_3d(to + 16 * D + box * (16 * S::BOX), &maps.v, bar, box * S::BOX, 0, page);
-          bulk_load(scales + 16, a.cache.v_scale + static_cast<size_t>(page) * kKv8Page, 16, bar);
-        } else if (some) {
-          atomicOr(a.status, kDevBadIndex);
+            for (int box = 0; box < D / S::BOX; ++box) {
+              tma_load_3d(to + j * S::kPage + box * (16 * S::BOX), &maps.k, bar, box * S::BOX, 0, page);
+              tma_load_3d(to + j * S::kPage + 16 * D + box * (16 * S::BOX), &maps.v, bar, box * S::BOX, 0,
+                          page);
+            }
+          } else if (b[j] == -1) {
+            atomicOr(a.status, kDevBadIndex);
+          }
         }
       }
       advance(ahead);
     };
 
-    uint32_t qb[NT][3][D / 16];  // e4m3 parts of the queries: words of four, as the keys'
-    float qs[NT];                // 2^e of column g of an n-tile
-    float cs[NT][2];             // score scale of columns 2t, 2t + 1
-    int lim[NT][2];              // last key that these columns see
+    uint32_t qb[NT][D / 16][2];  // the queries as B fragments, in the keys' order
+    int lim[NT][2];              // last key that columns 2t, 2t + 1 see
     int edge;                    // least of them over the stream's columns
 
     auto open = [&]() {
@@ -410,7 +410,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
         const bool live = c < cols;
         const __half* src = a.q + static_cast<size_t>(at.x.t0 + (live ? c / group : 0)) * a.ld_q +
                             static_cast<size_t>(at.kvh * group + (live ? c % group : 0)) * D;
-        uint32_t h[D / 16][2];
 #pragma unroll
         for (int s = 0; s < S::KS; ++s)
 #pragma unroll
@@ -418,48 +417,22 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
             const uint2 v =
                 live ? __ldg(reinterpret_cast<const uint2*>(src + ((s * 4 + tq) * S::KW + w) * 4))
                      : make_uint2(0u, 0u);
-            h[s * S::KW + w][0] = v.x;
-            h[s * S::KW + w][1] = v.y;
-          }
-        // The head's largest element goes to 224 .. 448.
-        __half2 top = __floats2half2_rn(0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<const __half2*>(&h[i][e])));
-        float mx = fmaxf(__low2float(top), __high2float(top));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const int e = max(kv8_exponent(mx), -14);
-        // A query that is not finite gives NaN.
-        const float f = mx <= 65504.f ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23)
-                                      : __uint_as_float(0x7fffffffu);
-        qs[nt] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-        const __half2 f2 = __floats2half2_rn(f, f);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h[i][k]), f2);
-            h[i][k] = *reinterpret_cast<const uint32_t*>(&r);
+            qb[nt][s * S::KW + w][0] = v.x;
+            qb[nt][s * S::KW + w][1] = v.y;
           }
 #pragma unroll
-          for (int part = 0; part < 3; ++part) qb[nt][part][i] = take_codes(h[i]);
-        }
-#pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-          const int cc = x0 + nt * 8 + 2 * tq + e2;
+        for (int e = 0; e < 2; ++e) {
+          const int cc = x0 + nt * 8 + 2 * tq + e;
           // Columns beyond the stream's see everything; nothing of them is stored.
-          lim[nt][e2] = cc < cols ? max(-1, at.x.len - at.x.count + cc / group) : 0x7fffffff;
-          edge = min(edge, lim[nt][e2]);
-          cs[nt][e2] = __shfl_sync(0xffffffffu, qs[nt], (2 * tq + e2) * 4) * sl2;
-          m[nt][e2] = kNoReference;
-          l[nt][e2] = 0.f;
+          lim[nt][e] = cc < cols ? max(-1, at.x.len - at.x.count + cc / group) : 0x7fffffff;
+          edge = min(edge, lim[nt][e]);
+          m[nt][e] = kNoReference;
+          l[nt][e] = 0.f;
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-          for (int e2 = 0; e2 < 4; ++e2) o[nt][i][e2] = 0.f;
+          for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
       }
       edge = __reduce_min_sync(0xffffffffu, edge);
     };
@@ -468,81 +441,95 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     const bool swap = S::swapped(g, tq);
     const uint32_t pair_lo = swap ? 0x1504u : 0x5140u, pair_hi = swap ? 0x3726u : 0x7362u;
     const int mine = S::key_of(g);  // key of score row g
-    auto multiply = [&](const uint8_t* page, const uint8_t* scales) {
-      float s[NT][3][4];
+    auto multiply = [&](const uint8_t* unit, const uint8_t* scales, unsigned there) {
+      float s[KP][NT][2][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int part = 0; part < 3; ++part)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][part][e] = 0.f;
-#pragma unroll
-      for (int st = 0; st < S::KS; ++st) {
-        uint32_t k0[S::KW], k1[S::KW];
-        read_words<S::KW>(k0, page + S::k_at(g, tq, st));
-        read_words<S::KW>(k1, page + S::k_at(g, tq, st) + 8 * S::BOX);
-#pragma unroll
-        for (int w = 0; w < S::KW; w += 2) {
-          const int i = st * S::KW + w;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int part = 0; part < 3; ++part)
-              mma16832(s[nt][part], k0[w], k1[w], k0[w + 1], k1[w + 1], qb[nt][part][i],
-                       qb[nt][part][i + 1]);
-        }
-      }
-      const uint8_t* sc = scales + mine;
-      const float ks[2] = {__uint_as_float(static_cast<uint32_t>(sc[0]) << 23),
-                           __uint_as_float(static_cast<uint32_t>(sc[8]) << 23)};
-      // (A byte 0, which no write leaves, counts as the least normal number.)
-      uint32_t vb[2] = {max(static_cast<uint32_t>(sc[16]), 1u), max(static_cast<uint32_t>(sc[24]), 1u)};
-      float p[NT][4];
-      float top = 0.f;
-      const int key = at.page * kKv8Page + mine;
-      const bool at_edge = (at.page + 1) * kKv8Page - 1 > edge;
-      if (at_edge) {
-        // A page that ends past the last key, or some column's.
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (key + 8 * h >= at.x.len) vb[h] = 127u;
+      for (int j = 0; j < KP; ++j) {
+        const uint8_t* page = unit + j * S::kPage;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float v = fmaf(fmaf(s[nt][2][e], 0.0625f, s[nt][1][e]), 0.0625f, s[nt][0][e]) *
-                            (ks[e >> 1] * cs[nt][e & 1]);
-            s[nt][0][e] = key + (e >> 1) * 8 <= lim[nt][e & 1] ? v : -INFINITY;
+          for (int e = 0; e < 4; ++e) s[j][nt][0][e] = s[j][nt][1][e] = 0.f;
+#pragma unroll
+        for (int st = 0; st < S::KS; ++st) {
+          uint32_t k0[S::KW], k1[S::KW];
+          read_words<S::KW>(k0, page + S::k_at(g, tq, st));
+          read_words<S::KW>(k1, page + S::k_at(g, tq, st) + 8 * S::BOX);
+#pragma unroll
+          for (int w = 0; w < S::KW; ++w) {
+            const int i = st * S::KW + w;
+            const uint32_t a0 = kv8_half2_lo(k0[w]), a2 = kv8_half2_hi(k0[w]);
+            const uint32_t a1 = kv8_half2_lo(k1[w]), a3 = kv8_half2_hi(k1[w]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816(s[j][nt][i & 1], a0, a1, a2, a3, qb[nt][i][0], qb[nt][i][1]);
           }
-      } else {
+        }
+      }
+      float ks[KP][2];
+      uint32_t vb[KP][2];
+#pragma unroll
+      for (int j = 0; j < KP; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t* sc = scales + j * 32 + mine + 8 * h;
+          ks[j][h] = __uint_as_float(static_cast<uint32_t>(sc[0]) << 23) * sl2;
+          // (A byte 0, which no write leaves, counts as the least normal number.)
+          vb[j][h] = max(static_cast<uint32_t>(sc[16]), 1u);
+        }
+#pragma unroll
+      for (int j = 0; j < KP; ++j)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            s[nt][0][e] = fmaf(fmaf(s[nt][2][e], 0.0625f, s[nt][1][e]), 0.0625f, s[nt][0][e]) *
-                          (ks[e >> 1] * cs[nt][e & 1]);
+            s[j][nt][0][e] = (s[j][nt][0][e] + s[j][nt][1][e]) * ks[j][e >> 1];
+      const int key = at.unit * (KP * kKv8Page);
+      const bool at_edge = key + KP * kKv8Page - 1 > edge || there != (1u << KP) - 1u;
+      int end[KP];  // first key of the page that is not there
+#pragma unroll
+      for (int j = 0; j < KP; ++j) end[j] = there >> j & 1u ? at.x.len : 0;
+      if (at_edge) {
+        // A unit that ends past the last key or some column's, or lacks a page.
+#pragma unroll
+        for (int j = 0; j < KP; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k = key + j * kKv8Page + mine + 8 * h;
+            if (k >= end[j]) vb[j][h] = 127u;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (k > lim[nt][e] || k >= end[j]) s[j][nt][0][2 * h + e] = -INFINITY;
+          }
       }
-      const float vs[2] = {__uint_as_float(vb[0] << 23), __uint_as_float(vb[1] << 23)};
+      float p[KP][NT][4], top;
       auto weigh = [&]() {
         top = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int j = 0; j < KP; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[nt][1][e] = ex2(s[nt][0][e] - m[nt][e & 1]);
-            p[nt][e] = s[nt][1][e] * vs[e >> 1];
-            top = fmaxf(top, p[nt][e]);
-          }
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s[j][nt][1][e] = ex2(s[j][nt][0][e] - m[nt][e & 1]);
+              p[j][nt][e] = s[j][nt][1][e] * __uint_as_float(vb[j][e >> 1] << 23);
+              top = fmaxf(top, p[j][nt][e]);
+            }
       };
       weigh();
       if (__any_sync(0xffffffffu, top > kMostWeight)) {
-        const float ev[2] = {static_cast<float>(static_cast<int>(vb[0]) - 127),
-                             static_cast<float>(static_cast<int>(vb[1]) - 127)};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(s[nt][0][e] + ev[0], s[nt][0][e + 2] + ev[1]);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < KP; ++j)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                mx = fmaxf(mx, s[j][nt][0][2 * h + e] + static_cast<float>(static_cast<int>(vb[j][h]) - 127));
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
             if (mx > m[nt][e]) {
@@ -558,42 +545,46 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
           }
         weigh();
       }
-      uint32_t pb[NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        l[nt][0] += s[nt][1][0] + s[nt][1][2];
-        l[nt][1] += s[nt][1][1] + s[nt][1][3];
-        pb[nt][0] = transpose8x8(half2_bits(p[nt][0], p[nt][1]));
-        pb[nt][1] = transpose8x8(half2_bits(p[nt][2], p[nt][3]));
-      }
+      for (int j = 0; j < KP; ++j) {
+        uint32_t pb[NT][2];
 #pragma unroll
-      for (int st = 0; st < S::VS; ++st) {
-        uint32_t v[4][S::VW];
+        for (int nt = 0; nt < NT; ++nt) {
+          l[nt][0] += s[j][nt][1][0] + s[j][nt][1][2];
+          l[nt][1] += s[j][nt][1][1] + s[j][nt][1][3];
+          pb[nt][0] = transpose8x8(half2_bits(p[j][nt][0], p[j][nt][1]));
+          pb[nt][1] = transpose8x8(half2_bits(p[j][nt][2], p[j][nt][3]));
+        }
+        const uint8_t* page = unit + j * S::kPage + 16 * D;
 #pragma unroll
-        for (int h = 0; h < 4; ++h)
-          read_words<S::VW>(v[h], page + 16 * D + S::v_at(g, tq, h ^ (swap ? 1 : 0), st));
-        if (at_edge) {
-          // Rows past the last key may hold anything, NaN among it.
+        for (int st = 0; st < S::VS; ++st) {
+          uint32_t v[4][S::VW];
 #pragma unroll
           for (int h = 0; h < 4; ++h)
-            if (at.page * kKv8Page + S::value_key(tq, h ^ (swap ? 1 : 0)) >= at.x.len) {
+            read_words<S::VW>(v[h], page + S::v_at(g, tq, h ^ (swap ? 1 : 0), st));
+          if (at_edge) {
+            // Rows past the last key may hold anything, NaN among it.
 #pragma unroll
-              for (int w = 0; w < S::VW; ++w) v[h][w] = 0u;
+            for (int h = 0; h < 4; ++h)
+              if (key + j * kKv8Page + S::value_key(tq, h ^ (swap ? 1 : 0)) >= end[j]) {
+#pragma unroll
+                for (int w = 0; w < S::VW; ++w) v[h][w] = 0u;
+              }
+          }
+#pragma unroll
+          for (int w = 0; w < S::VW; ++w)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t sel = h ? pair_hi : pair_lo;
+              const uint32_t lo = __byte_perm(v[0][w], v[1][w], sel);
+              const uint32_t hi = __byte_perm(v[2][w], v[3][w], sel);
+              const uint32_t a0 = kv8_half2_lo(lo), a1 = kv8_half2_hi(lo);
+              const uint32_t a2 = kv8_half2_lo(hi), a3 = kv8_half2_hi(hi);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816(o[nt][(st * S::VW + w) * 2 + h], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
             }
         }
-#pragma unroll
-        for (int w = 0; w < S::VW; ++w)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t sel = h ? pair_hi : pair_lo;
-            const uint32_t lo = __byte_perm(v[0][w], v[1][w], sel);
-            const uint32_t hi = __byte_perm(v[2][w], v[3][w], sel);
-            const uint32_t a0 = kv8_half2_lo(lo), a1 = kv8_half2_hi(lo);
-            const uint32_t a2 = kv8_half2_lo(hi), a3 = kv8_half2_hi(hi);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma16816(o[nt][(st * S::VW + w) * 2 + h], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-          }
       }
     };
 
@@ -607,7 +598,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
             l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
     };
 
-    bool starts = at.page == 0;
+    bool starts = at.unit == 0;
     // The stream's sums so far: its output where this warp had it whole, else a piece.
     auto close = [&](bool ends) {
       sum_l();
@@ -645,19 +636,17 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     unsigned phases = 0;           // bit s: parity of stage s's next page
     int i = 0;
     for (; i < n; ++i) {
-      const bool ok = have >> stage & 1u;
-      if (ok) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phases >> stage & 1u, a.status))) break;
-        phases ^= 1u << stage;
-      }
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phases >> stage & 1u, a.status))) break;
+      phases ^= 1u << stage;
+      const unsigned there = have >> (stage * KP) & ((1u << KP) - 1u);
       if (i + ST - 1 < n) fetch(next);  // the stage that every lane has left behind
-      if (ok) multiply(ring + stage * S::kStage, ring + S::kScalesAt + stage * 32);
+      if (there) multiply(ring + stage * S::kStage, ring + S::kScalesAt + stage * (32 * KP), there);
       __syncwarp();
-      const bool ends = at.page == at.x.pages - 1;
+      const bool ends = at.unit == at.units - 1;
       if (ends || i + 1 == n) close(ends);
       if (i + 1 < n) {
         advance(at);
-        if (at.page == 0) {
+        if (at.unit == 0) {
           starts = true;
           open();
         }
@@ -668,7 +657,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     // After a wait that ran out: pages in flight land before the warp goes on (bounded too).
     for (int k = 0; i < n && k < ST - 1 && i + k < n; ++k) {
       const int f = (stage + k) % ST;
-      if (have >> f & 1u) mbar_wait(&full[f], phases >> f & 1u, a.status);
+      mbar_wait(&full[f], phases >> f & 1u, a.status);
     }
   }
   __syncthreads();
@@ -739,7 +728,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       // The stream that earlier CTAs began ends here: the join pass takes it.
       // It is the CTA's first chain, so its row is the CTA's first.
       const long long stream = static_cast<long long>(kvh) * x.chunks + p.z;
-      rec = Record{cut_owner(cut, units_before + stream * x.pages), kvh, x0, x.count, x.len, x.t0, {0, 0}};
+      rec = Record{cut_owner(cut, units_before + stream * stream_units<KP>(x)), kvh, x0, x.count, x.len, x.t0, {0, 0}};
     }
   }
   if (threadIdx.x == 0) records[blockIdx.x] = rec;
