@@ -175,15 +175,34 @@ __device__ __forceinline__ long long row_units(const Kv8Row& x, int hkv) {
   return static_cast<long long>(x.chunks) * hkv * stream_units<KP>(x);
 }
 
+// a / b for a >= 0, b > 0: a 64-bit division costs hundreds of cycles, and
+// nearly no batch needs one.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  if ((a | b) >> 32 == 0)
+    return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
+// The even cut of the units over CTAs: the first `more` take one unit more.
 struct Cut {
-  int ctas;         // CTAs with work
-  long long total;  // units
+  int ctas;               // CTAs with work
+  long long total, each;  // units, and of a CTA at least
+  int more;
 };
-__device__ __forceinline__ long long cut_begin(const Cut& c, long long i) {
-  return c.total * i / c.ctas;
+__device__ __forceinline__ Cut make_cut(long long total, int most, int least) {
+  Cut c;
+  c.total = total;
+  c.ctas = static_cast<int>(
+      min(static_cast<long long>(most), max(1LL, divide(total + least - 1, least))));
+  c.each = divide(total, c.ctas);
+  c.more = static_cast<int>(total - c.each * c.ctas);
+  return c;
+}
+__device__ __forceinline__ long long cut_begin(const Cut& c, int i) {
+  return c.each * i + min(i, c.more);
 }
 __device__ __forceinline__ int cut_owner(const Cut& c, long long unit) {
-  return static_cast<int>(((unit + 1) * c.ctas - 1) / c.total);
+  const long long big = (c.each + 1) * c.more;
+  return static_cast<int>(unit < big ? divide(unit, c.each + 1) : c.more + divide(unit - big, c.each));
 }
 
 // The workspace: per CTA a record and two pieces (the stream it continues, the
@@ -226,8 +245,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   // Pieces that warps leave: the row (-1: none), kv head, chunk, and whether the
-  // piece has the stream's first (1) and last (2) page.
-  __shared__ int4 left[kWarps * 2];
+  // piece has the stream's first (1) and last (2) page; and of the row its new
+  // tokens, keys, first token and units of a stream.
+  __shared__ int4 left[kWarps * 2], left_row[kWarps * 2];
   __shared__ int order[kWarps * 2 + 1], chains[kWarps * 2 + 1], chain_count;
   __shared__ long long units_before;  // units before the row of the CTA's first one
   // Launched behind the tile pass this one runs beside it: that pass lets its
@@ -240,34 +260,45 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
   const int g = lane >> 2, tq = lane & 3;
   const int hkv = a.cache.hkv;
 
-  // All units, and the row of this warp's first one.
-  Cut cut{};
-  long long mine[4];
-  for (int base = 0; base < a.rows; base += 128) {
+  if (lane == 0 && warp < 2) prefetch_tensormap(warp ? &maps.v : &maps.k);
+  // All units: their number up to each row of a group of 128 rows, one scan.
+  long long upto[4];
+  auto scan = [&](int base, bool report) {  // returns the group's units
+    long long sum = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int r = base + 32 * k + lane;
-      mine[k] = r < a.rows ? row_units<KP>(kv8_row(a, r, group, kCols, tile_from,
-                                                blockIdx.x == 0 && warp == 0), hkv)
-                           : 0;
+      upto[k] = r < a.rows ? row_units<KP>(kv8_row(a, r, group, kCols, tile_from, report), hkv) : 0;
     }
-    long long n = mine[0] + mine[1] + mine[2] + mine[3];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    cut.total += n;
-  }
+    for (int k = 0; k < 4; ++k) {
+      if (base + 32 * k < a.rows) {
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const long long v = __shfl_up_sync(0xffffffffu, upto[k], off);
+          if (lane >= off) upto[k] += v;
+        }
+        upto[k] += sum;
+        sum = __shfl_sync(0xffffffffu, upto[k], 31);
+      }
+    }
+    return sum;
+  };
+  long long total = 0;
+  for (int base = 0; base < a.rows; base += 128) total += scan(base, blockIdx.x == 0 && warp == 0);
   // A CTA takes kLeast units at least, where there are so many.
-  cut.ctas = static_cast<int>(
-      min(static_cast<long long>(gridDim.x), max(1LL, (cut.total + kLeast - 1) / kLeast)));
+  const Cut cut = make_cut(total, gridDim.x, kLeast);
   Record* records = reinterpret_cast<Record*>(a.workspace);
-  if (cut.total == 0 || static_cast<int>(blockIdx.x) >= cut.ctas) {
+  if (total == 0 || static_cast<int>(blockIdx.x) >= cut.ctas) {
     if (threadIdx.x == 0) records[blockIdx.x].first = -1;
     if (beside) griddep_wait();
     return;
   }
-  const long long c0 = cut_begin(cut, blockIdx.x), c1 = cut_begin(cut, blockIdx.x + 1);
-  const long long w0 = c0 + (c1 - c0) * warp / kWarps, w1 = c0 + (c1 - c0) * (warp + 1) / kWarps;
-  const int n = static_cast<int>(w1 - w0);
+  const long long c0 = cut_begin(cut, blockIdx.x);
+  const int units = static_cast<int>(cut_begin(cut, blockIdx.x + 1) - c0);
+  const int from = static_cast<int>(divide(static_cast<long long>(units) * warp, kWarps));
+  const int n = static_cast<int>(divide(static_cast<long long>(units) * (warp + 1), kWarps)) - from;
+  const long long w0 = c0 + from;
 
   float o[NT][D / 16][4];
   float m[NT][2], l[NT][2];
@@ -281,35 +312,27 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
   __syncwarp();
 
   if (n > 0) {
+    // The row of the warp's first unit.
     int row = -1;
     long long before = 0;  // units before the row
-    for (int base = 0; base < a.rows && row < 0; base += 128) {
-      if (a.rows > 128) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = base + 32 * k + lane;
-          mine[k] =
-              r < a.rows ? row_units<KP>(kv8_row(a, r, group, kCols, tile_from, false), hkv) : 0;
-        }
-      }
+    for (int base = 0; row < 0; base += 128) {
+      long long next = before;
+      if (a.rows > 128) next += scan(base, false);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (base + 32 * k >= a.rows || row >= 0) continue;
-        long long incl = mine[k];
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const long long v = __shfl_up_sync(0xffffffffu, incl, off);
-          if (lane >= off) incl += v;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, before + incl > w0);
+        if (row >= 0 || base + 32 * k >= a.rows) continue;
+        const unsigned hit = __ballot_sync(0xffffffffu, before + upto[k] > w0);
         if (hit) {
-          const int src = __ffs(hit) - 1;
-          row = base + 32 * k + src;
-          before += __shfl_sync(0xffffffffu, incl - mine[k], src);
-        } else {
-          before += __shfl_sync(0xffffffffu, incl, 31);
+          row = base + 32 * k + __ffs(hit) - 1;
+          if (row > base) {
+            // Units up to the row before it, which may be the last of the 32 before.
+            const int prev = row - base - 1;
+            const long long of = prev < 32 ? upto[0] : prev < 64 ? upto[1] : prev < 96 ? upto[2] : upto[3];
+            before += __shfl_sync(0xffffffffu, of, prev & 31);
+          }
         }
       }
+      if (row < 0) before = next;
     }
     if (w0 == c0 && lane == 0) units_before = before;
     const float sl2 = a.scale * kLog2e;
@@ -323,10 +346,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     at.x = kv8_row(a, row, group, kCols, tile_from, false);
     at.units = stream_units<KP>(at.x);
     {
-      at.unit = static_cast<int>((w0 - before) % at.units);
-      const int stream = static_cast<int>((w0 - before) / at.units);
-      at.kvh = stream / at.x.chunks;
-      at.chunk = stream % at.x.chunks;
+      const long long skip = w0 - before;
+      const int stream = static_cast<int>(divide(skip, at.units));
+      at.unit = static_cast<int>(skip - static_cast<long long>(stream) * at.units);
+      at.kvh = at.x.chunks == 1 ? stream : stream / at.x.chunks;
+      at.chunk = stream - at.kvh * at.x.chunks;
     }
     Cursor ahead = at;
     auto advance = [&](Cursor& c) {
@@ -625,7 +649,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
           *reinterpret_cast<float4*>(piece + S::kUnits * 4 + (nt * 8 + 2 * tq) * 2) =
               make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]);
       }
-      if (lane == 0) left[p] = make_int4(at.row, at.kvh, at.chunk, (starts ? 1 : 0) | (ends ? 2 : 0));
+      if (lane == 0) {
+        left[p] = make_int4(at.row, at.kvh, at.chunk, (starts ? 1 : 0) | (ends ? 2 : 0));
+        left_row[p] = make_int4(at.x.count, at.x.len, at.x.t0, at.units);
+      }
     };
 
 #pragma unroll
@@ -686,7 +713,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     const int k0 = chains[ch], k1 = chains[ch + 1];
     const int4 p = left[order[k0]];
     const bool begins = p.w & 1, ends = left[order[k1 - 1]].w & 2;
-    const Kv8Row x = kv8_row(a, p.x, group, kCols, tile_from, false);
+    const int4 of = left_row[order[k0]];
+    const Kv8Row x{of.x, of.y, of.z, 0, static_cast<int>((static_cast<long long>(of.x) * group + kCols - 1) / kCols)};
     const int kvh = p.y, x0 = p.z * kCols;
     float* dst = reinterpret_cast<float*>(records + gridDim.x) +
                  (static_cast<size_t>(blockIdx.x) * 2 + (begins ? 1 : 0)) * S::kPiece;
@@ -728,7 +756,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       // The stream that earlier CTAs began ends here: the join pass takes it.
       // It is the CTA's first chain, so its row is the CTA's first.
       const long long stream = static_cast<long long>(kvh) * x.chunks + p.z;
-      rec = Record{cut_owner(cut, units_before + stream * stream_units<KP>(x)), kvh, x0, x.count, x.len, x.t0, {0, 0}};
+      rec = Record{cut_owner(cut, units_before + stream * of.w), kvh, x0, x.count, x.len, x.t0, {0, 0}};
     }
   }
   if (threadIdx.x == 0) records[blockIdx.x] = rec;
@@ -745,7 +773,7 @@ struct Join {
   static constexpr int kThreads = kUnits * kShares;
 };
 template <int D, int NT>
-__global__ void __launch_bounds__(Join<D, NT>::kThreads) kv8_join_kernel(const Kv8AttnArgs a, int group) {
+__global__ void __launch_bounds__(Join<D, NT>::kThreads, 1) kv8_join_kernel(const Kv8AttnArgs a, int group) {
   using S = Shape<D, NT>;
   constexpr int kShares = Join<D, NT>::kShares;
   __shared__ float4 sums[kShares > 1 ? kShares - 1 : 1][S::kUnits];
@@ -763,28 +791,30 @@ __global__ void __launch_bounds__(Join<D, NT>::kThreads) kv8_join_kernel(const K
   auto piece = [&](int c) {
     return base + (static_cast<size_t>(c) * 2 + (c == first ? 1 : 0)) * S::kPiece;
   };
-  auto ml_of = [&](int c) {
-    return __ldcg(reinterpret_cast<const float4*>(piece(c) + S::kUnits * 4 + col * 2));
-  };
   float2 M = make_float2(kNoReference, kNoReference), L = make_float2(0.f, 0.f);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float4& ml, const float4& v) {
+    const float m0 = fmaxf(M.x, ml.x), m1 = fmaxf(M.y, ml.z);
+    const float f0 = ex2(M.x - m0), f1 = ex2(M.y - m1), g0 = ex2(ml.x - m0), g1 = ex2(ml.z - m1);
+    M = make_float2(m0, m1);
+    L = make_float2(L.x * f0 + ml.y * g0, L.y * f1 + ml.w * g1);
+    acc = make_float4(acc.x * f0 + v.x * g0, acc.y * f1 + v.y * g1, acc.z * f0 + v.z * g0,
+                      acc.w * f1 + v.w * g1);
+  };
   if (live) {
-#pragma unroll 8
-    for (int k = first + share; k <= end; k += kShares) {
-      const float4 ml = ml_of(k);
-      M = make_float2(fmaxf(M.x, ml.x), fmaxf(M.y, ml.z));
-    }
-#pragma unroll 8
-    for (int k = first + share; k <= end; k += kShares) {
-      const float4 ml = ml_of(k);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(piece(k) + u * 4));
-      const float f0 = ex2(ml.x - M.x), f1 = ex2(ml.z - M.y);
-      L.x += ml.y * f0;
-      L.y += ml.w * f1;
-      acc.x += v.x * f0;
-      acc.y += v.y * f1;
-      acc.z += v.z * f0;
-      acc.w += v.w * f1;
+    // Eight pieces at a time, all their loads in flight together.
+    for (int k = first + share; k <= end; k += 8 * kShares) {
+      float4 ml[8], v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i * kShares <= end) {
+          const float* p = piece(k + i * kShares);
+          ml[i] = __ldcg(reinterpret_cast<const float4*>(p + S::kUnits * 4 + col * 2));
+          v[i] = __ldcg(reinterpret_cast<const float4*>(p + u * 4));
+        }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i * kShares <= end) add(ml[i], v[i]);
     }
   }
   if (kShares > 1) {
@@ -796,15 +826,7 @@ __global__ void __launch_bounds__(Join<D, NT>::kThreads) kv8_join_kernel(const K
   }
   if (share > 0 || !live) return;
 #pragma unroll
-  for (int p = 0; p < kShares - 1; ++p) {
-    const float4 ml = refs[p][u], v = sums[p][u];
-    const float m0 = fmaxf(M.x, ml.x), m1 = fmaxf(M.y, ml.z);
-    const float f0 = ex2(M.x - m0), f1 = ex2(M.y - m1), g0 = ex2(ml.x - m0), g1 = ex2(ml.z - m1);
-    M = make_float2(m0, m1);
-    L = make_float2(L.x * f0 + ml.y * g0, L.y * f1 + ml.w * g1);
-    acc = make_float4(acc.x * f0 + v.x * g0, acc.y * f1 + v.y * g1, acc.z * f0 + v.z * g0,
-                      acc.w * f1 + v.w * g1);
-  }
+  for (int p = 0; p < kShares - 1; ++p) add(refs[p][u], sums[p][u]);
   const Kv8Row x{rec.count, rec.len, rec.t0, 0, 0};
   store_unit(a, x, group, rec.kvh, rec.x0 + col, S::dim_of((u >> 5) % (D / 16), (u >> 2) & 7), acc,
              1.f / L.x, 1.f / L.y);
