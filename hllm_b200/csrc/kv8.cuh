@@ -170,6 +170,8 @@ struct Kv8Row {
   int chunks;          // column groups per kv head
 };
 
+__device__ __forceinline__ int kv8_pages(int len) { return len > 0 ? (len - 1) / kKv8Page + 1 : 1; }
+
 // Row r as the stream pass (tiles false: rows under tile_from columns) or the
 // tile pass (the others) sees it: rows of the other pass, and rows out of the
 // batch's bounds (reported), have count 0.
@@ -185,7 +187,7 @@ __device__ __forceinline__ Kv8Row kv8_row(const Kv8AttnArgs& a, int r, int group
   if (bad && report) atomicOr(a.status, kDevBadIndex);
   x.count = bad || (count * group >= tile_from) != tiles ? 0 : static_cast<int>(count);
   if (bad) x.len = 0;
-  x.pages = max(1, (x.len + kKv8Page - 1) / kKv8Page);
+  x.pages = kv8_pages(x.len);
   x.chunks = static_cast<int>((static_cast<long long>(x.count) * group + cols - 1) / cols);
   return x;
 }

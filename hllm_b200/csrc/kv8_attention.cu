@@ -110,6 +110,9 @@ struct Layout {
   }
 };
 
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
 // Four bytes from global to shared memory, asynchronously (zeros where !live),
 // and the arrival on a barrier once a lane's copies have landed.
 __device__ __forceinline__ void copy4_async(uint32_t dst, const void* src, bool live) {
@@ -124,34 +127,31 @@ template <int D, int NT>
 struct Shape : Layout<D> {
   using Layout<D>::VW;
   static constexpr int kCols = 8 * NT;
-  // Enough warps to hide the latency of one page's chain of products, with the
-  // registers for the sums and the queries.
-  static constexpr int KP = D <= 128 && NT == 1 ? 2 : 1;  // pages of a unit: two chains of products in flight
-  static constexpr int kWarps = D * NT > 128 ? 8 : KP == 2 && D > 64 ? 10 : 12;
+  // Enough warps to hide the latency of one unit's chain of products, and
+  // enough bytes in flight to hide that of memory (132 KB an SM at D = 128).
+  static constexpr int KP = D <= 128 && NT == 1 ? 2 : 1;  // pages of a unit
+  static constexpr int kWarps = D * NT > 64 ? 8 : 12;
   static constexpr int kThreads = kWarps * 32;
   // A piece: D / 16 x NT fragments of 32 lanes x 4 sums, then cols x (m, l).
   static constexpr int kUnits = D / 16 * NT * 32;
   static constexpr int kPiece = kUnits * 4 + kCols * 2;  // floats
-  // A warp's shared memory: its ring of pages, whose place the piece it leaves
-  // open takes at the end; the piece it continues, which may be done earlier;
-  // the pages' scales and the ring's barriers.
+  // A warp's shared memory: its ring of units, whose place the piece that it
+  // ends with takes; their scales; the ring's barriers.  Behind the warps' lie
+  // kSlots places for pieces that are done earlier (one a stream that ends
+  // within a warp's share and began before it; any more go to the workspace).
   static constexpr int kPage = 32 * D;  // codes of K, then of V
   static constexpr int kStage = KP * kPage;
   static constexpr int kPieceBytes = kPiece * static_cast<int>(sizeof(float));
-  static constexpr int kRoom = 224 * 1024 / kWarps / 1024 * 1024;
+  static constexpr int kSlots = D * NT <= 128 ? 4 : 2;
+  static constexpr int kRoom = (225 * 1024 - kSlots * kPieceBytes) / kWarps / 1024 * 1024;
   __host__ __device__ static constexpr int bytes(int stages) {
-    return (stages * (kStage + 32 * KP + 8) + kPieceBytes + 1023) / 1024 * 1024;
+    return (stages * (kStage + 32 * KP + 8) + 1023) / 1024 * 1024;
   }
   static constexpr int kStages = bytes(4) <= kRoom ? 4 : bytes(3) <= kRoom ? 3 : 2;
   static constexpr int kWarpBytes = bytes(kStages);
-  static constexpr int kPieceAt = kStages * kStage, kScalesAt = kPieceAt + kPieceBytes;
-  static constexpr int kBarsAt = kScalesAt + kStages * 32 * KP;
-  static constexpr int kSmem = kWarps * kWarpBytes + 1024;  // 1024-byte alignment slack
-  static_assert(kPieceAt >= kPieceBytes && kWarpBytes <= kRoom, "shared memory of a warp");
-  static_assert(kScalesAt % 16 == 0 && kBarsAt % 8 == 0, "alignment");
-  __device__ static float* piece(uint8_t* smem, int p) {
-    return reinterpret_cast<float*>(smem + (p >> 1) * kWarpBytes + (p & 1 ? 0 : kPieceAt));
-  }
+  static constexpr int kScalesAt = kStages * kStage, kBarsAt = kScalesAt + kStages * 32 * KP;
+  static constexpr int kSmem = kWarps * kWarpBytes + kSlots * kPieceBytes + 1024;  // 1024: alignment
+  static_assert(kScalesAt >= kPieceBytes && kWarpBytes <= kRoom, "shared memory of a warp");
   // Value dimension of unit (i, lane): rows g and g + 8 of product i are
   // consecutive dimensions.
   __device__ static int dim_of(int i, int g) {
@@ -205,8 +205,8 @@ __device__ __forceinline__ int cut_owner(const Cut& c, long long unit) {
   return static_cast<int>(unit < big ? divide(unit, c.each + 1) : c.more + divide(unit - big, c.each));
 }
 
-// The workspace: per CTA a record and two pieces (the stream it continues, the
-// stream it leaves open).  The record is of a stream that earlier CTAs began
+// The workspace: per CTA a record, two pieces (the stream it continues, the
+// stream it leaves open), and a piece a warp.  The record is of a stream that earlier CTAs began
 // and this one ended: the CTA that began it (-1: there is none), and what its
 // output needs.
 struct Record {
@@ -248,6 +248,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
   // piece has the stream's first (1) and last (2) page; and of the row its new
   // tokens, keys, first token and units of a stream.
   __shared__ int4 left[kWarps * 2], left_row[kWarps * 2];
+  __shared__ float* where[kWarps * 2];
+  __shared__ int slots_taken;
   __shared__ int order[kWarps * 2 + 1], chains[kWarps * 2 + 1], chain_count;
   __shared__ long long units_before;  // units before the row of the CTA's first one
   // Launched behind the tile pass this one runs beside it: that pass lets its
@@ -261,14 +263,29 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
   const int hkv = a.cache.hkv;
 
   if (lane == 0 && warp < 2) prefetch_tensormap(warp ? &maps.v : &maps.k);
+  if (threadIdx.x == 0) slots_taken = 0;
+  // The block tables and the queries are needed only after the lengths: a line
+  // of each a thread comes to L2 meanwhile.
+  {
+    const long long i = static_cast<long long>(blockIdx.x) * S::kThreads + threadIdx.x;
+    if (i * 32 < static_cast<long long>(a.rows) * a.max_blocks) prefetch_l2(a.tables + i * 32);
+    const long long per = (static_cast<long long>(a.hq) * D + 63) / 64;
+    if (i < per * a.tokens) prefetch_l2(a.q + divide(i, per) * a.ld_q + (i - divide(i, per) * per) * 64);
+  }
   // All units: their number up to each row of a group of 128 rows, one scan.
   long long upto[4];
+  int4 rows[4];  // a lane's rows: new tokens, keys, first token, chunks
   auto scan = [&](int base, bool report) {  // returns the group's units
     long long sum = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int r = base + 32 * k + lane;
-      upto[k] = r < a.rows ? row_units<KP>(kv8_row(a, r, group, kCols, tile_from, report), hkv) : 0;
+      upto[k] = 0;
+      if (r < a.rows) {
+        const Kv8Row x = kv8_row(a, r, group, kCols, tile_from, report);
+        upto[k] = row_units<KP>(x, hkv);
+        rows[k] = make_int4(x.count, x.len, x.t0, x.chunks);
+      }
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -309,7 +326,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     for (int i = 0; i < ST; ++i) mbar_init(&full[i], 33);  // the boxes, and every lane's scales
     fence_mbar_init();
   }
-  __syncwarp();
+  __syncthreads();  // slots_taken
 
   if (n > 0) {
     // The row of the warp's first unit.
@@ -343,7 +360,15 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     };
     Cursor at;
     at.row = row;
-    at.x = kv8_row(a, row, group, kCols, tile_from, false);
+    {
+      const int k = row % 128 >> 5;
+      const int4 r = k == 0 ? rows[0] : k == 1 ? rows[1] : k == 2 ? rows[2] : rows[3];
+      at.x.count = __shfl_sync(0xffffffffu, r.x, row & 31);
+      at.x.len = __shfl_sync(0xffffffffu, r.y, row & 31);
+      at.x.t0 = __shfl_sync(0xffffffffu, r.z, row & 31);
+      at.x.chunks = __shfl_sync(0xffffffffu, r.w, row & 31);
+      at.x.pages = kv8_pages(at.x.len);
+    }
     at.units = stream_units<KP>(at.x);
     {
       const long long skip = w0 - before;
@@ -432,8 +457,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       for (int nt = 0; nt < NT; ++nt) {
         const int c = x0 + nt * 8 + g;
         const bool live = c < cols;
-        const __half* src = a.q + static_cast<size_t>(at.x.t0 + (live ? c / group : 0)) * a.ld_q +
-                            static_cast<size_t>(at.kvh * group + (live ? c % group : 0)) * D;
+        const int token = live && at.x.count > 1 ? c / group : 0;
+        const __half* src = a.q + static_cast<size_t>(at.x.t0 + token) * a.ld_q +
+                            static_cast<size_t>(at.kvh * group + (live ? c - token * group : 0)) * D;
 #pragma unroll
         for (int s = 0; s < S::KS; ++s)
 #pragma unroll
@@ -448,7 +474,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
         for (int e = 0; e < 2; ++e) {
           const int cc = x0 + nt * 8 + 2 * tq + e;
           // Columns beyond the stream's see everything; nothing of them is stored.
-          lim[nt][e] = cc < cols ? max(-1, at.x.len - at.x.count + cc / group) : 0x7fffffff;
+          const int tok = at.x.count > 1 ? cc / group : 0;
+          lim[nt][e] = cc < cols ? max(-1, at.x.len - at.x.count + tok) : 0x7fffffff;
           edge = min(edge, lim[nt][e]);
           m[nt][e] = kNoReference;
           l[nt][e] = 0.f;
@@ -624,7 +651,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
 
     bool starts = at.unit == 0;
     // The stream's sums so far: its output where this warp had it whole, else a piece.
-    auto close = [&](bool ends) {
+    auto close = [&](bool ends, bool last) {
       sum_l();
       if (starts && ends) {
 #pragma unroll
@@ -638,7 +665,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
         return;
       }
       const int p = warp * 2 + (starts ? 1 : 0);
-      float* piece = S::piece(smem, p);
+      float* piece = reinterpret_cast<float*>(ring);
+      if (!last) {
+        const int slot = __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(&slots_taken, 1) : 0, 0);
+        piece = slot < S::kSlots
+                    ? reinterpret_cast<float*>(smem + kWarps * S::kWarpBytes + slot * S::kPieceBytes)
+                    : reinterpret_cast<float*>(records + gridDim.x) +
+                          (static_cast<size_t>(gridDim.x) * 2 + blockIdx.x * kWarps + warp) * S::kPiece;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -652,6 +686,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       if (lane == 0) {
         left[p] = make_int4(at.row, at.kvh, at.chunk, (starts ? 1 : 0) | (ends ? 2 : 0));
         left_row[p] = make_int4(at.x.count, at.x.len, at.x.t0, at.units);
+        where[p] = piece;
       }
     };
 
@@ -670,7 +705,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       if (there) multiply(ring + stage * S::kStage, ring + S::kScalesAt + stage * (32 * KP), there);
       __syncwarp();
       const bool ends = at.unit == at.units - 1;
-      if (ends || i + 1 == n) close(ends);
+      if (ends || i + 1 == n) close(ends, i + 1 == n);
       if (i + 1 < n) {
         advance(at);
         if (at.unit == 0) {
@@ -722,7 +757,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       const int nt = u / (D / 16 * 32), col = nt * 8 + 2 * (u & 3);
       if (x0 + col >= x.count * group) continue;
       auto ml_of = [&](int k) {  // (m, l) of the unit's two columns
-        return *reinterpret_cast<const float4*>(S::piece(smem, order[k]) + S::kUnits * 4 + col * 2);
+        return *reinterpret_cast<const float4*>(where[order[k]] + S::kUnits * 4 + col * 2);
       };
       float2 M = make_float2(kNoReference, kNoReference), L = make_float2(0.f, 0.f);
 #pragma unroll 4
@@ -737,7 +772,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
         const float f0 = ex2(ml.x - M.x), f1 = ex2(ml.z - M.y);
         L.x += ml.y * f0;
         L.y += ml.w * f1;
-        const float4 v = *reinterpret_cast<const float4*>(S::piece(smem, order[k]) + u * 4);
+        const float4 v = *reinterpret_cast<const float4*>(where[order[k]] + u * 4);
         acc.x += v.x * f0;
         acc.y += v.y * f1;
         acc.z += v.z * f0;
@@ -896,9 +931,10 @@ bool with_tiles(int max_row_tokens, int hq, int hkv, int dim) {
   return kv8_tile_supported(dim) &&
          static_cast<long long>(max_row_tokens) * (hq / hkv) >= kTileFrom;
 }
+// Records, two pieces a CTA, and one a warp (at most 12).
 size_t stream_workspace(int dim, int sm_count) {
   return static_cast<size_t>(stream_ctas(sm_count)) *
-         (sizeof(Record) + 2 * piece_bytes(dim, dim <= 128 ? 2 : 1));
+         (sizeof(Record) + 14 * piece_bytes(dim, dim <= 128 ? 2 : 1));
 }
 
 }  // namespace
