@@ -215,24 +215,24 @@ struct Record {
   int pad[2];
 };
 
-// The output of one unit of a finished stream: sums of columns 2t, 2t + 1 and
-// of dimensions dim, dim + 1, times the columns' factors.
-__device__ __forceinline__ void store_unit(const Kv8AttnArgs& a, const Kv8Row& x, int group,
-                                           int kvh, int col, int dim, const float4& v, float f0,
-                                           float f1) {
-  const int cols = x.count * group;
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int c = col + e;
-    if (c < cols) {
-      const bool none = x.len - x.count + c / group < 0;  // no key: zeros
-      const float f = e ? f1 : f0;
-      const __half2 h = none ? __floats2half2_rn(0.f, 0.f)
-                             : __floats2half2_rn((e ? v.y : v.x) * f, (e ? v.w : v.z) * f);
-      *reinterpret_cast<__half2*>(a.out + static_cast<size_t>(x.t0 + c / group) * a.ld_out +
-                                  static_cast<size_t>(kvh * group + c % group) * a.cache.dim + dim) = h;
-    }
-  }
+// Where column `col` of a stream goes (null past the row's columns), and the
+// factor that makes its sums the output (0: it has no key, and its sums none).
+struct Output {
+  __half* to;
+  float factor;
+};
+__device__ __forceinline__ Output output_of(const Kv8AttnArgs& a, const Kv8Row& x, int group, int kvh,
+                                            int col, float l) {
+  if (col >= x.count * group) return Output{nullptr, 0.f};
+  const int token = x.count > 1 ? col / group : 0;
+  return Output{a.out + static_cast<size_t>(x.t0 + token) * a.ld_out +
+                    static_cast<size_t>(kvh * group + col - token * group) * a.cache.dim,
+                x.len - x.count + token < 0 ? 0.f : 1.f / l};
+}
+// One unit: sums of two columns at dimensions dim, dim + 1.
+__device__ __forceinline__ void store_unit(const Output& c0, const Output& c1, int dim, const float4& v) {
+  if (c0.to) *reinterpret_cast<__half2*>(c0.to + dim) = __floats2half2_rn(v.x * c0.factor, v.z * c0.factor);
+  if (c1.to) *reinterpret_cast<__half2*>(c1.to + dim) = __floats2half2_rn(v.y * c1.factor, v.w * c1.factor);
 }
 
 template <int D, int NT>
@@ -391,25 +391,66 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
         if (c.x.chunks) return;
       }
     };
-    int tab_row = -1, tab_q0 = 0, tab = -1;  // 32 entries of the block table, one a lane
-    unsigned have = 0;                       // bit stage * KP + j: page j of the stage is there
-    auto fetch = [&](int stage) {
-      const int q0 = ahead.unit * KP;
-      if (ahead.row != tab_row || q0 < tab_q0 || q0 + KP > tab_q0 + 32) {
-        tab_row = ahead.row;
-        tab_q0 = q0;
-        const int i = q0 + lane;
-        // Entries past the last key's page may hold anything.
-        tab = i < a.max_blocks && i * kKv8Page < ahead.x.len
-                  ? __ldg(a.tables + static_cast<size_t>(ahead.row) * a.max_blocks + i)
-                  : -2;
-        if (tab != -2 && (tab < 0 || tab >= a.cache.blocks)) tab = -1;
+    // The block table in pieces of 32 entries, one a lane.  With the memory busy
+    // a load takes microseconds, so the next piece, the row's first one (for its
+    // next stream) and the next row's first one are asked for well ahead.
+    auto table = [&](int r, int piece) {
+      const int i = piece * 32 + lane;
+      return r < a.rows && i < a.max_blocks ? __ldg(a.tables + static_cast<size_t>(r) * a.max_blocks + i) : -1;
+    };
+    int tab_row = at.row, tab_piece = at.unit * KP >> 5;
+    int tab = table(tab_row, tab_piece);
+    int tab_first = tab_piece ? table(tab_row, 0) : tab, tab_next = table(tab_row, tab_piece + 1);
+    int row_next = table(tab_row + 1, 0);
+    // The queries of the stream after the one at hand, asked for with its first pages.
+    uint32_t qn[NT][D / 16][2];
+    int entered = 0, opened = 0, qn_of = 0;  // streams that the loader, the arithmetic, qn are at
+    // The queries of a stream.
+    auto load_q = [&](const Cursor& c, uint32_t (&to)[NT][D / 16][2]) {
+      const int x0 = c.chunk * kCols, cols = c.x.count * group;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int col = x0 + nt * 8 + g;
+        const bool live = col < cols;
+        const int token = live && c.x.count > 1 ? col / group : 0;
+        const __half* src = a.q + static_cast<size_t>(c.x.t0 + token) * a.ld_q +
+                            static_cast<size_t>(c.kvh * group + (live ? col - token * group : 0)) * D;
+#pragma unroll
+        for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+          for (int w = 0; w < S::KW; ++w) {
+            const uint2 v =
+                live ? __ldg(reinterpret_cast<const uint2*>(src + ((s * 4 + tq) * S::KW + w) * 4))
+                     : make_uint2(0u, 0u);
+            to[nt][s * S::KW + w][0] = v.x;
+            to[nt][s * S::KW + w][1] = v.y;
+          }
       }
+    };
+    unsigned have = 0;  // bit stage * KP + j: page j of the stage is there
+    auto fetch = [&](int stage, bool first) {
+      const int q0 = ahead.unit * KP;
+      if (ahead.row != tab_row) {
+        tab_first = ahead.row == tab_row + 1 ? row_next : table(ahead.row, 0);
+        tab_row = ahead.row;
+        tab_piece = -1;
+        row_next = table(tab_row + 1, 0);
+      }
+      if (q0 >> 5 != tab_piece) {
+        tab = q0 < 32 ? tab_first : tab_next;
+        tab_piece = q0 >> 5;
+        if ((tab_piece + 1) * 32 < ahead.x.pages) tab_next = table(tab_row, tab_piece + 1);
+      }
+      // A page past the last key is none (-2), whatever its entry holds.
+      auto page_at = [&](int j) {
+        const int b = __shfl_sync(0xffffffffu, tab, (q0 & 31) + j);
+        return (q0 + j) * kKv8Page >= ahead.x.len ? -2 : b < 0 || b >= a.cache.blocks ? -1 : b;
+      };
       uint64_t* const bar = &full[stage];
       const uint32_t scales = smem_u32(ring + S::kScalesAt + stage * (32 * KP));
       // Scales: eight words a page, four of K and four of V.
       {
-        const int b = __shfl_sync(0xffffffffu, tab, q0 - tab_q0 + (lane >> 3 & (KP - 1)));
+        const int b = page_at(lane >> 3 & (KP - 1));
         if (lane < 8 * KP) {
           const size_t page = static_cast<size_t>(max(b, 0)) * hkv + ahead.kvh;
           copy4_async(scales + lane * 4,
@@ -421,7 +462,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       int b[KP], there = 0;
 #pragma unroll
       for (int j = 0; j < KP; ++j) {
-        b[j] = __shfl_sync(0xffffffffu, tab, q0 - tab_q0 + j);
+        b[j] = page_at(j);
         there |= b[j] >= 0 ? 1 << j : 0;
       }
       have = (have & ~(((1u << KP) - 1u) << (stage * KP))) | static_cast<unsigned>(there) << (stage * KP);
@@ -443,6 +484,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
           }
         }
       }
+      if (ahead.unit == 0 && !first) {
+        ++entered;
+        if (qn_of <= opened) {
+          qn_of = entered;
+          load_q(ahead, qn);
+        }
+      }
       advance(ahead);
     };
 
@@ -455,21 +503,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       edge = 0x7fffffff;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int c = x0 + nt * 8 + g;
-        const bool live = c < cols;
-        const int token = live && at.x.count > 1 ? c / group : 0;
-        const __half* src = a.q + static_cast<size_t>(at.x.t0 + token) * a.ld_q +
-                            static_cast<size_t>(at.kvh * group + (live ? c - token * group : 0)) * D;
-#pragma unroll
-        for (int s = 0; s < S::KS; ++s)
-#pragma unroll
-          for (int w = 0; w < S::KW; ++w) {
-            const uint2 v =
-                live ? __ldg(reinterpret_cast<const uint2*>(src + ((s * 4 + tq) * S::KW + w) * 4))
-                     : make_uint2(0u, 0u);
-            qb[nt][s * S::KW + w][0] = v.x;
-            qb[nt][s * S::KW + w][1] = v.y;
-          }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int cc = x0 + nt * 8 + 2 * tq + e;
@@ -656,11 +689,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       if (starts && ends) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float f0 = 1.f / l[nt][0], f1 = 1.f / l[nt][1];
+          const int col = at.chunk * kCols + nt * 8 + 2 * tq;
+          const Output c0 = output_of(a, at.x, group, at.kvh, col, l[nt][0]);
+          const Output c1 = output_of(a, at.x, group, at.kvh, col + 1, l[nt][1]);
 #pragma unroll
           for (int i = 0; i < D / 16; ++i)
-            store_unit(a, at.x, group, at.kvh, at.chunk * kCols + nt * 8 + 2 * tq, S::dim_of(i, g),
-                       make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]), f0, f1);
+            store_unit(c0, c1, S::dim_of(i, g),
+                       make_float4(o[nt][i][0], o[nt][i][1], o[nt][i][2], o[nt][i][3]));
         }
         return;
       }
@@ -692,7 +727,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
 
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i)
-      if (i < n) fetch(i);
+      if (i < n) fetch(i, i == 0);
+    load_q(at, qb);
     open();
     int stage = 0, next = ST - 1;  // of the page at hand, and of the one to fetch
     unsigned phases = 0;           // bit s: parity of stage s's next page
@@ -701,17 +737,28 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phases >> stage & 1u, a.status))) break;
       phases ^= 1u << stage;
       const unsigned there = have >> (stage * KP) & ((1u << KP) - 1u);
-      if (i + ST - 1 < n) fetch(next);  // the stage that every lane has left behind
+      if (i + ST - 1 < n) fetch(next, false);  // the stage that every lane has left behind
+      const bool ends = at.unit == at.units - 1, more = i + 1 < n;
       if (there) multiply(ring + stage * S::kStage, ring + S::kScalesAt + stage * (32 * KP), there);
       __syncwarp();
-      const bool ends = at.unit == at.units - 1;
-      if (ends || i + 1 == n) close(ends, i + 1 == n);
-      if (i + 1 < n) {
+      if (ends || !more) close(ends, !more);
+      if (ends && more) {
         advance(at);
-        if (at.unit == 0) {
-          starts = true;
-          open();
+        starts = true;
+        if (qn_of == ++opened) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              qb[nt][k][0] = qn[nt][k][0];
+              qb[nt][k][1] = qn[nt][k][1];
+            }
+        } else {
+          load_q(at, qb);
         }
+        open();
+      } else {
+        ++at.unit;
       }
       stage = stage + 1 == ST ? 0 : stage + 1;
       next = next + 1 == ST ? 0 : next + 1;
@@ -779,8 +826,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
         acc.w += v.w * f1;
       }
       if (begins && ends) {
-        store_unit(a, x, group, kvh, x0 + col, S::dim_of((u >> 5) % (D / 16), (u >> 2) & 7), acc,
-                   1.f / L.x, 1.f / L.y);
+        store_unit(output_of(a, x, group, kvh, x0 + col, L.x), output_of(a, x, group, kvh, x0 + col + 1, L.y),
+                   S::dim_of((u >> 5) % (D / 16), (u >> 2) & 7), acc);
       } else {
         *reinterpret_cast<float4*>(dst + u * 4) = acc;
         if (u % (D / 16 * 32) < 4)
@@ -863,8 +910,9 @@ __global__ void __launch_bounds__(Join<D, NT>::kThreads, 1) kv8_join_kernel(cons
 #pragma unroll
   for (int p = 0; p < kShares - 1; ++p) add(refs[p][u], sums[p][u]);
   const Kv8Row x{rec.count, rec.len, rec.t0, 0, 0};
-  store_unit(a, x, group, rec.kvh, rec.x0 + col, S::dim_of((u >> 5) % (D / 16), (u >> 2) & 7), acc,
-             1.f / L.x, 1.f / L.y);
+  store_unit(output_of(a, x, group, rec.kvh, rec.x0 + col, L.x),
+             output_of(a, x, group, rec.kvh, rec.x0 + col + 1, L.y),
+             S::dim_of((u >> 5) % (D / 16), (u >> 2) & 7), acc);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
