@@ -113,8 +113,14 @@ struct Layout {
 __device__ __forceinline__ void prefetch_l2(const void* p) {
   asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
-// Four bytes from global to shared memory, asynchronously (zeros where !live),
-// and the arrival on a barrier once a lane's copies have landed.
+// 4 or 16 bytes from global to shared memory, asynchronously (zeros where
+// !live); the arrival on a barrier once a lane's copies have landed; and the
+// wait for them.
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void copy4_async(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0)
                : "memory");
@@ -136,22 +142,26 @@ struct Shape : Layout<D> {
   static constexpr int kUnits = D / 16 * NT * 32;
   static constexpr int kPiece = kUnits * 4 + kCols * 2;  // floats
   // A warp's shared memory: its ring of units, whose place the piece that it
-  // ends with takes; their scales; the ring's barriers.  Behind the warps' lie
+  // ends with takes; their scales; the ring's barriers; the queries of a stream
+  // to come (each lane's own); three pieces of the block table.  Behind the warps' lie
   // kSlots places for pieces that are done earlier (one a stream that ends
   // within a warp's share and began before it; any more go to the workspace).
   static constexpr int kPage = 32 * D;  // codes of K, then of V
   static constexpr int kStage = KP * kPage;
   static constexpr int kPieceBytes = kPiece * static_cast<int>(sizeof(float));
-  static constexpr int kSlots = D * NT <= 128 ? 4 : 2;
+  static constexpr int kQueryBytes = kCols * D * 2;
+  static constexpr int kSlots = D * NT <= 64 ? 4 : 1;
   static constexpr int kRoom = (225 * 1024 - kSlots * kPieceBytes) / kWarps / 1024 * 1024;
   __host__ __device__ static constexpr int bytes(int stages) {
-    return (stages * (kStage + 32 * KP + 8) + 1023) / 1024 * 1024;
+    return (stages * (kStage + 32 * KP + 8) + 8 + kQueryBytes + 3 * 128 + 1023) / 1024 * 1024;
   }
   static constexpr int kStages = bytes(4) <= kRoom ? 4 : bytes(3) <= kRoom ? 3 : 2;
   static constexpr int kWarpBytes = bytes(kStages);
   static constexpr int kScalesAt = kStages * kStage, kBarsAt = kScalesAt + kStages * 32 * KP;
+  static constexpr int kQueriesAt = (kBarsAt + kStages * 8 + 15) / 16 * 16, kTableAt = kQueriesAt + kQueryBytes;
   static constexpr int kSmem = kWarps * kWarpBytes + kSlots * kPieceBytes + 1024;  // 1024: alignment
-  static_assert(kScalesAt >= kPieceBytes && kWarpBytes <= kRoom, "shared memory of a warp");
+  static_assert(kScalesAt >= kPieceBytes && kTableAt + 3 * 128 <= kWarpBytes && kWarpBytes <= kRoom,
+                "shared memory of a warp");
   // Value dimension of unit (i, lane): rows g and g + 8 of product i are
   // consecutive dimensions.
   __device__ static int dim_of(int i, int g) {
@@ -393,53 +403,86 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     };
     // The block table in pieces of 32 entries, one a lane.  With the memory busy
     // a load takes microseconds, so the next piece, the row's first one (for its
-    // next stream) and the next row's first one are asked for well ahead.
-    auto table = [&](int r, int piece) {
+    // next stream) and the next row's first one are on their way well ahead, to
+    // shared memory, where each lane reads its own entries.
+    int* const tables = reinterpret_cast<int*>(ring + S::kTableAt) + lane;  // + 32 k: first, next, next row's
+    auto table = [&](int k, int r, int piece) {
       const int i = piece * 32 + lane;
-      return r < a.rows && i < a.max_blocks ? __ldg(a.tables + static_cast<size_t>(r) * a.max_blocks + i) : -1;
+      if (r < a.rows && i < a.max_blocks)
+        copy4_async(smem_u32(tables + 32 * k), a.tables + static_cast<size_t>(r) * a.max_blocks + i, true);
     };
     int tab_row = at.row, tab_piece = at.unit * KP >> 5;
-    int tab = table(tab_row, tab_piece);
-    int tab_first = tab_piece ? table(tab_row, 0) : tab, tab_next = table(tab_row, tab_piece + 1);
-    int row_next = table(tab_row + 1, 0);
-    // The queries of the stream after the one at hand, asked for with its first pages.
-    uint32_t qn[NT][D / 16][2];
-    int entered = 0, opened = 0, qn_of = 0;  // streams that the loader, the arithmetic, qn are at
-    // The queries of a stream.
-    auto load_q = [&](const Cursor& c, uint32_t (&to)[NT][D / 16][2]) {
-      const int x0 = c.chunk * kCols, cols = c.x.count * group;
+    table(0, tab_row, 0);
+    table(1, tab_row, tab_piece + 1);
+    table(2, tab_row + 1, 0);
+    int tab = tab_piece * 32 + lane < a.max_blocks
+                  ? __ldg(a.tables + static_cast<size_t>(tab_row) * a.max_blocks + tab_piece * 32 + lane)
+                  : -1;
+    // The queries of a stream, in shared memory: each lane copies what it reads.
+    // They arrive with the stream's first unit, unless an earlier stream's are
+    // still there (streams of one unit), and then are loaded when it is their turn.
+    int entered = 0, opened = 0, queries_of = 0;  // streams that the loader, the arithmetic, the copy are at
+    constexpr int kHalves = S::KW / 2;            // 16-byte pieces of a lane's words
+    auto query_of = [&](const Cursor& c, int nt, bool* live) {
+      const int col = c.chunk * kCols + nt * 8 + g;
+      *live = col < c.x.count * group;
+      const int token = *live && c.x.count > 1 ? col / group : 0;
+      return a.q + static_cast<size_t>(c.x.t0 + token) * a.ld_q +
+             static_cast<size_t>(c.kvh * group + (*live ? col - token * group : 0)) * D + tq * S::KW * 4;
+    };
+    auto copy_queries = [&](const Cursor& c) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int col = x0 + nt * 8 + g;
-        const bool live = col < cols;
-        const int token = live && c.x.count > 1 ? col / group : 0;
-        const __half* src = a.q + static_cast<size_t>(c.x.t0 + token) * a.ld_q +
-                            static_cast<size_t>(c.kvh * group + (live ? col - token * group : 0)) * D;
+        bool live;
+        const __half* src = query_of(c, nt, &live);
 #pragma unroll
         for (int s = 0; s < S::KS; ++s)
 #pragma unroll
-          for (int w = 0; w < S::KW; ++w) {
-            const uint2 v =
-                live ? __ldg(reinterpret_cast<const uint2*>(src + ((s * 4 + tq) * S::KW + w) * 4))
-                     : make_uint2(0u, 0u);
-            to[nt][s * S::KW + w][0] = v.x;
-            to[nt][s * S::KW + w][1] = v.y;
+          for (int h = 0; h < kHalves; ++h)
+            copy16_async(smem_u32(ring + S::kQueriesAt + (((nt * S::KS + s) * kHalves + h) * 32 + lane) * 16),
+                         src + s * S::KW * 16 + h * 8, live);
+      }
+    };
+    uint32_t qb[NT][D / 16][2];  // the queries as B fragments, in the keys' order
+    auto take_queries = [&](bool copied) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        bool live;
+        const __half* src = query_of(at, nt, &live);
+#pragma unroll
+        for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (copied)
+              v = *reinterpret_cast<const uint4*>(ring + S::kQueriesAt +
+                                                  (((nt * S::KS + s) * kHalves + h) * 32 + lane) * 16);
+            else if (live)
+              v = __ldg(reinterpret_cast<const uint4*>(src + s * S::KW * 16 + h * 8));
+            qb[nt][s * S::KW + 2 * h][0] = v.x;
+            qb[nt][s * S::KW + 2 * h][1] = v.y;
+            qb[nt][s * S::KW + 2 * h + 1][0] = v.z;
+            qb[nt][s * S::KW + 2 * h + 1][1] = v.w;
           }
       }
     };
     unsigned have = 0;  // bit stage * KP + j: page j of the stage is there
     auto fetch = [&](int stage, bool first) {
       const int q0 = ahead.unit * KP;
-      if (ahead.row != tab_row) {
-        tab_first = ahead.row == tab_row + 1 ? row_next : table(ahead.row, 0);
-        tab_row = ahead.row;
-        tab_piece = -1;
-        row_next = table(tab_row + 1, 0);
-      }
-      if (q0 >> 5 != tab_piece) {
-        tab = q0 < 32 ? tab_first : tab_next;
+      if (ahead.row != tab_row || q0 >> 5 != tab_piece) {
+        copy_wait();
+        if (ahead.row != tab_row) {
+          if (ahead.row != tab_row + 1) {
+            table(2, ahead.row, 0);
+            copy_wait();
+          }
+          tab_row = ahead.row;
+          tables[0] = tables[64];
+          table(2, tab_row + 1, 0);
+        }
         tab_piece = q0 >> 5;
-        if ((tab_piece + 1) * 32 < ahead.x.pages) tab_next = table(tab_row, tab_piece + 1);
+        tab = tables[tab_piece ? 32 : 0];
+        if ((tab_piece + 1) * 32 < ahead.x.pages) table(1, tab_row, tab_piece + 1);
       }
       // A page past the last key is none (-2), whatever its entry holds.
       auto page_at = [&](int j) {
@@ -456,6 +499,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
           copy4_async(scales + lane * 4,
                       (lane & 4 ? a.cache.v_scale : a.cache.k_scale) + page * kKv8Page + (lane & 3) * 4,
                       b >= 0);
+        }
+        if (ahead.unit == 0 && !first) {
+          ++entered;
+          if (queries_of <= opened) {
+            queries_of = entered;
+            copy_queries(ahead);
+          }
         }
         copy_arrive(bar);
       }
@@ -484,17 +534,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
           }
         }
       }
-      if (ahead.unit == 0 && !first) {
-        ++entered;
-        if (qn_of <= opened) {
-          qn_of = entered;
-          load_q(ahead, qn);
-        }
-      }
       advance(ahead);
     };
 
-    uint32_t qb[NT][D / 16][2];  // the queries as B fragments, in the keys' order
     int lim[NT][2];              // last key that columns 2t, 2t + 1 see
     int edge;                    // least of them over the stream's columns
 
@@ -728,7 +770,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i)
       if (i < n) fetch(i, i == 0);
-    load_q(at, qb);
+    take_queries(false);
     open();
     int stage = 0, next = ST - 1;  // of the page at hand, and of the one to fetch
     unsigned phases = 0;           // bit s: parity of stage s's next page
@@ -745,17 +787,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       if (ends && more) {
         advance(at);
         starts = true;
-        if (qn_of == ++opened) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              qb[nt][k][0] = qn[nt][k][0];
-              qb[nt][k][1] = qn[nt][k][1];
-            }
-        } else {
-          load_q(at, qb);
-        }
+        take_queries(queries_of == ++opened);
         open();
       } else {
         ++at.unit;
@@ -763,6 +795,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       stage = stage + 1 == ST ? 0 : stage + 1;
       next = next + 1 == ST ? 0 : next + 1;
     }
+    copy_wait();
     // After a wait that ran out: pages in flight land before the warp goes on (bounded too).
     for (int k = 0; i < n && k < ST - 1 && i + k < n; ++k) {
       const int f = (stage + k) % ST;
