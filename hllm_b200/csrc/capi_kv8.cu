@@ -162,8 +162,8 @@ hllm_b200_status hllm_b200_kv8_write(const hllm_b200_kv8* cache, const void* qkv
   if (tokens == 0) return HLLM_B200_OK;
   if (!qkv || !positions || !slots || !q_out || (rotary_dim && !turns))
     return refuse("8-bit KV write: null argument");
-  if (!aligned16(qkv) || !aligned16(q_out))
-    return refuse("8-bit KV write: qkv and q_out must be 16-byte aligned");
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(q_norm) || !aligned16(k_norm))
+    return refuse("8-bit KV write: qkv, q_out and norm weights must be 16-byte aligned");
   hb::Kv8WriteArgs a{};
   a.cache = cache_of(cache);
   a.qkv = qkv;

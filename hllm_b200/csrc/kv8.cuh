@@ -153,12 +153,13 @@ __device__ __forceinline__ uint32_t kv8_half2_hi(uint32_t w) {
       : "r"(w));
   return h;
 }
-// Two values as codes (the first in the low byte), ties to even.
-__device__ __forceinline__ uint32_t kv8_codes(float lo, float hi) {
+// Four values as codes (the first in the low byte), ties to even.
+__device__ __forceinline__ uint32_t kv8_codes(float a, float b, float c, float d) {
   uint32_t w;
-  asm("{\n\t.reg .b16 c;\n\tcvt.rn.satfinite.e4m3x2.f32 c, %2, %1;\n\tcvt.u32.u16 %0, c;\n\t}"
+  asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\tmov.b32 %0, {lo, hi};\n\t}"
       : "=r"(w)
-      : "f"(lo), "f"(hi));
+      : "f"(a), "f"(b), "f"(c), "f"(d));
   return w;
 }
 

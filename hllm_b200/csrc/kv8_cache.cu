@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kv8.cuh"
@@ -10,25 +11,39 @@
 namespace hb {
 namespace {
 
+// Eight consecutive elements of a row as they lie in memory, and as F32.
 template <typename T>
-__device__ __forceinline__ float4 load4(const T* p);
+struct Eight {
+  uint4 w;
+  __device__ __forceinline__ void load(const T* p, bool live) {
+    w = live ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ static float2 pair(uint32_t v) {
+    if constexpr (std::is_same<T, __half>::value) {
+      return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    } else {
+      return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    }
+  }
+  __device__ __forceinline__ void values(float* y) const {
+    const float2 a = pair(w.x), b = pair(w.y), c = pair(w.z), d = pair(w.w);
+    y[0] = a.x, y[1] = a.y, y[2] = b.x, y[3] = b.y, y[4] = c.x, y[5] = c.y, y[6] = d.x, y[7] = d.y;
+  }
+};
 template <>
-__device__ __forceinline__ float4 load4<float>(const float* p) {
-  return *reinterpret_cast<const float4*>(p);
-}
-template <>
-__device__ __forceinline__ float4 load4<__half>(const __half* p) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-template <>
-__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
-  return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u),
-                     __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-}
+struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p, bool live) {
+    a = b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live) {
+      a = __ldg(reinterpret_cast<const float4*>(p));
+      b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    }
+  }
+  __device__ __forceinline__ void values(float* y) const {
+    y[0] = a.x, y[1] = a.y, y[2] = a.z, y[3] = a.w, y[4] = b.x, y[5] = b.y, y[6] = b.z, y[7] = b.w;
+  }
+};
 
 // ---------------------------------------------------------------- write
 // Per token t and head h of qkv: y = x * (1 / sqrt(mean x^2 + eps)) * w for q
@@ -39,299 +54,333 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
 // page slot / 16, row slot % 16.  Memory-bound: every element is read once and
 // written once.
 //
+// A warp takes one token and 32 / LANES of its heads at a time, the next
+// heads' loads in flight under this step's arithmetic.  A lane holds both
+// members of eight pairs: elements 8 j .. and rotary/2 + 8 j .. of a head (or
+// 16 j .. where pairs are neighbours, and past `rotary`), so pairs meet in
+// registers, and the lane keeps its pairs' cosines for all the token's heads.
+// Where rotary / 2 is not a multiple of 8 (kExchange) chunks of eight would
+// cross a border, and a lane takes 16 consecutive elements and fetches the
+// other members through shared memory.
+//
 // The angle is reduced to a fraction of a turn in 64 bits (position * turns
 // minus its nearest integer), so a position of 10^6 is as exact as 0; F32
-// angles would be off by 0.03 rad there.  The CTA's heads share one token's
-// cosines through shared memory: 64 pairs of 64-bit products a token, not a
-// head.
+// angles would be off by 0.03 rad there.  The fraction's own rounding to F32 is
+// kept and put back to first order: cos(a + r) = cos a - r sin a.
 constexpr int kWriteThreads = 256;
+constexpr int kWriteWarps = kWriteThreads / 32;
+// Warps that a call should have: below it a token's heads are spread over
+// several warps, each with the token's cosines to compute.
+constexpr int kWarpsWanted = 148 * 24;
+enum { kHalves, kNeighbours, kExchange };
 
-template <typename T, int LANES, int GROUPS>  // LANES threads a head, GROUPS x 4 elements each
-__global__ void __launch_bounds__(kWriteThreads) kv8_write_kernel(const Kv8WriteArgs a) {
-  constexpr int kUnits = kWriteThreads / LANES;
-  __shared__ float2 cs[kKv8MaxDim / 2];
-  __shared__ __align__(16) float buf[kUnits][4 * LANES * GROUPS];
+// y0, y1 of a pair turned by r = (cos, sin).
+__device__ __forceinline__ void turn(float& y0, float& y1, float2 r) {
+  const float a = y0, b = y1;
+  y0 = a * r.x - b * r.y;
+  y1 = b * r.x + a * r.y;
+}
+
+template <typename T, int LANES, int FORM>  // LANES threads a head, 16 elements each
+__global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 2 : 3)
+    kv8_write_kernel(const __grid_constant__ Kv8WriteArgs a, int slices) {
+  constexpr int kHeads = 32 / LANES;
+  __shared__ __align__(16) float2 turns_of[kWriteWarps][kKv8MaxDim / 2];
+  __shared__ float other_of[FORM == kExchange ? kWriteWarps : 1][FORM == kExchange ? kHeads : 1]
+                           [FORM == kExchange ? LANES * 16 + 1 : 1];
   griddep_enter();
-  const int t = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int unit = lane / LANES, j = lane % LANES;
+  const long long at_warp = static_cast<long long>(blockIdx.x) * kWriteWarps + warp;
+  const int t = static_cast<int>(at_warp / slices), slice = static_cast<int>(at_warp % slices);
+  if (t >= a.tokens) return;  // whole warps; nothing below spans warps
   const int d = a.cache.dim, hkv = a.cache.hkv, hq = a.hq;
-  const int heads = hq + 2 * hkv;
-  const int unit = threadIdx.x / LANES, lane = threadIdx.x % LANES;
-  const int step = gridDim.y * kUnits;
-  const int h0 = blockIdx.y * kUnits + unit;
+  const int heads = hq + 2 * hkv, half = a.rotary >> 1;
+  // Where the lane's two chunks of eight begin, and whether they turn.
+  const bool used = j * 16 < d;
+  const bool turns = FORM == kHalves ? j * 8 < half : j * 16 < a.rotary;
+  const int pairs_before = half >> 3;  // lanes that turn, in halves
+  const int i0 = FORM != kHalves ? j * 16 : turns ? j * 8 : a.rotary + (j - pairs_before) * 16;
+  const int i1 = FORM == kHalves && turns ? half + j * 8 : i0 + 8;
+
+  const int slot = __ldg(a.slots + t);
+  const int pos = __ldg(a.positions + t);
   const T* row = static_cast<const T*>(a.qkv) + static_cast<size_t>(t) * heads * d;
-  const int slot = a.slots[t];
-  const int pos = a.positions[t];
-  float4 x[GROUPS];
+  Eight<T> x0, x1;
   auto fetch = [&](int h) {
-#pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      const int i = (g * LANES + lane) * 4;
-      x[g] = h < heads && i < d ? load4<T>(row + static_cast<size_t>(h) * d + i)
-                                : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
+    const bool live = used && h < heads;
+    const T* p = row + static_cast<size_t>(live ? h : 0) * d;
+    x0.load(p + i0, live);
+    x1.load(p + i1, live);
   };
-  fetch(h0);
-  const int half = a.rotary >> 1;
-  for (int i = threadIdx.x; i < half; i += kWriteThreads) {
-    const double turns = static_cast<double>(pos) * a.turns[i];
+  int h = slice * kHeads + unit;
+  fetch(h);
+  float2* cs = turns_of[warp];
+  for (int i = lane; i < half; i += 32) {
+    const double all = static_cast<double>(pos) * a.turns[i];
+    const double part = 2.0 * (all - rint(all));  // half turns, -1 .. 1
+    const float f = static_cast<float>(part);
+    const float r = static_cast<float>(part - f) * 3.14159265f;
     float s, c;
-    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-    cs[i] = make_float2(c * a.factor, s * a.factor);
+    sincospif(f, &s, &c);
+    cs[i] = make_float2((c - r * s) * a.factor, (s + r * c) * a.factor);
   }
   const bool stored = slot >= 0 && slot < a.cache.blocks * kKv8Page;
-  if (threadIdx.x == 0 && slot >= 0 && !stored) atomicOr(a.status, kDevBadIndex);
-  __syncthreads();
+  if (slice == 0 && lane == 0 && slot >= 0 && !stored) atomicOr(a.status, kDevBadIndex);
+  __syncwarp();
+  float2 r[8];
+  if (FORM != kExchange) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      r[e] = used && turns ? cs[min(j * 8 + e, kKv8MaxDim / 2 - 1)] : make_float2(1.f, 0.f);
+  }
+  const size_t page = static_cast<size_t>(stored ? slot / kKv8Page : 0) * hkv;
+  const int in_page = slot % kKv8Page;
 
-  auto sum_lanes = [&](float v) {
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-  };
-  auto max_lanes = [&](float v) {
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-  };
-  for (int base = blockIdx.y * kUnits; base < heads; base += step) {  // uniform over the CTA
-    const int h = base + unit;
-    const bool live = h < heads;
+  for (int base = slice * kHeads; base < heads; base += slices * kHeads, h += slices * kHeads) {
+    const bool live = used && h < heads;
     const bool is_q = h < hq, is_v = h >= hq + hkv;
     const float* w = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;
-    float y[GROUPS][4];
+    float y[16];
+    x0.values(y);
+    x1.values(y + 8);
+    fetch(h + slices * kHeads);
+    // Shuffles take part in whole warps: a warp may hold heads of different kinds.
+    if (a.q_norm != nullptr || a.k_norm != nullptr) {
+      Eight<float> w0, w1;
+      w0.load(w + i0, w != nullptr && live);
+      w1.load(w + i1, w != nullptr && live);
+      float ss = 0.f;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      y[g][0] = x[g].x;
-      y[g][1] = x[g].y;
-      y[g][2] = x[g].z;
-      y[g][3] = x[g].w;
-    }
-    fetch(h + step);  // the next head's loads run under this head's arithmetic
-    // Shuffles take part in whole warps: a warp may hold two heads of different kinds.
-    float ss = 0.f;
+      for (int e = 0; e < 16; ++e) ss += y[e] * y[e];
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g)
-      ss += y[g][0] * y[g][0] + y[g][1] * y[g][1] + y[g][2] * y[g][2] + y[g][3] * y[g][3];
-    ss = sum_lanes(ss);
-    if (w && live) {
-      const float inv = 1.0f / sqrtf(ss / static_cast<float>(d) + a.eps);
+      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (w != nullptr) {
+        const float inv = 1.0f / sqrtf(ss / static_cast<float>(d) + a.eps);
+        float m[16];
+        w0.values(m);
+        w1.values(m + 8);
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        const int i = (g * LANES + lane) * 4;
-        if (i < d) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[g][e] = y[g][e] * inv * w[i + e];
-        }
+        for (int e = 0; e < 16; ++e) y[e] = y[e] * inv * m[e];
       }
     }
-    if (a.interleaved) {
-      if (!is_v) {
+    if constexpr (FORM == kHalves) {
+      if (turns && !is_v) {
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          const int i = (g * LANES + lane) * 4;
+        for (int e = 0; e < 8; ++e) turn(y[e], y[8 + e], r[e]);
+      }
+    } else if constexpr (FORM == kNeighbours) {
+      if (turns && !is_v) {
 #pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            if (i + e < a.rotary) {
-              const float2 r = cs[(i + e) >> 1];
-              const float y0 = y[g][e], y1 = y[g][e + 1];
-              y[g][e] = y0 * r.x - y1 * r.y;
-              y[g][e + 1] = y1 * r.x + y0 * r.y;
-            }
-          }
-        }
+        for (int e = 0; e < 8; ++e)
+          if (j * 8 + e < half) turn(y[2 * e], y[2 * e + 1], r[e]);
       }
     } else {
-      // The other half of a pair lies in another lane: through shared memory.
-      float* b = buf[unit];
+      float* b = other_of[warp][unit];
       __syncwarp();
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g)
-        *reinterpret_cast<float4*>(b + (g * LANES + lane) * 4) =
-            make_float4(y[g][0], y[g][1], y[g][2], y[g][3]);
+      for (int e = 0; e < 16; ++e) b[j * 16 + e] = y[e];
       __syncwarp();
       if (!is_v) {
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          const int i = (g * LANES + lane) * 4;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = i + e;
-            if (j < a.rotary) {
-              const bool lo = j < half;
-              const float2 r = cs[lo ? j : j - half];
-              const float other = b[lo ? j + half : j - half];
-              y[g][e] = lo ? y[g][e] * r.x - other * r.y : y[g][e] * r.x + other * r.y;
-            }
+        for (int e = 0; e < 16; ++e) {
+          const int i = j * 16 + e;
+          if (i < a.rotary) {
+            const bool lo = i < half;
+            const float2 q = cs[lo ? i : i - half];
+            const float other = b[lo ? i + half : i - half];
+            y[e] = lo ? y[e] * q.x - other * q.y : y[e] * q.x + other * q.y;
           }
         }
       }
     }
-    if (is_q) {
-      if (live) {
-        __half* dst = a.q_out + (static_cast<size_t>(t) * hq + h) * d;
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          const int i = (g * LANES + lane) * 4;
-          if (i < d) {
-            __half2 p[2] = {__floats2half2_rn(y[g][0], y[g][1]), __floats2half2_rn(y[g][2], y[g][3])};
-            *reinterpret_cast<uint2*>(dst + i) = *reinterpret_cast<uint2*>(p);
-          }
-        }
-      }
+    if (is_q && live) {
+      __half* dst = a.q_out + (static_cast<size_t>(t) * hq + h) * d;
+      *reinterpret_cast<uint4*>(dst + i0) = make_uint4(half2_bits(y[0], y[1]), half2_bits(y[2], y[3]),
+                                                       half2_bits(y[4], y[5]), half2_bits(y[6], y[7]));
+      *reinterpret_cast<uint4*>(dst + i1) =
+          make_uint4(half2_bits(y[8], y[9]), half2_bits(y[10], y[11]), half2_bits(y[12], y[13]),
+                     half2_bits(y[14], y[15]));
     }
+    if (base + kHeads <= hq) continue;  // q only: the same for the whole warp
     float top = 0.f;
+    bool plain = true;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g)
+    for (int e = 0; e < 16; ++e) {
+      const float m = fabsf(y[e]);
+      plain = plain && m <= kKv8Limit;
+      top = fmaxf(top, m);
+    }
+    if (!plain) {  // values that are not finite, or past the format
+      top = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float m = fabsf(y[g][e]);
+      for (int e = 0; e < 16; ++e) {
+        const float m = fabsf(y[e]);
         if (m <= kKv8Limit) top = fmaxf(top, m);
-        else y[g][e] = __uint_as_float(0x7fffffffu);  // not finite, or past the format
+        else y[e] = __uint_as_float(0x7fffffffu);
       }
-    top = max_lanes(top);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (!is_q && live && stored) {
       const int e = kv8_exponent(top);
       const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      const int kvh = is_v ? h - hq - hkv : h - hq;
-      const size_t at = (static_cast<size_t>(slot / kKv8Page) * hkv + kvh) * kKv8Page + slot % kKv8Page;
+      const size_t at = (page + (is_v ? h - hq - hkv : h - hq)) * kKv8Page + in_page;
       uint8_t* dst = (is_v ? a.cache.v : a.cache.k) + at * d;
+      uint32_t c[4];
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        const int i = (g * LANES + lane) * 4;
-        if (i < d)
-          *reinterpret_cast<uint32_t*>(dst + i) =
-              kv8_codes(y[g][0] * inv, y[g][1] * inv) | (kv8_codes(y[g][2] * inv, y[g][3] * inv) << 16);
-      }
-      if (lane == 0) (is_v ? a.cache.v_scale : a.cache.k_scale)[at] = static_cast<uint8_t>(e + 127);
+      for (int k = 0; k < 4; ++k)
+        c[k] = kv8_codes(y[4 * k] * inv, y[4 * k + 1] * inv, y[4 * k + 2] * inv, y[4 * k + 3] * inv);
+      *reinterpret_cast<uint2*>(dst + i0) = make_uint2(c[0], c[1]);
+      *reinterpret_cast<uint2*>(dst + i1) = make_uint2(c[2], c[3]);
+      if (j == 0) (is_v ? a.cache.v_scale : a.cache.k_scale)[at] = static_cast<uint8_t>(e + 127);
     }
   }
 }
 
-template <typename T, int LANES, int GROUPS>
+template <typename T, int LANES, int FORM>
 cudaError_t launch_write(const Kv8WriteArgs& a, cudaStream_t stream) {
-  constexpr int kUnits = kWriteThreads / LANES;
-  const int heads = a.hq + 2 * a.cache.hkv;
-  // Few tokens: a head a unit, so that the whole call is one round of loads.
-  // Many tokens: one CTA walks a token's heads and computes its angles once.
-  const int slices = (heads + kUnits - 1) / kUnits;
-  const int y = a.tokens >= 592 ? 1 : slices;
-  return launch_dependent(kv8_write_kernel<T, LANES, GROUPS>, dim3(a.tokens, y),
-                          dim3(kWriteThreads), 0, stream, a);
+  constexpr int kHeads = 32 / LANES;
+  const long long steps = (a.hq + 2LL * a.cache.hkv + kHeads - 1) / kHeads;
+  const int slices = static_cast<int>(
+      std::min(steps, std::max(1LL, static_cast<long long>(kWarpsWanted / a.tokens))));
+  const long long warps = static_cast<long long>(a.tokens) * slices;
+  return launch_dependent(kv8_write_kernel<T, LANES, FORM>,
+                          dim3(static_cast<unsigned>((warps + kWriteWarps - 1) / kWriteWarps)),
+                          dim3(kWriteThreads), 0, stream, a, slices);
+}
+
+template <typename T, int FORM>
+cudaError_t size_write(const Kv8WriteArgs& a, cudaStream_t stream) {
+  if (a.cache.dim <= 64) return launch_write<T, 4, FORM>(a, stream);
+  if (a.cache.dim <= 128) return launch_write<T, 8, FORM>(a, stream);
+  return launch_write<T, 16, FORM>(a, stream);
 }
 
 template <typename T>
 cudaError_t dispatch_write(const Kv8WriteArgs& a, cudaStream_t stream) {
-  if (a.cache.dim <= 64) return launch_write<T, 16, 1>(a, stream);
-  if (a.cache.dim <= 128) return launch_write<T, 32, 1>(a, stream);
-  return launch_write<T, 32, 2>(a, stream);
+  if (a.interleaved) return size_write<T, kNeighbours>(a, stream);
+  return a.rotary % 16 == 0 ? size_write<T, kHalves>(a, stream) : size_write<T, kExchange>(a, stream);
 }
 
 // ---------------------------------------------------------------- read
 // value = code * 2^e, rounded once to the output type.  Memory-bound.  A CTA
-// takes kReadTokens consecutive output rows: one warp finds their pages, then
-// every thread converts 16 codes at a time (one 16-byte load).
+// takes kReadTokens consecutive output rows: its threads find the rows' pages
+// together, then a warp takes K or V of a token at a time, each lane as many
+// codes as fill 16 bytes of output, kReadBatch loads in flight a lane.
 constexpr int kReadThreads = 256;
 constexpr int kReadTokens = 16;
+constexpr int kReadBatch = 4;
 
 template <typename T>
-__device__ __forceinline__ void store16(T* dst, const uint4& w, float s);
+struct Sixteen {  // 16 bytes of output
+  static constexpr int kCodes = 8;
+  using Codes = uint2;
+  __device__ __forceinline__ static uint32_t two(uint32_t h, float s) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    if constexpr (std::is_same<T, __half>::value) {
+      return half2_bits(v.x * s, v.y * s);
+    } else {
+      const __nv_bfloat162 p = __floats2bfloat162_rn(v.x * s, v.y * s);
+      return *reinterpret_cast<const uint32_t*>(&p);
+    }
+  }
+  __device__ __forceinline__ static uint4 of(uint2 w, float s) {
+    return make_uint4(two(kv8_half2_lo(w.x), s), two(kv8_half2_hi(w.x), s),
+                      two(kv8_half2_lo(w.y), s), two(kv8_half2_hi(w.y), s));
+  }
+};
 template <>
-__device__ __forceinline__ void store16<float>(float* dst, const uint4& w, float s) {
-  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = kv8_half2_lo(v[j]), hi = kv8_half2_hi(v[j]);
+struct Sixteen<float> {
+  static constexpr int kCodes = 4;
+  using Codes = uint32_t;
+  __device__ __forceinline__ static uint4 of(uint32_t w, float s) {
+    const uint32_t lo = kv8_half2_lo(w), hi = kv8_half2_hi(w);
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
     const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    reinterpret_cast<float4*>(dst)[j] = make_float4(a.x * s, a.y * s, b.x * s, b.y * s);
+    return make_uint4(__float_as_uint(a.x * s), __float_as_uint(a.y * s), __float_as_uint(b.x * s),
+                      __float_as_uint(b.y * s));
   }
-}
-template <>
-__device__ __forceinline__ void store16<__half>(__half* dst, const uint4& w, float s) {
-  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-  uint32_t o[8];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = kv8_half2_lo(v[j]), hi = kv8_half2_hi(v[j]);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    const __half2 p = __floats2half2_rn(a.x * s, a.y * s), q = __floats2half2_rn(b.x * s, b.y * s);
-    o[2 * j] = *reinterpret_cast<const uint32_t*>(&p);
-    o[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&q);
-  }
-  reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
-}
-template <>
-__device__ __forceinline__ void store16<__nv_bfloat16>(__nv_bfloat16* dst, const uint4& w, float s) {
-  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-  uint32_t o[8];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = kv8_half2_lo(v[j]), hi = kv8_half2_hi(v[j]);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    const __nv_bfloat162 p = __floats2bfloat162_rn(a.x * s, a.y * s);
-    const __nv_bfloat162 q = __floats2bfloat162_rn(b.x * s, b.y * s);
-    o[2 * j] = *reinterpret_cast<const uint32_t*>(&p);
-    o[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&q);
-  }
-  reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
-}
+};
 
 template <typename T>
-__global__ void __launch_bounds__(kReadThreads) kv8_read_kernel(const Kv8ReadArgs a) {
+__global__ void __launch_bounds__(kReadThreads)
+    kv8_read_kernel(const __grid_constant__ Kv8ReadArgs a, uint32_t inverse) {
+  using Out = Sixteen<T>;
+  using Codes = typename Out::Codes;
   __shared__ long long source[kReadTokens];  // row of (kv head 0) in the pool, -1: none, -2: no output
+  __shared__ int ends[kReadTokens];          // rows that end at a token of the CTA (the first: or before it)
   griddep_enter();
   const int t0 = blockIdx.x * kReadTokens;
   const int hkv = a.cache.hkv, d = a.cache.dim;
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    // Row of each token: the number of rows that end at or before it.
-    const int t = t0 + lane;
-    int r = 0;
-    for (int base = 0; base < a.rows; base += 32) {
-      const int end = base + lane < a.rows ? a.offsets[base + lane + 1] : 0x7fffffff;
-      const int n = min(32, a.rows - base);
-      for (int k = 0; k < n; ++k) r += __shfl_sync(0xffffffffu, end, k) <= t ? 1 : 0;
-    }
-    if (lane < kReadTokens) {
-      long long src = -2;
-      const int begin = a.offsets[0];
-      if (r < a.rows && t < a.tokens && t >= begin) {
-        const int first = a.first ? a.first[r] : 0;
-        const long long p = static_cast<long long>(first) + (t - a.offsets[r]);
-        src = -1;
-        if (p >= 0 && p < a.lengths[r] && p < static_cast<long long>(a.max_blocks) * kKv8Page) {
-          const int b = a.tables[static_cast<size_t>(r) * a.max_blocks + p / kKv8Page];
-          if (b >= 0 && b < a.cache.blocks)
-            src = static_cast<long long>(b) * hkv * kKv8Page + p % kKv8Page;
-        }
-        if (src < 0) atomicOr(a.status, kDevBadIndex);
-      }
-      source[lane] = src;
-    }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x < kReadTokens) ends[threadIdx.x] = 0;
+  __syncthreads();
+  for (int base = warp * 32; base < a.rows; base += kReadThreads) {
+    const int k = base + lane < a.rows ? max(__ldg(a.offsets + base + lane + 1), t0) - t0 : kReadTokens;
+    const unsigned before = __ballot_sync(0xffffffffu, k == 0);
+    if (lane == 0 && before) atomicAdd(&ends[0], __popc(before));
+    if (k > 0 && k < kReadTokens) atomicAdd(&ends[k], 1);
   }
   __syncthreads();
-  const int chunks = d >> 4;
-  const int per = hkv * chunks;
-  for (int i = threadIdx.x; i < 2 * kReadTokens * per; i += kReadThreads) {
-    const int which = i / (kReadTokens * per), rest = i % (kReadTokens * per);
-    const int tl = rest / per, u = rest % per;
-    const int kvh = u / chunks, c = u % chunks;
+  if (threadIdx.x < kReadTokens) {
+    const int t = t0 + lane;
+    int r = 0;  // row of the token: the number of rows that end at or before it
+    for (int k = 0; k <= lane; ++k) r += ends[k];
+    long long src = -2;
+    if (r < a.rows && t < a.tokens && t >= a.offsets[0]) {
+      const int first = a.first ? a.first[r] : 0;
+      const long long p = static_cast<long long>(first) + (t - a.offsets[r]);
+      src = -1;
+      if (p >= 0 && p < a.lengths[r] && p < static_cast<long long>(a.max_blocks) * kKv8Page) {
+        const int b = a.tables[static_cast<size_t>(r) * a.max_blocks + p / kKv8Page];
+        if (b >= 0 && b < a.cache.blocks)
+          src = static_cast<long long>(b) * hkv * kKv8Page + p % kKv8Page;
+      }
+      if (src < 0) atomicOr(a.status, kDevBadIndex);
+    }
+    source[lane] = src;
+  }
+  __syncthreads();
+  const uint32_t chunks = static_cast<uint32_t>(d) / Out::kCodes;
+  const uint32_t per = static_cast<uint32_t>(hkv) * chunks;
+  for (int item = warp; item < 2 * kReadTokens; item += kReadThreads / 32) {
+    const int tl = item >> 1, which = item & 1;
     const long long src = source[tl];
     if (src == -2) continue;
-    T* dst = static_cast<T*>(which ? a.v_out : a.k_out) +
-             (static_cast<size_t>(t0 + tl) * hkv + kvh) * d + c * 16;
-    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-    float s = 0.f;
-    if (src >= 0) {
-      const size_t at = static_cast<size_t>(src) + static_cast<size_t>(kvh) * kKv8Page;
-      w = __ldg(reinterpret_cast<const uint4*>((which ? a.cache.v : a.cache.k) + at * d + c * 16));
-      s = kv8_scale(__ldg((which ? a.cache.v_scale : a.cache.k_scale) + at));
+    const uint8_t* codes = which ? a.cache.v : a.cache.k;
+    const uint8_t* scales = which ? a.cache.v_scale : a.cache.k_scale;
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(which ? a.v_out : a.k_out) +
+                                          static_cast<size_t>(t0 + tl) * hkv * d);
+    for (uint32_t u0 = lane; u0 < per; u0 += 32 * kReadBatch) {
+      Codes w[kReadBatch];
+      uint32_t s[kReadBatch];
+#pragma unroll
+      for (int k = 0; k < kReadBatch; ++k) {
+        const uint32_t u = u0 + 32 * k;
+        w[k] = Codes{};
+        s[k] = 127u;
+        if (src >= 0 && u < per) {
+          const uint32_t kvh = __umulhi(u, inverse);  // u / chunks
+          const size_t at = static_cast<size_t>(src) + static_cast<size_t>(kvh) * kKv8Page;
+          w[k] = __ldg(reinterpret_cast<const Codes*>(codes + at * d) + (u - kvh * chunks));
+          s[k] = __ldg(scales + at);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kReadBatch; ++k)
+        if (u0 + 32 * k < per) dst[u0 + 32 * k] = Out::of(w[k], kv8_scale(s[k]));
     }
-    store16<T>(dst, w, s);
   }
+}
+
+template <typename T>
+cudaError_t launch_read(const Kv8ReadArgs& a, cudaStream_t stream) {
+  const dim3 grid((a.tokens + kReadTokens - 1) / kReadTokens);
+  // ceil(2^32 / chunks): u * inverse >> 32 is u / chunks for u * chunks < 2^32.
+  const uint32_t chunks = static_cast<uint32_t>(a.cache.dim) / Sixteen<T>::kCodes;
+  const uint32_t inverse = static_cast<uint32_t>((0x100000000ull + chunks - 1) / chunks);
+  return launch_dependent(kv8_read_kernel<T>, grid, dim3(kReadThreads), 0, stream, a, inverse);
 }
 
 }  // namespace
@@ -347,14 +396,10 @@ cudaError_t kv8_write_launch(const Kv8WriteArgs& a, cudaStream_t stream) {
 
 cudaError_t kv8_read_launch(const Kv8ReadArgs& a, cudaStream_t stream) {
   if (a.tokens == 0 || a.rows == 0) return cudaSuccess;
-  const dim3 grid((a.tokens + kReadTokens - 1) / kReadTokens);
   switch (a.type) {
-    case kKv8F32:
-      return launch_dependent(kv8_read_kernel<float>, grid, dim3(kReadThreads), 0, stream, a);
-    case kKv8F16:
-      return launch_dependent(kv8_read_kernel<__half>, grid, dim3(kReadThreads), 0, stream, a);
-    default:
-      return launch_dependent(kv8_read_kernel<__nv_bfloat16>, grid, dim3(kReadThreads), 0, stream, a);
+    case kKv8F32: return launch_read<float>(a, stream);
+    case kKv8F16: return launch_read<__half>(a, stream);
+    default: return launch_read<__nv_bfloat16>(a, stream);
   }
 }
 

@@ -39,7 +39,7 @@ def _refuse(message: str):
     raise StageError(_lib.INVALID_REQUEST, message)
 
 
-def _need(tensor, name: str, dtype, device, shape=None, optional=False):
+def _need(tensor, name: str, dtype, index: int, shape=None, optional=False):
     """Checks one tensor and returns its address (None for a missing optional one)."""
     if tensor is None and optional:
         return None
@@ -47,24 +47,37 @@ def _need(tensor, name: str, dtype, device, shape=None, optional=False):
         _refuse(f"{name} must be a tensor")
     if tensor.dtype != dtype:
         _refuse(f"{name} must be {dtype}, not {tensor.dtype}")
-    if tensor.device != device:
-        _refuse(f"{name} is on {tensor.device}, the cache on {device}")
-    if shape is not None and tuple(tensor.shape) != tuple(shape):
+    if tensor.get_device() != index:
+        _refuse(f"{name} is on {tensor.device}, the cache on cuda:{index}")
+    if shape is not None and tensor.shape != shape:
         _refuse(f"{name} must have shape {tuple(shape)}, not {tuple(tensor.shape)}")
     if not tensor.is_contiguous():
         _refuse(f"{name} must be contiguous")
     return tensor.data_ptr()
 
 
-def _call(function, device, *args) -> None:
-    """One library call with `device` current, on its current stream (the last argument)."""
-    if torch.cuda.current_device() == device.index:
-        status = function(*args, torch.cuda.current_stream().cuda_stream)
+# The device and stream that torch has current, without the objects around them
+# (3 us less host time a call).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                          lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(name: str, index: int, *args) -> None:
+    """One library call with device `index` current, on its current stream (the last argument)."""
+    function = _functions.get(name)
+    if function is None:
+        function = _functions[name] = getattr(lib(), name)
+    if _current_device() == index:
+        status = function(*args, _current_stream(index))
     else:
-        with torch.cuda.device(device):
-            status = function(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            status = function(*args, _current_stream(index))
     if status:
         _lib.check(status)
+
+
+_functions: dict = {}
 
 
 class Cache:
@@ -101,12 +114,12 @@ class Cache:
                 (v_scale, "v_scale", (torch.uint8, torch.float8_e8m0fnu), k.shape[:3])):
             if t.dtype not in kinds:
                 _refuse(f"{name} must be one of {kinds}, not {t.dtype}")
-            _need(t, name, t.dtype, k.device, shape)
+            _need(t, name, t.dtype, k.get_device(), shape)
         self.k, self.v = k.view(torch.float8_e4m3fn), v.view(torch.float8_e4m3fn)
         self.k_scale = k_scale.view(torch.float8_e8m0fnu)
         self.v_scale = v_scale.view(torch.float8_e8m0fnu)
         self.blocks, self.kv_heads, _, self.head_dim = k.shape
-        self.device = k.device
+        self.device, self._index = k.device, k.get_device()
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         self._status = self.status.data_ptr()
         self._c = _lib.KV8(k.data_ptr(), k_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr(),
@@ -163,7 +176,7 @@ def write(cache: Cache, qkv, positions, slots, rope: Rope, q_norm=None, k_norm=N
     (float32, float16 or bfloat16), int32 positions and slots [tokens] (slot
     -1: not stored; the slots of a call are distinct).  Returns q, float16
     [tokens, heads * head_dim]."""
-    device, d = cache.device, cache.head_dim
+    index, d = cache._index, cache.head_dim
     if not isinstance(qkv, torch.Tensor) or qkv.dtype not in _TYPES or qkv.dim() != 2:
         _refuse("qkv must be a float32, float16 or bfloat16 matrix")
     tokens, width = qkv.shape
@@ -172,16 +185,16 @@ def write(cache: Cache, qkv, positions, slots, rope: Rope, q_norm=None, k_norm=N
         _refuse(f"qkv rows of {width} are not (heads + 2 x {cache.kv_heads}) x {d}")
     if rope.rotary_dim > d:
         _refuse(f"rope turns {rope.rotary_dim} of a head of {d}")
-    x = _need(qkv, "qkv", qkv.dtype, device)
-    p = _need(positions, "positions", torch.int32, device, (tokens,))
-    s = _need(slots, "slots", torch.int32, device, (tokens,))
-    qn = _need(q_norm, "q_norm", torch.float32, device, (d,), optional=True)
-    kn = _need(k_norm, "k_norm", torch.float32, device, (d,), optional=True)
-    turns = _need(rope.turns, "rope.turns", torch.float64, device)
+    x = _need(qkv, "qkv", qkv.dtype, index)
+    p = _need(positions, "positions", torch.int32, index, (tokens,))
+    s = _need(slots, "slots", torch.int32, index, (tokens,))
+    qn = _need(q_norm, "q_norm", torch.float32, index, (d,), optional=True)
+    kn = _need(k_norm, "k_norm", torch.float32, index, (d,), optional=True)
+    turns = _need(rope.turns, "rope.turns", torch.float64, index)
     if out is None:
-        out = torch.empty((tokens, hq * d), dtype=torch.float16, device=device)
-    o = _need(out, "out", torch.float16, device, (tokens, hq * d))
-    _call(lib().hllm_b200_kv8_write, device, cache._ref, x, _TYPES[qkv.dtype], tokens, hq, p, s, qn,
+        out = torch.empty((tokens, hq * d), dtype=torch.float16, device=cache.device)
+    o = _need(out, "out", torch.float16, index, (tokens, hq * d))
+    _call("hllm_b200_kv8_write", index, cache._ref, x, _TYPES[qkv.dtype], tokens, hq, p, s, qn,
           kn, eps, turns, rope.rotary_dim, rope.interleaved, rope.factor, o, cache._status)
     return out
 
@@ -192,22 +205,22 @@ def read(cache: Cache, block_tables, lengths, offsets, tokens: int, first=None,
     lengths[r]) go to rows [offsets[r], offsets[r + 1]) of k and v [tokens,
     kv_heads, head_dim] (int32 tensors; first None: 0).  Returns (k, v); `out`
     is such a pair to fill, whose rows from offsets[-1] on are left alone."""
-    device = cache.device
+    index = cache._index
     if dtype not in _TYPES:
         _refuse("dtype must be float32, float16 or bfloat16")
     if not isinstance(block_tables, torch.Tensor) or block_tables.dim() != 2:
         _refuse("block_tables must be [rows, most pages]")
     rows, width = block_tables.shape
-    t = _need(block_tables, "block_tables", torch.int32, device)
-    n = _need(lengths, "lengths", torch.int32, device, (rows,))
-    f = _need(first, "first", torch.int32, device, (rows,), optional=True)
-    c = _need(offsets, "offsets", torch.int32, device, (rows + 1,))
+    t = _need(block_tables, "block_tables", torch.int32, index)
+    n = _need(lengths, "lengths", torch.int32, index, (rows,))
+    f = _need(first, "first", torch.int32, index, (rows,), optional=True)
+    c = _need(offsets, "offsets", torch.int32, index, (rows + 1,))
     shape = (tokens, cache.kv_heads, cache.head_dim)
     if out is None:
-        out = (torch.empty(shape, dtype=dtype, device=device),
-               torch.empty(shape, dtype=dtype, device=device))
-    k, v = (_need(x, name, dtype, device, shape) for x, name in zip(out, ("k", "v")))
-    _call(lib().hllm_b200_kv8_read, device, cache._ref, t, rows, width, f, n, c, tokens,
+        out = (torch.empty(shape, dtype=dtype, device=cache.device),
+               torch.empty(shape, dtype=dtype, device=cache.device))
+    k, v = (_need(x, name, dtype, index, shape) for x, name in zip(out, ("k", "v")))
+    _call("hllm_b200_kv8_read", index, cache._ref, t, rows, width, f, n, c, tokens,
           _TYPES[dtype], k, v, cache._status)
     return out
 
@@ -230,37 +243,42 @@ def attention(cache: Cache, q, cu_seqlens, lengths, block_tables, max_tokens: Op
     lengths[r] keys; int32 block_tables [rows, most pages].  ``max_tokens`` is
     the most new tokens of a row (default: tokens; 1 for a decode batch),
     ``scale`` defaults to 1/sqrt(head_dim).  Returns float16 like q."""
-    device, d = cache.device, cache.head_dim
+    index, d = cache._index, cache.head_dim
     if not isinstance(q, torch.Tensor) or q.dim() != 2 or q.dtype != torch.float16:
         _refuse("q must be a float16 matrix")
     tokens, width = q.shape
     hq = width // d
     if width % d or hq == 0 or hq % cache.kv_heads:
         _refuse(f"q rows of {width} are not heads x {d}, a multiple of {cache.kv_heads} heads")
-    if q.device != device:
-        _refuse(f"q is on {q.device}, the cache on {device}")
+    if q.get_device() != index:
+        _refuse(f"q is on {q.device}, the cache on {cache.device}")
     if out is None:
-        out = torch.empty((tokens, width), dtype=torch.float16, device=device)
-    elif (not isinstance(out, torch.Tensor) or out.dtype != torch.float16 or out.device != device
-          or tuple(out.shape) != (tokens, width)):
-        _refuse(f"out must be a float16 {(tokens, width)} matrix on {device}")
-    for name, x in (("q", q), ("out", out)):
-        if tokens > 0 and (x.stride(1) != 1 or x.stride(0) < width):
-            _refuse(f"{name} must have contiguous rows")
+        out = torch.empty((tokens, width), dtype=torch.float16, device=cache.device)
+    elif (not isinstance(out, torch.Tensor) or out.dtype != torch.float16
+          or out.get_device() != index or out.shape != (tokens, width)):
+        _refuse(f"out must be a float16 {(tokens, width)} matrix on {cache.device}")
+    ld_q = ld_out = width
+    if tokens > 0:
+        (ld_q, across), (ld_out, out_across) = q.stride(), out.stride()
+        if across != 1 or ld_q < width:
+            _refuse("q must have contiguous rows")
+        if out_across != 1 or ld_out < width:
+            _refuse("out must have contiguous rows")
     if not isinstance(block_tables, torch.Tensor) or block_tables.dim() != 2:
         _refuse("block_tables must be [rows, most pages]")
     rows, blocks = block_tables.shape
-    t = _need(block_tables, "block_tables", torch.int32, device)
-    n = _need(lengths, "lengths", torch.int32, device, (rows,))
-    c = _need(cu_seqlens, "cu_seqlens", torch.int32, device, (rows + 1,))
+    t = _need(block_tables, "block_tables", torch.int32, index)
+    n = _need(lengths, "lengths", torch.int32, index, (rows,))
+    c = _need(cu_seqlens, "cu_seqlens", torch.int32, index, (rows + 1,))
     most = tokens if max_tokens is None else int(max_tokens)
     if most < 0:
         _refuse("max_tokens must not be negative")
     if workspace is None:
-        workspace = attention_workspace(rows, tokens, most, hq, cache.kv_heads, d, device)
-    w = _need(workspace, "workspace", torch.uint8, device)
-    _call(lib().hllm_b200_kv8_attention, device, cache._ref, q.data_ptr(),
-          q.stride(0) if tokens else width, c, n, t, rows, tokens, most, hq, blocks,
+        workspace = attention_workspace(rows, tokens, most, hq, cache.kv_heads, d,
+                                        cache.device)
+    w = _need(workspace, "workspace", torch.uint8, index)
+    _call("hllm_b200_kv8_attention", index, cache._ref, q.data_ptr(),
+          ld_q, c, n, t, rows, tokens, most, hq, blocks,
           1.0 / math.sqrt(d) if scale is None else scale, out.data_ptr(),
-          out.stride(0) if tokens else width, w, workspace.numel(), cache._status)
+          ld_out, w, workspace.numel(), cache._status)
     return out

@@ -500,7 +500,8 @@ hllm_b200_status hllm_b200_rope_turns(const hllm_b200_rope* rope, double* turns,
  * hllm_b200_rope_turns, turns on the device), q to q_out F16 [tokens][Hq d],
  * K and V quantised into slots[t].  A token with slot -1 is not stored.  The
  * slots of a call are distinct, as the packer's are; of tokens that share one,
- * each stored byte is from one of them.  qkv and q_out are 16-byte aligned. */
+ * each stored byte is from one of them.  qkv, q_out and the norm weights are
+ * 16-byte aligned. */
 hllm_b200_status hllm_b200_kv8_write(const hllm_b200_kv8* cache, const void* qkv,
                                      hllm_b200_dtype dtype, uint64_t tokens, uint32_t hq,
                                      const int32_t* positions, const int32_t* slots,
