@@ -56,8 +56,8 @@ struct Eight<float> {
 //
 // A warp takes one token and 32 / LANES of its heads at a time, the next
 // heads' loads in flight under this step's arithmetic.  A lane holds both
-// members of eight pairs: elements 8 j .. and rotary/2 + 8 j .. of a head (or
-// 16 j .. where pairs are neighbours, and past `rotary`), so pairs meet in
+// members of eight pairs: elements 8 j .. and rotary/2 + 8 j .. of a head (past
+// `rotary`, and where pairs are neighbours: of halves of that), so pairs meet in
 // registers, and the lane keeps its pairs' cosines for all the token's heads.
 // Where rotary / 2 is not a multiple of 8 (kExchange) chunks of eight would
 // cross a border, and a lane takes 16 consecutive elements and fetches the
@@ -67,11 +67,14 @@ struct Eight<float> {
 // minus its nearest integer), so a position of 10^6 is as exact as 0; F32
 // angles would be off by 0.03 rad there.  The fraction's own rounding to F32 is
 // kept and put back to first order: cos(a + r) = cos a - r sin a.
-constexpr int kWriteThreads = 256;
+constexpr int kWriteThreads = 128;
 constexpr int kWriteWarps = kWriteThreads / 32;
-// Warps that a call should have: below it a token's heads are spread over
-// several warps, each with the token's cosines to compute.
-constexpr int kWarpsWanted = 148 * 24;
+// Warps that a call should have (three rounds of full SMs): below it a token's
+// heads are spread over several warps, each with the token's cosines to
+// compute.  8192 tokens of 32 + 8 + 8 heads of 128: 45 us so, 48 at one round;
+// 128 threads a CTA and 80 registers (24 warps an SM) 45 us, 96 registers 46,
+// the loads of two steps ahead at 116 registers 51.
+constexpr int kWarpsWanted = 148 * 24 * 3;
 enum { kHalves, kNeighbours, kExchange };
 
 // y0, y1 of a pair turned by r = (cos, sin).
@@ -82,7 +85,7 @@ __device__ __forceinline__ void turn(float& y0, float& y1, float2 r) {
 }
 
 template <typename T, int LANES, int FORM>  // LANES threads a head, 16 elements each
-__global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 2 : 3)
+__global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 4 : 6)
     kv8_write_kernel(const __grid_constant__ Kv8WriteArgs a, int slices) {
   constexpr int kHeads = 32 / LANES;
   __shared__ __align__(16) float2 turns_of[kWriteWarps][kKv8MaxDim / 2];
@@ -96,12 +99,17 @@ __global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 2 : 3)
   if (t >= a.tokens) return;  // whole warps; nothing below spans warps
   const int d = a.cache.dim, hkv = a.cache.hkv, hq = a.hq;
   const int heads = hq + 2 * hkv, half = a.rotary >> 1;
-  // Where the lane's two chunks of eight begin, and whether they turn.
+  // Where the lane's two chunks of eight begin: lanes side by side read and
+  // write 16 bytes side by side (a 32-byte stride doubled the load wavefronts).
   const bool used = j * 16 < d;
-  const bool turns = FORM == kHalves ? j * 8 < half : j * 16 < a.rotary;
-  const int pairs_before = half >> 3;  // lanes that turn, in halves
-  const int i0 = FORM != kHalves ? j * 16 : turns ? j * 8 : a.rotary + (j - pairs_before) * 16;
-  const int i1 = FORM == kHalves && turns ? half + j * 8 : i0 + 8;
+  const bool turns = j * 8 < half;  // in halves: whether the lane's chunks turn
+  const int i0 = FORM == kExchange ? j * 16
+                 : FORM == kNeighbours || turns ? j * 8
+                                                : a.rotary + j * 8 - half;
+  const int i1 = FORM == kExchange      ? i0 + 8
+                 : FORM == kNeighbours ? (d >> 1) + j * 8
+                 : turns                ? half + j * 8
+                                        : i0 + ((d - a.rotary) >> 1);
 
   const int slot = __ldg(a.slots + t);
   const int pos = __ldg(a.positions + t);
@@ -131,8 +139,10 @@ __global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 2 : 3)
   float2 r[8];
   if (FORM != kExchange) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      r[e] = used && turns ? cs[min(j * 8 + e, kKv8MaxDim / 2 - 1)] : make_float2(1.f, 0.f);
+    for (int e = 0; e < 8; ++e) {
+      const int pair = FORM == kHalves ? j * 8 + e : ((e < 4 ? i0 : i1) >> 1) + (e & 3);
+      r[e] = used && pair < half ? cs[pair] : make_float2(1.f, 0.f);
+    }
   }
   const size_t page = static_cast<size_t>(stored ? slot / kKv8Page : 0) * hkv;
   const int in_page = slot % kKv8Page;
@@ -170,10 +180,10 @@ __global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 2 : 3)
         for (int e = 0; e < 8; ++e) turn(y[e], y[8 + e], r[e]);
       }
     } else if constexpr (FORM == kNeighbours) {
-      if (turns && !is_v) {
+      if (!is_v) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (j * 8 + e < half) turn(y[2 * e], y[2 * e + 1], r[e]);
+          if (((e < 4 ? i0 : i1) >> 1) + (e & 3) < half) turn(y[2 * e], y[2 * e + 1], r[e]);
       }
     } else {
       float* b = other_of[warp][unit];
@@ -243,7 +253,7 @@ cudaError_t launch_write(const Kv8WriteArgs& a, cudaStream_t stream) {
   constexpr int kHeads = 32 / LANES;
   const long long steps = (a.hq + 2LL * a.cache.hkv + kHeads - 1) / kHeads;
   const int slices = static_cast<int>(
-      std::min(steps, std::max(1LL, static_cast<long long>(kWarpsWanted / a.tokens))));
+      std::min(steps, static_cast<long long>((kWarpsWanted + a.tokens - 1) / a.tokens)));
   const long long warps = static_cast<long long>(a.tokens) * slices;
   return launch_dependent(kv8_write_kernel<T, LANES, FORM>,
                           dim3(static_cast<unsigned>((warps + kWriteWarps - 1) / kWriteWarps)),
