@@ -50,16 +50,49 @@ constexpr int kThreads = kSoftmax + 256 + 32;
 constexpr int kSpread = 8;        // V exponents this near their tile's largest are taken out of the weights
 constexpr int kApart = 1000;      // others
 
-// D[tmem] (+)= A[tmem] * B[smem desc]: A is F16 pairs, a row per lane.
-__device__ __forceinline__ void umma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                            uint32_t idesc, uint32_t accumulate) {
+// The products' instructions, by the lane for which `on` holds, in code that a
+// whole warp runs: its addresses then stay in uniform registers (one thread's
+// branch took 85 cycles an instruction, more than the product).  Descriptors
+// are two words, of which only the low one moves.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(on));
+  return on != 0u;
+}
+// D[tmem] (+)= A[smem] * B[smem]:
+__device__ __forceinline__ void mma_ss(bool on, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
+                                       uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 a, {%2, %4};\n\tmov.b64 b, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], a, b, %5, p;\n\t}\n" ::"r"(static_cast<uint32_t>(on)),
+      "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// D[tmem] (+)= A[tmem] * B[smem], A being F16 pairs, a row per lane:
+__device__ __forceinline__ void mma_ts(bool on, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t hi,
+                                       uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 b, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], b, %5, p;\n\t}\n" ::"r"(static_cast<uint32_t>(on)),
+      "r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// `bar` is arrived at once the lane's products so far are done.
+__device__ __forceinline__ void mma_commit(bool on, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}\n" ::"r"(
+          static_cast<uint32_t>(on)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+
 // Two F32 operations an instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -202,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2],
       o_done[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int found[2];             // row, tile in the row
+  __shared__ int found[3];             // row, tile in the row, tile of all
   // By key tile: E + 127 of its K; E' of its V, or kApart; and then each key's
   // 2^ev (0 where there is no key) and ev (-inf).
   __shared__ volatile int exps[4][2];
@@ -227,16 +260,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbar_init();
   }
   if (warp == 16) {
-    // The row of this CTA's tile; late tiles, which have the most keys, go first.
-    const int want = static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x);
+    // The row of this CTA's tile.  Late tiles, which have the most keys, go
+    // first, and the CTAs that the grid has too many last.
+    auto tiles_of = [&](int r, bool report) {
+      return r < a.rows ? kv8_row(a, r, group, kCta, tile_from, report, true).chunks : 0;
+    };
+    int total = 0;
+    for (int base = 0; base < a.rows; base += 32)
+      total += __reduce_add_sync(0xffffffffu,
+                                 tiles_of(base + lane, blockIdx.x + blockIdx.y + blockIdx.z == 0));
+    const int want = total - 1 - static_cast<int>(blockIdx.x);
     int row = -1, before = 0;
-    for (int base = 0; base < a.rows && row < 0; base += 32) {
-      const int r = base + lane;
-      int incl = r < a.rows
-                     ? kv8_row(a, r, group, kCta, tile_from, blockIdx.x + blockIdx.y + blockIdx.z == 0,
-                               true).chunks
-                     : 0;
-      const int own = incl;
+    for (int base = 0; want >= 0 && base < a.rows && row < 0; base += 32) {
+      const int own = tiles_of(base + lane, false);
+      int incl = own;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, incl, off);
@@ -254,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       found[0] = row;
       found[1] = want - before;
+      found[2] = want;
     }
   }
   __syncthreads();
@@ -281,81 +319,88 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 16) {
     // ---------------------------------------------------------------- products
-    if (lane == 0 && n > 0) {
-      constexpr uint32_t idesc_s = umma_idesc(kRows, kKeys, 0);
-      constexpr uint32_t idesc_pv = umma_idesc(kRows, D, 0) | (1u << 16);  // V: MN-major
-      const uint32_t base = smem_u32(smem);
-      // A descriptor's address field counts 16 bytes: offsets are added to it.
-      auto scores = [&](int t, int g) {  // S of group g on key tile t
-        const uint64_t qd = sw128_desc(base + T::kQ + (SHARED ? g * T::kOperand : 0u));
-        const uint64_t kd = sw128_desc(base + T::kK + (t & 1) * T::kOperand);
+    constexpr uint32_t idesc_s = umma_idesc(kRows, kKeys, 0);
+    constexpr uint32_t idesc_pv = umma_idesc(kRows, D, 0) | (1u << 16);  // V: MN-major
+    const bool on = elect_one();
+    const uint32_t base = smem_u32(smem);
+    const uint64_t desc_k = sw128_desc(base), desc_v = sw128_desc_mn(base, T::kAtom);
+    const uint32_t k_lo = static_cast<uint32_t>(desc_k), k_hi = static_cast<uint32_t>(desc_k >> 32);
+    const uint32_t v_lo = static_cast<uint32_t>(desc_v), v_hi = static_cast<uint32_t>(desc_v >> 32);
+    // (Through shuffles, so that what follows is uniform to the compiler.)
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const int tiles = __shfl_sync(0xffffffffu, n, 0);
+    // A descriptor's address field counts 16 bytes: offsets are added to it.
+    auto scores = [&](int t, int g) {  // S of group g on key tile t
+      const uint32_t qd = k_lo + ((T::kQ + (SHARED ? g * T::kOperand : 0u)) >> 4);
+      const uint32_t kd = k_lo + ((T::kK + (t & 1) * T::kOperand) >> 4);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = ((kk >> 2) * T::kAtom + (kk & 3) * 32) >> 4;
-          umma_f16(tmem + T::kTmemS + g * 128, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[g]);
-      };
-      auto sums = [&](int t, int g, bool first) {  // O of group g += P V
-        const uint64_t vd = sw128_desc_mn(base + T::kV + (t & 1) * T::kOperand, T::kAtom);
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = ((kk >> 2) * T::kAtom + (kk & 3) * 32) >> 4;
+        mma_ss(on, tm + T::kTmemS + g * 128, qd + off, kd + off, k_hi, idesc_s, kk > 0 ? 1u : 0u);
+      }
+      mma_commit(on, &s_full[g]);
+    };
+    auto sums = [&](int t, int g, bool fresh) {  // O of group g (+)= P V
+      const uint32_t vd = v_lo + ((T::kV + (t & 1) * T::kOperand) >> 4);
 #pragma unroll
-        for (int ks = 0; ks < kKeys / 16; ++ks)
-          umma_f16_ta(tmem + T::kTmemO + g * 128, tmem + T::kTmemS + g * 128 + ks * 8,
-                      vd + ks * (2048 >> 4), idesc_pv, !first || ks > 0 ? 1u : 0u);
-        umma_commit(&o_done[g]);
-      };
-      auto wait = [&](uint64_t* bar, int use) {
-        const bool ok = mbar_wait(bar, use & 1, a.status);
-        tc_fence_after();
-        return ok;
-      };
-      bool ok = wait(&q_full, 0);
-      if (SHARED) {
-        ok = ok && wait(&k_full[0], 0);
-        if (ok) {
-          scores(0, 0);
-          // Half a period behind: one group's weights then run under the
-          // other's products, and neither waits for the exponentials of both.
-          ok = wait(&p_full[0], 0);
-          if (ok) scores(0, 1);
-          umma_commit(&k_empty[0]);
-        }
-        for (int i = 0; ok && i < n; ++i) {
-          const int u = (i + 1) >> 1;  // use of the stage of key tile i + 1
+      for (int ks = 0; ks < kKeys / 16; ++ks)
+        mma_ts(on, tm + T::kTmemO + g * 128, tm + T::kTmemS + g * 128 + ks * 8, vd + ks * (2048 >> 4), v_hi,
+               idesc_pv, !fresh || ks > 0 ? 1u : 0u);
+      mma_commit(on, &o_done[g]);
+    };
+    auto wait = [&](uint64_t* bar, int use) {
+      const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, use & 1, a.status));
+      tc_fence_after();
+      return ok;
+    };
+    bool ok = tiles > 0 && wait(&q_full, 0);
+    if (SHARED) {
+      ok = ok && wait(&k_full[0], 0);
+      if (ok) {
+        scores(0, 0);
+        // Half a period behind: one group's weights then run under the
+        // other's products, and neither waits for the exponentials of both.
+        ok = wait(&p_full[0], 0);
+        if (ok) scores(0, 1);
+        mma_commit(on, &k_empty[0]);
+      }
+#pragma unroll 1
+      for (int t = 0; ok && t < tiles; ++t) {
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            ok = ok && wait(&p_full[g], i);
-            if (g == 0) ok = ok && wait(&v_full[i & 1], i >> 1);
+        for (int g = 0; g < 2; ++g) {
+          ok = ok && wait(&p_full[g], t);
+          if (g == 0) ok = ok && wait(&v_full[t & 1], t >> 1);
+          if (!ok) break;
+          sums(t, g, t == 0);
+          if (g == 1) mma_commit(on, &v_empty[t & 1]);
+          if (t + 1 < tiles) {
+            if (g == 0) ok = wait(&k_full[(t + 1) & 1], (t + 1) >> 1);
             if (!ok) break;
-            sums(i, g, i == 0);
-            if (g == 1) umma_commit(&v_empty[i & 1]);
-            if (i + 1 < n) {
-              if (g == 0) ok = wait(&k_full[(i + 1) & 1], u);
-              if (!ok) break;
-              scores(i + 1, g);
-              if (g == 1) umma_commit(&k_empty[(i + 1) & 1]);
-            }
+            scores(t + 1, g);
+            if (g == 1) mma_commit(on, &k_empty[(t + 1) & 1]);
           }
         }
-      } else {
-        for (int t = 0; ok && t < 2 && t < n; ++t) {
-          ok = wait(&k_full[t], 0);
+      }
+    } else {
+#pragma unroll 1
+      for (int t = 0; ok && t < 2 && t < tiles; ++t) {
+        ok = wait(&k_full[t], 0);
+        if (!ok) break;
+        scores(t, t);
+        mma_commit(on, &k_empty[t]);
+      }
+#pragma unroll 1
+      for (int t = 0; ok && t < tiles; ++t) {
+        const int g = t & 1;
+        ok = wait(&p_full[g], t >> 1) && wait(&v_full[g], t >> 1);
+        if (!ok) break;
+        sums(t, g, t < 2);
+        mma_commit(on, &v_empty[g]);
+        if (t + 2 < tiles) {
+          ok = wait(&k_full[g], (t + 2) >> 1);
           if (!ok) break;
-          scores(t, t);
-          umma_commit(&k_empty[t]);
-        }
-        for (int t = 0; ok && t < n; ++t) {
-          const int g = t & 1;
-          ok = wait(&p_full[g], t >> 1) && wait(&v_full[g], t >> 1);
-          if (!ok) break;
-          sums(t, g, t < 2);
-          umma_commit(&v_empty[g]);
-          if (t + 2 < n) {
-            ok = wait(&k_full[g], (t + 2) >> 1);
-            if (!ok) break;
-            scores(t + 2, g);
-            umma_commit(&k_empty[g]);
-          }
+          scores(t + 2, g);
+          mma_commit(on, &k_empty[g]);
         }
       }
     }
@@ -665,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (ok && (SHARED || g == 0)) {
       const bool split = gridDim.z > 1;
-      const size_t cell = (static_cast<size_t>(gridDim.x - 1 - blockIdx.x) * hkv + kvh) * gridDim.z +
+      const size_t cell = (static_cast<size_t>(found[2]) * hkv + kvh) * gridDim.z +
                           blockIdx.z;
       float4* piece = reinterpret_cast<float4*>(partial + cell * T::kPiece);
       const float inv = 1.f / l;
