@@ -775,9 +775,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     int stage = 0, next = ST - 1;  // of the page at hand, and of the one to fetch
     unsigned phases = 0;           // bit s: parity of stage s's next page
     int i = 0;
+    bool fresh = false;  // a stream's first unit, whose queries are not taken yet
     for (; i < n; ++i) {
       if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phases >> stage & 1u, a.status))) break;
       phases ^= 1u << stage;
+      if (fresh) {  // copied queries have arrived with the unit
+        take_queries(queries_of == opened);
+        fresh = false;
+      }
       const unsigned there = have >> (stage * KP) & ((1u << KP) - 1u);
       if (i + ST - 1 < n) fetch(next, false);  // the stage that every lane has left behind
       const bool ends = at.unit == at.units - 1, more = i + 1 < n;
@@ -786,8 +791,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       if (ends || !more) close(ends, !more);
       if (ends && more) {
         advance(at);
-        starts = true;
-        take_queries(queries_of == ++opened);
+        starts = fresh = true;
+        ++opened;
         open();
       } else {
         ++at.unit;

@@ -633,6 +633,29 @@ def test_streams_repeats_and_workspaces(torch, kv8):
     cache.check()
 
 
+@pytest.mark.parametrize("heads", [(32, 8, 128), (16, 4, 64), (6, 2, 256)])
+def test_cold_memory(torch, kv8, heads):
+    """Caches, tables and queries that are in no cache of the GPU arrive late:
+    many streams a warp, new queries each time, and everything else written
+    over in between."""
+    hq, hkv, d = heads
+    rng = np.random.default_rng(20)
+    rows = [(int(n), 1) for n in rng.integers(20, 1500, 64)]
+    needs = [(n + 15) // 16 for n, _ in rows]
+    cache = random_cache(torch, kv8, rng, sum(needs), hkv, d)
+    table = tables_for(torch, rng, needs, sum(needs))
+    args = (ints(torch, np.arange(len(rows) + 1)), ints(torch, [n for n, _ in rows]), ints(torch, table))
+    sweep = torch.empty(320 << 20, dtype=torch.uint8, device="cuda")
+    work = kv8.attention_workspace(len(rows), len(rows), 1, hq, hkv, d)
+    for i in range(6):
+        q = (1.5 * torch.randn((len(rows), hq * d), device="cuda")).half()
+        sweep.fill_(i)
+        got = kv8.attention(cache, q, *args, max_tokens=1, workspace=work)
+        want, tol = reference(torch, cache, table, rows, q, hq)
+        assert bool(((got.double() - want).abs() <= tol).all()), i
+    cache.check()
+
+
 def test_gpu_side_refusals(torch, kv8):
     cache = kv8.Cache(4, 2, 64)
     rope = kv8.Rope(64, 1e4)
