@@ -43,6 +43,9 @@ def _need(tensor, name: str, dtype, index: int, shape=None, optional=False):
     """Checks one tensor and returns its address (None for a missing optional one)."""
     if tensor is None and optional:
         return None
+    if (isinstance(tensor, torch.Tensor) and tensor.dtype is dtype and tensor.get_device() == index
+            and tensor.is_contiguous() and (shape is None or tensor.shape == shape)):
+        return tensor.data_ptr()
     if not isinstance(tensor, torch.Tensor):
         _refuse(f"{name} must be a tensor")
     if tensor.dtype != dtype:
@@ -51,9 +54,7 @@ def _need(tensor, name: str, dtype, index: int, shape=None, optional=False):
         _refuse(f"{name} is on {tensor.device}, the cache on cuda:{index}")
     if shape is not None and tensor.shape != shape:
         _refuse(f"{name} must have shape {tuple(shape)}, not {tuple(tensor.shape)}")
-    if not tensor.is_contiguous():
-        _refuse(f"{name} must be contiguous")
-    return tensor.data_ptr()
+    _refuse(f"{name} must be contiguous")
 
 
 # The device and stream that torch has current, without the objects around them
@@ -192,8 +193,10 @@ def write(cache: Cache, qkv, positions, slots, rope: Rope, q_norm=None, k_norm=N
     kn = _need(k_norm, "k_norm", torch.float32, index, (d,), optional=True)
     turns = _need(rope.turns, "rope.turns", torch.float64, index)
     if out is None:
-        out = torch.empty((tokens, hq * d), dtype=torch.float16, device=cache.device)
-    o = _need(out, "out", torch.float16, index, (tokens, hq * d))
+        out = qkv.new_empty((tokens, hq * d), dtype=torch.float16)
+        o = out.data_ptr()
+    else:
+        o = _need(out, "out", torch.float16, index, (tokens, hq * d))
     _call("hllm_b200_kv8_write", index, cache._ref, x, _TYPES[qkv.dtype], tokens, hq, p, s, qn,
           kn, eps, turns, rope.rotary_dim, rope.interleaved, rope.factor, o, cache._status)
     return out
@@ -217,9 +220,11 @@ def read(cache: Cache, block_tables, lengths, offsets, tokens: int, first=None,
     c = _need(offsets, "offsets", torch.int32, index, (rows + 1,))
     shape = (tokens, cache.kv_heads, cache.head_dim)
     if out is None:
-        out = (torch.empty(shape, dtype=dtype, device=cache.device),
-               torch.empty(shape, dtype=dtype, device=cache.device))
-    k, v = (_need(x, name, dtype, index, shape) for x, name in zip(out, ("k", "v")))
+        values = cache.k.new_empty(shape, dtype=dtype)
+        out = (values, torch.empty_like(values))
+        k, v = values.data_ptr(), out[1].data_ptr()
+    else:
+        k, v = (_need(x, name, dtype, index, shape) for x, name in zip(out, ("k", "v")))
     _call("hllm_b200_kv8_read", index, cache._ref, t, rows, width, f, n, c, tokens,
           _TYPES[dtype], k, v, cache._status)
     return out
@@ -253,7 +258,7 @@ def attention(cache: Cache, q, cu_seqlens, lengths, block_tables, max_tokens: Op
     if q.get_device() != index:
         _refuse(f"q is on {q.device}, the cache on {cache.device}")
     if out is None:
-        out = torch.empty((tokens, width), dtype=torch.float16, device=cache.device)
+        out = q.new_empty((tokens, width))
     elif (not isinstance(out, torch.Tensor) or out.dtype != torch.float16
           or out.get_device() != index or out.shape != (tokens, width)):
         _refuse(f"out must be a float16 {(tokens, width)} matrix on {cache.device}")
