@@ -446,6 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* const full = values ? v_full : k_full;
     uint64_t* const empty = values ? v_empty : k_empty;
     uint8_t* const operand = smem + (values ? T::kV : T::kK);
+    bool ok = true;
 #pragma unroll 1
     for (int t = 0; t < n; ++t) {
       // The tile's exponents; bytes are e + 127, and 0 is no key's.
@@ -466,7 +467,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       pages = pages_of(ids);  // -1 everywhere past the last tile
       ids = load_ids(t + 2);
       load_scales(t + 1);
-      named_bar_sync(3 + group_of, 128);
+      // All four warps go on, or none: a wait that ran out is known to all here.
+      ok = named_bar_all(3 + group_of, 128, ok);
+      if (!ok) break;
       int e_k = 0, e_v = 0, low = 1000;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -476,8 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // (max (s f) is max (s) f for a scale >= 0 only.)
       const bool apart = e_v - low > kSpread || !(a.scale >= 0.f);
-      const bool ok = t < 2 || mbar_wait(&empty[t & 1], ((t - 2) >> 1) & 1, a.status);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      ok = t < 2 || mbar_wait(&empty[t & 1], ((t - 2) >> 1) & 1, a.status);
       if (!values) {
         // The scores of tile t - 2 followed the sums of tile t - 4, so that
         // tile's entry is read by nobody any more.
