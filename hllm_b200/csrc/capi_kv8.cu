@@ -230,8 +230,7 @@ hllm_b200_status hllm_b200_kv8_attention_workspace(uint32_t rows, uint64_t token
   int sm_count = 0;
   const cudaError_t e = current_sm_count(&sm_count);
   if (e != cudaSuccess) return cuda_status(e);
-  *bytes = hb::kv8_attention_workspace(static_cast<int>(rows), static_cast<int>(tokens),
-                                       static_cast<int>(max_row_tokens), static_cast<int>(hq),
+  *bytes = hb::kv8_attention_workspace(static_cast<int>(max_row_tokens), static_cast<int>(hq),
                                        static_cast<int>(kv_heads), static_cast<int>(head_dim),
                                        sm_count);
   return HLLM_B200_OK;
@@ -282,8 +281,8 @@ hllm_b200_status hllm_b200_kv8_attention(const hllm_b200_kv8* cache, const uint1
   a.workspace = static_cast<float*>(workspace);
   a.status = status;
   a.sm_count = sm_count;
-  if (workspace_bytes < hb::kv8_attention_workspace(a.rows, a.tokens, a.max_row_tokens, a.hq,
-                                                    a.cache.hkv, a.cache.dim, sm_count)) {
+  if (workspace_bytes <
+      hb::kv8_attention_workspace(a.max_row_tokens, a.hq, a.cache.hkv, a.cache.dim, sm_count)) {
     refuse("8-bit KV attention: the workspace is too small");
     return HLLM_B200_RESOURCE_EXHAUSTED;
   }

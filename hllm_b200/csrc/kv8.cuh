@@ -86,13 +86,12 @@ struct Kv8AttnArgs {
 // size, its share of the workspace, and its launches: tiles, then, once the
 // stream pass is launched, the join of their key splits.
 bool kv8_tile_supported(int dim);
-size_t kv8_tile_workspace(int rows, int tokens, int hq, int hkv, int dim, int sm_count);
+size_t kv8_tile_workspace(int dim, int sm_count);
 cudaError_t kv8_tile_launch(const Kv8AttnArgs& a, int tile_from, float* partial, cudaStream_t stream);
 cudaError_t kv8_tile_join_launch(const Kv8AttnArgs& a, int tile_from, const float* partial,
                                  cudaStream_t stream);
 
-size_t kv8_attention_workspace(int rows, int tokens, int max_row_tokens, int hq, int hkv, int dim,
-                               int sm_count);
+size_t kv8_attention_workspace(int max_row_tokens, int hq, int hkv, int dim, int sm_count);
 cudaError_t kv8_attention_launch(const Kv8AttnArgs& a, cudaStream_t stream);
 
 #ifdef __CUDACC__

@@ -34,7 +34,6 @@
 #include <math.h>
 
 #include <algorithm>
-#include <mutex>
 
 #include "common.cuh"
 #include "kv8.cuh"
@@ -226,7 +225,8 @@ struct Record {
 };
 
 // Where column `col` of a stream goes (null past the row's columns), and the
-// factor that makes its sums the output (0: it has no key, and its sums none).
+// factor that makes its sums the output (0: it has no key, or none on a page
+// that is there, and its sums are zeros).
 struct Output {
   __half* to;
   float factor;
@@ -237,7 +237,7 @@ __device__ __forceinline__ Output output_of(const Kv8AttnArgs& a, const Kv8Row& 
   const int token = x.count > 1 ? col / group : 0;
   return Output{a.out + static_cast<size_t>(x.t0 + token) * a.ld_out +
                     static_cast<size_t>(kvh * group + col - token * group) * a.cache.dim,
-                x.len - x.count + token < 0 ? 0.f : 1.f / l};
+                x.len - x.count + token < 0 || l == 0.f ? 0.f : 1.f / l};
 }
 // One unit: sums of two columns at dimensions dim, dim + 1.
 __device__ __forceinline__ void store_unit(const Output& c0, const Output& c1, int dim, const float4& v) {
@@ -954,15 +954,13 @@ __global__ void __launch_bounds__(Join<D, NT>::kThreads, 1) kv8_join_kernel(cons
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
+    const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+                           cudaSuccess && q == cudaDriverEntryPointSuccess;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(found ? p : nullptr);
+  }();
   return fn;
 }
 
@@ -1025,12 +1023,9 @@ size_t stream_workspace(int dim, int sm_count) {
 
 }  // namespace
 
-size_t kv8_attention_workspace(int rows, int tokens, int max_row_tokens, int hq, int hkv, int dim,
-                               int sm_count) {
+size_t kv8_attention_workspace(int max_row_tokens, int hq, int hkv, int dim, int sm_count) {
   return stream_workspace(dim, sm_count) +
-         (with_tiles(max_row_tokens, hq, hkv, dim)
-              ? kv8_tile_workspace(rows, tokens, hq, hkv, dim, sm_count)
-              : 0);
+         (with_tiles(max_row_tokens, hq, hkv, dim) ? kv8_tile_workspace(dim, sm_count) : 0);
 }
 
 cudaError_t kv8_attention_launch(const Kv8AttnArgs& a, cudaStream_t stream) {

@@ -253,7 +253,7 @@ cudaError_t launch_write(const Kv8WriteArgs& a, cudaStream_t stream) {
   constexpr int kHeads = 32 / LANES;
   const long long steps = (a.hq + 2LL * a.cache.hkv + kHeads - 1) / kHeads;
   const int slices = static_cast<int>(
-      std::min(steps, static_cast<long long>((kWarpsWanted + a.tokens - 1) / a.tokens)));
+      std::min(steps, (kWarpsWanted + a.tokens - 1LL) / a.tokens));
   const long long warps = static_cast<long long>(a.tokens) * slices;
   return launch_dependent(kv8_write_kernel<T, LANES, FORM>,
                           dim3(static_cast<unsigned>((warps + kWriteWarps - 1) / kWriteWarps)),

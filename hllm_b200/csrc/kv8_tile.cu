@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const size_t cell = (static_cast<size_t>(found[2]) * hkv + kvh) * gridDim.z +
                           blockIdx.z;
       float4* piece = reinterpret_cast<float4*>(partial + cell * T::kPiece);
-      const float inv = 1.f / l;
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: no key on a page that is there
       __half* out = col < cols ? a.out + static_cast<size_t>(x.t0 + col / group) * a.ld_out +
                                      static_cast<size_t>(kvh * group + col % group) * D
                                : nullptr;
@@ -826,7 +826,7 @@ __global__ void __launch_bounds__(256)
       hi.w += v1.w * w;
     }
     const bool none = x.len - x.count + col / group < 0;
-    const float inv = 1.f / l;
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: no key on a page that is there
     uint4 o = make_uint4(0u, 0u, 0u, 0u);
     if (!none)
       o = make_uint4(half2_bits(lo.x * inv, lo.y * inv), half2_bits(lo.z * inv, lo.w * inv),
@@ -873,10 +873,10 @@ cudaError_t launch_tile(const Kv8AttnArgs& a, const Plan& p, int tile_from, floa
 
 bool kv8_tile_supported(int dim) { return dim == 64 || dim == 128; }
 
-size_t kv8_tile_workspace(int rows, int tokens, int hq, int hkv, int dim, int sm_count) {
-  const Plan p = plan_tiles(rows, tokens, hq, hkv, sm_count);
-  return p.splits == 1 ? 0
-                       : static_cast<size_t>(p.tiles) * hkv * p.splits * 128 * (dim + 2) * sizeof(float);
+size_t kv8_tile_workspace(int dim, int sm_count) {
+  // Splits are made while the CTAs are no more than the SMs; fewer tokens can
+  // have more of them, so the room is for any count up to these.
+  return static_cast<size_t>(sm_count) * 128 * (dim + 2) * sizeof(float);
 }
 
 cudaError_t kv8_tile_launch(const Kv8AttnArgs& a, int tile_from, float* partial, cudaStream_t stream) {

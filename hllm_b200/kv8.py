@@ -232,7 +232,8 @@ def read(cache: Cache, block_tables, lengths, offsets, tokens: int, first=None,
 
 def attention_workspace(rows: int, tokens: int, max_tokens: int, heads: int, kv_heads: int,
                         head_dim: int, device="cuda"):
-    """A workspace for ``attention`` calls of at most these counts."""
+    """A workspace for ``attention`` calls of at most these counts, one after
+    another (calls that run at the same time need one each)."""
     n = C.c_uint64()
     with torch.cuda.device(device):
         _lib.check(lib().hllm_b200_kv8_attention_workspace(rows, tokens, max_tokens, heads, kv_heads,

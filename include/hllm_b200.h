@@ -530,10 +530,11 @@ hllm_b200_status hllm_b200_kv8_read(const hllm_b200_kv8* cache, const int32_t* b
  * are F16 at row stride ld_out; rows of no sequence are left as they are.
  * max_row_tokens bounds the rows' new tokens (1 for a decode batch); a longer
  * row, or one past `tokens` or max_blocks, is skipped and sets a status bit.
- * Keys of a missing page are left out and set one.  q and out are 16-byte
- * aligned, ld_q and ld_out multiples of 8.  `workspace` (16-byte aligned) has
- * at least hllm_b200_kv8_attention_workspace bytes for the same counts; its
- * contents before and after the call mean nothing. */
+ * Keys of a missing page are left out and set one (a token that sees no other
+ * gives zeros).  q and out are 16-byte aligned, ld_q and ld_out multiples of 8.
+ * `workspace` (16-byte aligned) has at least hllm_b200_kv8_attention_workspace
+ * bytes for these or larger counts and the same heads; its contents before and
+ * after the call mean nothing. */
 hllm_b200_status hllm_b200_kv8_attention_workspace(uint32_t rows, uint64_t tokens,
                                                    uint64_t max_row_tokens, uint32_t hq,
                                                    uint32_t kv_heads, uint32_t head_dim,

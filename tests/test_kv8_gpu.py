@@ -633,6 +633,109 @@ def test_streams_repeats_and_workspaces(torch, kv8):
     cache.check()
 
 
+def test_write_in_one_call_or_many(torch, kv8):
+    """How a call's tokens and heads are spread over warps leaves no trace."""
+    rng = np.random.default_rng(30)
+    T, hq, hkv, d = 11000, 3, 1, 64
+    x = torch.randn((T, (hq + 2 * hkv) * d), device="cuda").bfloat16()
+    positions = ints(torch, rng.integers(0, 1 << 20, T))
+    slots = ints(torch, rng.permutation(700 * 16)[:T])
+    norm = torch.rand(d, device="cuda") + 0.5
+    for rope, norms in ((kv8.Rope(d, 1e4), dict(q_norm=norm)),
+                        (kv8.Rope(d, 1e4, rotary_dim=40, interleaved=True), dict(k_norm=norm)),
+                        (kv8.Rope(d, 1e4, rotary_dim=24), {})):
+        one, many = kv8.Cache(700, hkv, d), kv8.Cache(700, hkv, d)
+        q = kv8.write(one, x, positions, slots, rope, **norms)
+        got = torch.empty_like(q)
+        at = 0
+        for n in (1, 2, 5, 60, 400, 1500, T - 1968):
+            part = slice(at, at + n)
+            kv8.write(many, x[part], positions[part], slots[part], rope, out=got[part], **norms)
+            at += n
+        assert at == T and torch.equal(got, q)
+        for a, b in zip(bytes_of(torch, one), bytes_of(torch, many)):
+            assert torch.equal(a, b)
+
+
+def test_read_of_many_rows(torch, kv8):
+    """Rows without tokens, and several rows to a CTA's tokens, past 256 rows."""
+    rng = np.random.default_rng(31)
+    hkv, d = 2, 64
+    lengths = np.where(rng.random(700) < 0.5, 0, rng.integers(0, 40, 700))
+    first = np.minimum(rng.integers(0, 3, 700), lengths)
+    needs = [(int(n) + 15) // 16 for n in lengths]
+    cache = random_cache(torch, kv8, rng, sum(needs), hkv, d)
+    table = tables_for(torch, rng, needs, sum(needs))
+    offsets = 5 + np.concatenate([[0], np.cumsum(lengths - first)])
+    T = int(offsets[-1]) + 9
+    out = tuple(torch.full((T, hkv, d), 7.0, device="cuda") for _ in range(2))
+    kv8.read(cache, ints(torch, table), ints(torch, lengths), ints(torch, offsets), T,
+             first=ints(torch, first), dtype=torch.float32, out=out)
+    cache.check()
+    kc, ks, vc, vs = bytes_of(torch, cache)
+    row = np.repeat(np.arange(700), lengths - first)
+    at = np.arange(len(row)) - (offsets[:-1] - 5)[row] + first[row]
+    page, line = torch.as_tensor(table[row, at // 16]).long().cuda(), torch.as_tensor(at % 16).cuda()
+    for c, s, o in ((kc, ks, out[0]), (vc, vs, out[1])):
+        values = kv8_util.values(torch, c, s).transpose(1, 2)  # [page][16][head][d]
+        want = torch.full((T, hkv, d), 7.0, device="cuda", dtype=torch.float64)
+        want[5:5 + len(row)] = values[page, line]
+        assert torch.equal(o.double(), want)
+
+
+def test_tokens_without_a_page(torch, kv8):
+    """Rows all of whose keys lie on missing pages give zeros, others what they see."""
+    rng = np.random.default_rng(32)
+    for hq, hkv, d, count in ((8, 2, 128, 1), (8, 2, 128, 90), (4, 2, 64, 40), (4, 4, 96, 3)):
+        rows = [(200, count), (150, count), (0, 0), (180, count)]
+        cache = random_cache(torch, kv8, rng, 40, hkv, d)
+        table = tables_for(torch, rng, [13, 10, 0, 12], 40)
+        holes = table.copy()
+        holes[1] = -1
+        holes[3, :] = 40
+        T = 3 * count
+        q = torch.randn((T, hq * d), device="cuda").half()
+        args = (ints(torch, [0, count, 2 * count, 2 * count, T]), ints(torch, [n for n, _ in rows]))
+        got = kv8.attention(cache, q, *args, ints(torch, holes), max_tokens=count)
+        with pytest.raises(StageError, match="out of range"):
+            cache.check()
+        want, tol = reference(torch, cache, table, rows, q, hq)
+        assert bool(((got.double() - want).abs() <= tol)[:count].all())
+        assert bool((got[count:] == 0).all())
+
+
+def test_a_workspace_serves_smaller_calls(torch, kv8):
+    """A workspace for large counts is enough for any smaller ones, whose split
+    over CTAs may be finer; and graphs may share one, replayed in turn."""
+    rng = np.random.default_rng(33)
+    hq, hkv, d = 16, 4, 128
+    work = kv8.attention_workspace(64, 1024, 1024, hq, hkv, d)
+    cache = random_cache(torch, kv8, rng, 300, hkv, d)
+    calls = []
+    for rows in ([(4000, 20)], [(700, 1)], [(64, 64)], [(1500, 100), (900, 1)], [(1024, 1024)]):
+        table = tables_for(torch, rng, [(n + 15) // 16 for n, _ in rows], 300)
+        T = sum(c for _, c in rows)
+        q = torch.randn((T, hq * d), device="cuda").half()
+        args = (q, ints(torch, np.concatenate([[0], np.cumsum([c for _, c in rows])])),
+                ints(torch, [n for n, _ in rows]), ints(torch, table))
+        want = kv8.attention(cache, *args)
+        out = torch.empty_like(want)
+        kv8.attention(cache, *args, out=out, workspace=work)
+        assert torch.equal(out, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kv8.attention(cache, *args, out=out, workspace=work)
+        calls.append((graph, out, want, args))
+    for _ in range(3):
+        for graph, out, _, _ in calls:
+            out.zero_()
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out, want, _ in calls:
+            assert torch.equal(out, want)
+    cache.check()
+
+
 @pytest.mark.parametrize("heads", [(32, 8, 128), (16, 4, 64), (6, 2, 256)])
 def test_cold_memory(torch, kv8, heads):
     """Caches, tables and queries that are in no cache of the GPU arrive late:
@@ -673,6 +776,7 @@ def test_gpu_side_refusals(torch, kv8):
             (lambda: kv8.write(cache, x.cpu(), p, p, rope), "cpu"),
             (lambda: kv8.write(cache, x, p, p, rope, q_norm=torch.ones(63, device="cuda")), "q_norm"),
             (lambda: kv8.write(cache, x, p, p, kv8.Rope(128, 1e4)), "head of 64"),
+            (lambda: kv8.write(cache, x, p, p, rope, q_norm=torch.ones(65, device="cuda")[1:]), "aligned"),
             (lambda: kv8.read(cache, tab, n, p, 3), "offsets"),
             (lambda: kv8.read(cache, tab, n, cu, 3, dtype=torch.int8), "dtype"),
             (lambda: kv8.attention(cache, q.float(), cu, n, tab), "float16"),
