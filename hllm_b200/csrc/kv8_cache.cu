@@ -58,7 +58,7 @@ struct Eight<float> {
 // heads' loads in flight under this step's arithmetic.  A lane holds both
 // members of eight pairs: elements 8 j .. and rotary/2 + 8 j .. of a head (past
 // `rotary`, and where pairs are neighbours: of halves of that), so pairs meet in
-// registers, and the lane keeps its pairs' cosines for all the token's heads.
+// registers; the pairs' cosines serve all the token's heads.
 // Where rotary / 2 is not a multiple of 8 (kExchange) chunks of eight would
 // cross a border, and a lane takes 16 consecutive elements and fetches the
 // other members through shared memory.
@@ -71,9 +71,9 @@ constexpr int kWriteThreads = 128;
 constexpr int kWriteWarps = kWriteThreads / 32;
 // Warps that a call should have (three rounds of full SMs): below it a token's
 // heads are spread over several warps, each with the token's cosines to
-// compute.  8192 tokens of 32 + 8 + 8 heads of 128: 45 us so, 48 at one round;
-// 128 threads a CTA and 80 registers (24 warps an SM) 45 us, 96 registers 46,
-// the loads of two steps ahead at 116 registers 51.
+// compute.  8192 tokens of 32 + 8 + 8 heads of 128 in F16: 40.5 us (4.6 TB/s) so,
+// 48 at one round; the cosines in registers (80 of them a thread) 45, the loads
+// of two steps ahead 44.
 constexpr int kWarpsWanted = 148 * 24 * 3;
 enum { kHalves, kNeighbours, kExchange };
 
@@ -124,6 +124,13 @@ __global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 4 : 6)
   int h = slice * kHeads + unit;
   fetch(h);
   float2* cs = turns_of[warp];
+  // Where pair i lies: a lane's pairs LANES apart, so that lanes read side by side.
+  auto place = [&](int i) {
+    if (FORM == kExchange) return i;
+    if (FORM == kHalves) return (i & 7) * LANES + (i >> 3);
+    const int q = d >> 2, hi = i >= q ? 1 : 0, k = i - hi * q;
+    return (hi * 4 + (k & 3)) * LANES + (k >> 2);
+  };
   for (int i = lane; i < half; i += 32) {
     const double all = static_cast<double>(pos) * a.turns[i];
     const double part = 2.0 * (all - rint(all));  // half turns, -1 .. 1
@@ -131,19 +138,12 @@ __global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 4 : 6)
     const float r = static_cast<float>(part - f) * 3.14159265f;
     float s, c;
     sincospif(f, &s, &c);
-    cs[i] = make_float2((c - r * s) * a.factor, (s + r * c) * a.factor);
+    cs[place(i)] = make_float2((c - r * s) * a.factor, (s + r * c) * a.factor);
   }
   const bool stored = slot >= 0 && slot < a.cache.blocks * kKv8Page;
   if (slice == 0 && lane == 0 && slot >= 0 && !stored) atomicOr(a.status, kDevBadIndex);
   __syncwarp();
-  float2 r[8];
-  if (FORM != kExchange) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int pair = FORM == kHalves ? j * 8 + e : ((e < 4 ? i0 : i1) >> 1) + (e & 3);
-      r[e] = used && pair < half ? cs[pair] : make_float2(1.f, 0.f);
-    }
-  }
+  auto r = [&](int e) { return cs[e * LANES + j]; };
   const size_t page = static_cast<size_t>(stored ? slot / kKv8Page : 0) * hkv;
   const int in_page = slot % kKv8Page;
 
@@ -177,13 +177,13 @@ __global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 4 : 6)
     if constexpr (FORM == kHalves) {
       if (turns && !is_v) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) turn(y[e], y[8 + e], r[e]);
+        for (int e = 0; e < 8; ++e) turn(y[e], y[8 + e], r(e));
       }
     } else if constexpr (FORM == kNeighbours) {
       if (!is_v) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (((e < 4 ? i0 : i1) >> 1) + (e & 3) < half) turn(y[2 * e], y[2 * e + 1], r[e]);
+          if (((e < 4 ? i0 : i1) >> 1) + (e & 3) < half) turn(y[2 * e], y[2 * e + 1], r(e));
       }
     } else {
       float* b = other_of[warp][unit];

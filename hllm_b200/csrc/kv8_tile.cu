@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2],
       o_done[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ float2 group_ml[2][kRows];  // m and l of the groups, where they share a tile
   __shared__ int found[3];             // row, tile in the row, tile of all
   // By key tile: E + 127 of its K; E' of its V, or kApart; and then each key's
   // 2^ev (0 where there is no key) and ev (-inf).
@@ -294,10 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       found[2] = want;
     }
   }
-  __syncthreads();
-  const int row = found[0];
-  if (row < 0) return;  // the whole CTA: fewer tiles than the grid has room for
-  if (warp == 16) {
+  if (warp == 0) {
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
   }
@@ -305,6 +303,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  const int row = found[0];
+  if (row < 0) {  // the whole CTA: fewer tiles than the grid has room for
+    if (warp == 0) tmem_dealloc(tmem, 512);
+    return;
+  }
 
   const Kv8Row x = kv8_row(a, row, group, kCta, tile_from, false, true);
   const int kvh = blockIdx.y, hkv = a.cache.hkv;
@@ -667,79 +670,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       mbar_arrive(&p_full[g]);
     }
-    if (ok && mine > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&o_done[g], (mine - 1) & 1, a.status));
-      tc_fence_after();
-    }
-    // Row sums of O, 32 dimensions at a time; zeros where this group had no key tile.
-    auto load_o = [&](int c, float (&v)[32]) {
-      uint32_t w[32];
-      if (mine > 0) {
-        tmem_ld32_nowait(oa + c, w);
-        tmem_ld_wait();
-      }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = mine > 0 ? __uint_as_float(w[i]) : 0.f;
+    // The sums are whole: those of this group, or, where both work on one tile of
+    // queries, of both (a group without a key tile has none).
+    auto finish = [&](int h) {  // the last of group h's products
+      const int uses = SHARED ? n : (n + 1 - h) >> 1;
+      if (uses > 0) ok = ok && mbar_wait(&o_done[h], (uses - 1) & 1, a.status);
+      return uses > 0;
     };
-    float4* half = reinterpret_cast<float4*>(smem + T::kK);  // K and V are done with
-    float2* half_ml = reinterpret_cast<float2*>(half + 128 * (D / 4));
-    float wo = 1.f, wh = 0.f;  // weights of this group's sums and of the other's
-    if (!SHARED) {
-      // Group 1's half goes through shared memory to group 0, once both
-      // groups' products are done.
-      if (g == 1 && ok && n > 0)
-        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[0], (((n + 1) >> 1) - 1) & 1, a.status));
-      if (g == 1 && ok) {
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          float v[32];
-          load_o(c, v);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            half[(c / 4 + i) * 128 + tid] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        }
-        half_ml[tid] = make_float2(m, l);
-      }
+    float w0 = 1.f, w1 = 0.f;  // weights of the groups' sums
+    bool have0, have1 = false;
+    if (SHARED) {
+      have0 = finish(g);
+      ok = __all_sync(0xffffffffu, ok);
+    } else {
+      group_ml[g][tid] = make_float2(m, l);
+      have0 = finish(0);
+      have1 = finish(1);
       ok = named_bar_all(1, kSoftmax, ok);
-      if (g == 0 && ok && n > 1) {
-        const float2 o = half_ml[tid];
-        const float mm = fmaxf(m, o.x);
-        wo = ex2(m - mm);
-        wh = ex2(o.x - mm);
-        l = l * wo + o.y * wh;
-        m = mm;
-      }
+      const float2 x0 = group_ml[0][tid], x1 = group_ml[1][tid];
+      m = fmaxf(x0.x, x1.x);
+      w0 = ex2(x0.x - m);
+      w1 = ex2(x1.x - m);
+      l = x0.y * w0 + x1.y * w1;
     }
-    if (ok && (SHARED || g == 0)) {
-      const bool split = gridDim.z > 1;
-      const size_t cell = (static_cast<size_t>(found[2]) * hkv + kvh) * gridDim.z +
-                          blockIdx.z;
+    tc_fence_after();
+    if (ok) {
+      const bool split = !SHARED && gridDim.z > 1;
+      const size_t cell = (static_cast<size_t>(found[2]) * hkv + kvh) * gridDim.z + blockIdx.z;
       float4* piece = reinterpret_cast<float4*>(partial + cell * T::kPiece);
       const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: no key on a page that is there
       __half* out = col < cols ? a.out + static_cast<size_t>(x.t0 + col / group) * a.ld_out +
                                      static_cast<size_t>(kvh * group + col % group) * D
                                : nullptr;
+      // 16 dimensions at a time; groups that share their rows take half each.
+      const uint32_t from = SHARED ? oa : lanes + T::kTmemO;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        float v[32];
-        load_o(c, v);
-        if (!SHARED && n > 1) {
+      for (int c = SHARED ? 0 : g * (D / 2); c < (SHARED ? D : (g + 1) * (D / 2)); c += 16) {
+        uint32_t v0[16], v1[16];
+        if (have0) tmem_ld16_nowait(from + c, v0);
+        if (!SHARED && have1) tmem_ld16_nowait(from + 128 + c, v1);
+        tmem_ld_wait();
+        float v[16];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 o = half[(c / 4 + i) * 128 + tid];
-            v[4 * i] = v[4 * i] * wo + o.x * wh;
-            v[4 * i + 1] = v[4 * i + 1] * wo + o.y * wh;
-            v[4 * i + 2] = v[4 * i + 2] * wo + o.z * wh;
-            v[4 * i + 3] = v[4 * i + 3] * wo + o.w * wh;
-          }
+        for (int i = 0; i < 16; ++i) {
+          v[i] = have0 ? __uint_as_float(v0[i]) * w0 : 0.f;
+          if (!SHARED && have1) v[i] += __uint_as_float(v1[i]) * w1;
         }
-        if (!SHARED && split) {
+        if (split) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
+          for (int i = 0; i < 4; ++i)
             piece[(c / 4 + i) * 128 + tid] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         } else if (out) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 2; ++i) {
             uint32_t h[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -748,14 +731,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (!SHARED && split)
-        reinterpret_cast<float2*>(piece + 128 * (D / 4))[tid] = make_float2(m, l);
+      if (split && g == 0) reinterpret_cast<float2*>(piece + 128 * (D / 4))[tid] = make_float2(m, l);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 16) tmem_dealloc(tmem, 512);
+  if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
 // Joins the key splits of a query tile in order: one CTA a tile and kv head.
