@@ -168,6 +168,7 @@ class Rope:
         _lib.check(lib().hllm_b200_rope_turns(C.byref(desc), turns, C.byref(factor)))
         self.factor = factor.value
         self.turns = torch.tensor(list(turns), dtype=torch.float64).to(device)
+        self._index, self._turns = self.turns.get_device(), self.turns.data_ptr()
 
 
 def write(cache: Cache, qkv, positions, slots, rope: Rope, q_norm=None, k_norm=None,
@@ -191,14 +192,15 @@ def write(cache: Cache, qkv, positions, slots, rope: Rope, q_norm=None, k_norm=N
     s = _need(slots, "slots", torch.int32, index, (tokens,))
     qn = _need(q_norm, "q_norm", torch.float32, index, (d,), optional=True)
     kn = _need(k_norm, "k_norm", torch.float32, index, (d,), optional=True)
-    turns = _need(rope.turns, "rope.turns", torch.float64, index)
+    if rope._index != index:
+        _refuse(f"rope's table is on {rope.turns.device}, the cache on {cache.device}")
     if out is None:
         out = qkv.new_empty((tokens, hq * d), dtype=torch.float16)
         o = out.data_ptr()
     else:
         o = _need(out, "out", torch.float16, index, (tokens, hq * d))
     _call("hllm_b200_kv8_write", index, cache._ref, x, _TYPES[qkv.dtype], tokens, hq, p, s, qn,
-          kn, eps, turns, rope.rotary_dim, rope.interleaved, rope.factor, o, cache._status)
+          kn, eps, rope._turns, rope.rotary_dim, rope.interleaved, rope.factor, o, cache._status)
     return out
 
 
@@ -259,7 +261,7 @@ def attention(cache: Cache, q, cu_seqlens, lengths, block_tables, max_tokens: Op
     if q.get_device() != index:
         _refuse(f"q is on {q.device}, the cache on {cache.device}")
     if out is None:
-        out = q.new_empty((tokens, width))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif (not isinstance(out, torch.Tensor) or out.dtype != torch.float16
           or out.get_device() != index or out.shape != (tokens, width)):
         _refuse(f"out must be a float16 {(tokens, width)} matrix on {cache.device}")
