@@ -285,15 +285,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == 16) {
     // The row of this CTA's tile.  Late tiles, which have the most keys, go
-    // first, and the CTAs that the grid has too many last.
+    // first, all kv heads of one together, and the CTAs that the grid has too
+    // many last.
     auto tiles_of = [&](int r, bool report) {
       return r < a.rows ? kv8_row(a, r, group, kCta, tile_from, report, true).chunks : 0;
     };
     int total = 0;
     for (int base = 0; base < a.rows; base += 32)
       total += __reduce_add_sync(0xffffffffu,
-                                 tiles_of(base + lane, blockIdx.x + blockIdx.y + blockIdx.z == 0));
-    const int want = total - 1 - static_cast<int>(blockIdx.x);
+                                 tiles_of(base + lane, blockIdx.x + blockIdx.z == 0));
+    const int want = total - 1 - static_cast<int>(blockIdx.x) / a.cache.hkv;
     int row = -1, before = 0;
     for (int base = 0; want >= 0 && base < a.rows && row < 0; base += 32) {
       const int own = tiles_of(base + lane, false);
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   const Kv8Row x = kv8_row(a, row, group, kCta, tile_from, false, true);
-  const int kvh = blockIdx.y, hkv = a.cache.hkv;
+  const int hkv = a.cache.hkv, kvh = blockIdx.x % hkv;
   const int x0 = found[1] * kCta, cols = x.count * group;
   const int past = x.len - x.count;  // position of the row's first new token
   // Keys that the CTA's last column sees, and this split's share of their tiles.
@@ -885,7 +886,7 @@ cudaError_t launch_tile(const Kv8AttnArgs& a, const Plan& p, int tile_from, floa
   static Kv8Configured configured;
   const cudaError_t e = configured.once(kv8_tile_kernel<D, SHARED>, static_cast<int>(T::kSmem));
   if (e != cudaSuccess) return e;
-  return launch_dependent(kv8_tile_kernel<D, SHARED>, dim3(p.tiles, a.cache.hkv, p.splits), dim3(kThreads),
+  return launch_dependent(kv8_tile_kernel<D, SHARED>, dim3(p.tiles * a.cache.hkv, 1, p.splits), dim3(kThreads),
                           T::kSmem, stream, a, a.hq / a.cache.hkv, tile_from, partial);
 }
 
