@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       o_done[2];
   __shared__ uint32_t tmem_slot;
   __shared__ float2 group_ml[2][kRows];  // m and l of the groups, where they share a tile
-  __shared__ int found[3];             // row, tile in the row, tile of all
+  __shared__ int found[3];             // row, tile of the row, tile of all rows
   // By key tile: E + 127 of its K; E' of its V, or kApart; and then each key's
   // 2^ev (0 where there is no key) and ev (-inf).
   __shared__ volatile int exps[4][2];
@@ -284,39 +284,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbar_init();
   }
   if (warp == 16) {
-    // The row of this CTA's tile.  Late tiles, which have the most keys, go
-    // first, all kv heads of one together, and the CTAs that the grid has too
-    // many last.
-    auto tiles_of = [&](int r, bool report) {
-      return r < a.rows ? kv8_row(a, r, group, kCta, tile_from, report, true).chunks : 0;
-    };
-    int total = 0;
-    for (int base = 0; base < a.rows; base += 32)
-      total += __reduce_add_sync(0xffffffffu,
-                                 tiles_of(base + lane, blockIdx.x + blockIdx.z == 0));
-    const int want = total - 1 - static_cast<int>(blockIdx.x) / a.cache.hkv;
-    int row = -1, before = 0;
-    for (int base = 0; want >= 0 && base < a.rows && row < 0; base += 32) {
-      const int own = tiles_of(base + lane, false);
-      int incl = own;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += v;
+    // The row of this CTA's tile: of 32 rows the one with the most keys first,
+    // and of a row the late tiles; all kv heads of a tile together; and the CTAs
+    // that the grid has too many last.
+    const bool reports = blockIdx.x + blockIdx.z == 0;
+    int w = static_cast<int>(blockIdx.x) / a.cache.hkv;  // tiles before it
+    int row = -1, tile = 0, cell = 0, tiles_before = 0;  // cell: its number in the rows' order
+    for (int base = 0; base < a.rows && (row < 0 || reports); base += 32) {
+      int own = 0, len = -1;
+      if (base + lane < a.rows) {
+        const Kv8Row x = kv8_row(a, base + lane, group, kCta, tile_from, reports, true);
+        own = x.chunks;
+        len = x.len;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > want);
+      int first = 0, lower = 0;  // tiles of rows that go before this one, and that stand before it
+      for (int j = 0; j < min(32, a.rows - base); ++j) {
+        const int chunks = __shfl_sync(0xffffffffu, own, j), keys = __shfl_sync(0xffffffffu, len, j);
+        if (keys > len || (keys == len && j < lane)) first += chunks;
+        if (j < lane) lower += chunks;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, row < 0 && w >= first && w < first + own);
       if (hit) {
         const int src = __ffs(hit) - 1;
         row = base + src;
-        before += __shfl_sync(0xffffffffu, incl - own, src);
-      } else {
-        before += __shfl_sync(0xffffffffu, incl, 31);
+        tile = __shfl_sync(0xffffffffu, own - 1 - (w - first), src);
+        cell = tiles_before + __shfl_sync(0xffffffffu, lower, src) + tile;
       }
+      const int sum = __reduce_add_sync(0xffffffffu, own);
+      w -= sum;
+      tiles_before += sum;
     }
     if (lane == 0) {
       found[0] = row;
-      found[1] = want - before;
-      found[2] = want;
+      found[1] = tile;
+      found[2] = cell;
     }
   }
   if (warp == 0) {

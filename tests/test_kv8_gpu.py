@@ -428,6 +428,17 @@ def test_nan_in_a_seen_key_reaches_its_heads_alone(torch, kv8, count):
             assert bool(got[seen][:, 4:, 5].isnan().all())
 
 
+@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 1, 64)])
+def test_many_chunks(torch, kv8, heads):
+    """More chunk rows than are looked at together, of any order of lengths,
+    among single tokens and rows without any."""
+    rng = np.random.default_rng(34)
+    counts = rng.choice([0, 1, 3, 16, 17, 40, 64, 129], 75)
+    rows = [(int(c + rng.integers(0, 300)), int(c)) for c in counts]
+    check_attention(torch, kv8, *heads, rows, seed=35)
+    check_attention(torch, kv8, *heads, [(n, c) for n, c in rows if c >= 16][:40], seed=36)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_two_query_tiles_a_cta(torch, kv8, d):
     """Enough columns for CTAs of two query tiles: sharp and flat scores, weights
