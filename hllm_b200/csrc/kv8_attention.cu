@@ -136,7 +136,7 @@ struct Shape : Layout<D> {
   static constexpr int kCols = 8 * NT;
   // Enough warps to hide the latency of one unit's chain of products, and
   // enough bytes in flight to hide that of memory (132 KB an SM at D = 128).
-  static constexpr int KP = NT > 1 || D > 128 ? 1 : D > 64 ? 2 : 4;  // pages of a unit
+  static constexpr int KP = D * NT > 128 ? 1 : D * NT > 64 || NT > 1 ? 2 : 4;  // pages of a unit
   static constexpr int kWarps = D * NT > 64 ? 8 : 12;
   static constexpr int kThreads = kWarps * 32;
   // A piece: D / 16 x NT fragments of 32 lanes x 4 sums, then cols x (m, l).
