@@ -136,7 +136,10 @@ struct Shape : Layout<D> {
   static constexpr int kCols = 8 * NT;
   // Enough warps to hide the latency of one unit's chain of products, and
   // enough bytes in flight to hide that of memory (132 KB an SM at D = 128).
-  static constexpr int KP = D * NT > 128 ? 1 : D * NT > 64 || NT > 1 ? 2 : 4;  // pages of a unit
+  // Pages of a unit, which share its waits and copies, and of them at a time in
+  // registers.
+  static constexpr int KP = D > 128 ? 1 : D > 64 || NT > 1 ? 2 : 4;
+  static constexpr int MP = D * NT > 128 ? 1 : KP;
   static constexpr int kWarps = D * NT > 64 ? 8 : 12;
   static constexpr int kThreads = kWarps * 32;
   // A piece: D / 16 x NT fragments of 32 lanes x 4 sums, then cols x (m, l).
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     kv8_stream_kernel(const __grid_constant__ PoolMaps maps, const Kv8AttnArgs a, int group,
                       int tile_from, bool beside) {
   using S = Shape<D, NT>;
-  constexpr int kCols = S::kCols, kWarps = S::kWarps, ST = S::kStages, KP = S::KP;
+  constexpr int kCols = S::kCols, kWarps = S::kWarps, ST = S::kStages, KP = S::KP, MP = S::MP;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -569,10 +572,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     const bool swap = S::swapped(g, tq);
     const uint32_t pair_lo = swap ? 0x1504u : 0x5140u, pair_hi = swap ? 0x3726u : 0x7362u;
     const int mine = S::key_of(g);  // key of score row g
-    auto multiply = [&](const uint8_t* unit, const uint8_t* scales, unsigned there) {
-      float s[KP][NT][2][4];
+    auto multiply = [&](const uint8_t* unit, const uint8_t* scales, unsigned there, int key) {
+      float s[MP][NT][2][4];
 #pragma unroll
-      for (int j = 0; j < KP; ++j) {
+      for (int j = 0; j < MP; ++j) {
         const uint8_t* page = unit + j * S::kPage;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -594,10 +597,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
           }
         }
       }
-      float ks[KP][2];
-      uint32_t vb[KP][2];
+      float ks[MP][2];
+      uint32_t vb[MP][2];
 #pragma unroll
-      for (int j = 0; j < KP; ++j)
+      for (int j = 0; j < MP; ++j)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint8_t* sc = scales + j * 32 + mine + 8 * h;
@@ -606,21 +609,20 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
           vb[j][h] = max(static_cast<uint32_t>(sc[16]), 1u);
         }
 #pragma unroll
-      for (int j = 0; j < KP; ++j)
+      for (int j = 0; j < MP; ++j)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             s[j][nt][0][e] = (s[j][nt][0][e] + s[j][nt][1][e]) * ks[j][e >> 1];
-      const int key = at.unit * (KP * kKv8Page);
-      const bool at_edge = key + KP * kKv8Page - 1 > edge || there != (1u << KP) - 1u;
-      int end[KP];  // first key of the page that is not there
+      const bool at_edge = key + MP * kKv8Page - 1 > edge || there != (1u << MP) - 1u;
+      int end[MP];  // first key of the page that is not there
 #pragma unroll
-      for (int j = 0; j < KP; ++j) end[j] = there >> j & 1u ? at.x.len : 0;
+      for (int j = 0; j < MP; ++j) end[j] = there >> j & 1u ? at.x.len : 0;
       if (at_edge) {
         // A unit that ends past the last key or some column's, or lacks a page.
 #pragma unroll
-        for (int j = 0; j < KP; ++j)
+        for (int j = 0; j < MP; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int k = key + j * kKv8Page + mine + 8 * h;
@@ -632,11 +634,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
                 if (k > lim[nt][e] || k >= end[j]) s[j][nt][0][2 * h + e] = -INFINITY;
           }
       }
-      float p[KP][NT][4], top;
+      float p[MP][NT][4], top;
       auto weigh = [&]() {
         top = 0.f;
 #pragma unroll
-        for (int j = 0; j < KP; ++j)
+        for (int j = 0; j < MP; ++j)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -654,7 +656,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
           for (int e = 0; e < 2; ++e) {
             float mx = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < KP; ++j)
+            for (int j = 0; j < MP; ++j)
 #pragma unroll
               for (int h = 0; h < 2; ++h)
                 mx = fmaxf(mx, s[j][nt][0][2 * h + e] + static_cast<float>(static_cast<int>(vb[j][h]) - 127));
@@ -674,7 +676,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
         weigh();
       }
 #pragma unroll
-      for (int j = 0; j < KP; ++j) {
+      for (int j = 0; j < MP; ++j) {
         uint32_t pb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -788,7 +790,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       const unsigned there = have >> (stage * KP) & ((1u << KP) - 1u);
       if (i + ST - 1 < n) fetch(next, false);  // the stage that every lane has left behind
       const bool ends = at.unit == at.units - 1, more = i + 1 < n;
-      if (there) multiply(ring + stage * S::kStage, ring + S::kScalesAt + stage * (32 * KP), there);
+#pragma unroll 1
+      for (int j = 0; j < KP; j += MP)
+        if (const unsigned some = there >> j & ((1u << MP) - 1u))
+          multiply(ring + stage * S::kStage + j * S::kPage, ring + S::kScalesAt + stage * (32 * KP) + j * 32,
+                   some, (at.unit * KP + j) * kKv8Page);
       __syncwarp();
       if (ends || !more) close(ends, !more);
       if (ends && more) {
