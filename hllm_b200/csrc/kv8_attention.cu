@@ -12,8 +12,8 @@
 // nothing.
 //
 // Work.  A row's new tokens and the query heads of one kv head form columns
-// (token, head), 8 NT of them a stream; a stream walks the row's pages, two at a
-// time (a unit).  The batch's units in order are one sequence, cut evenly over
+// (token, head), 8 NT of them a stream; a stream walks the row's pages, one to
+// four at a time (a unit).  The batch's units in order are one sequence, cut evenly over
 // the CTAs of one wave and, within a CTA, over its warps, whatever the rows'
 // lengths.  Everything about the cut follows from the lengths on the device:
 // a captured launch serves any lengths.  What a cut leaves of a stream is
@@ -30,6 +30,13 @@
 // for PV the bytes of four keys, paired by byte permutes.  Pages arrive by TMA,
 // one lane of a warp asking for its warp's, in boxes whose swizzle spreads each
 // read over all banks (rows and the order of reads are chosen for that).
+//
+// Bound by memory where rows are long: 64 rows of 1024 to 16384 keys, 32 heads on
+// 8 of 128, 141 us for 768 MB, 5.4 TB/s.  There a warp's unit of two pages is 2600
+// cycles, 1050 of them for asking for the next one.  Short calls are latency: one
+// row of 1000 keys 9.7 us, of which the way from the lengths over the table to the
+// first page is about 4, the joins 4.  The same rows with 16 query heads on a kv
+// head: 186 us (as two streams of 8 columns each, 265).
 #include <cudaTypedefs.h>
 #include <math.h>
 
@@ -135,9 +142,10 @@ struct Shape : Layout<D> {
   using Layout<D>::VW;
   static constexpr int kCols = 8 * NT;
   // Enough warps to hide the latency of one unit's chain of products, and
-  // enough bytes in flight to hide that of memory (132 KB an SM at D = 128).
+  // enough bytes in flight to hide that of memory (192 KB an SM at D = 128).
   // Pages of a unit, which share its waits and copies, and of them at a time in
-  // registers.
+  // registers.  64 long rows: D = 64, 8 columns 100 us at two pages a unit, 87 at
+  // four; 16 columns, D = 64 173 at one, 135 at two; D = 128 215 and 186.
   static constexpr int KP = D > 128 ? 1 : D > 64 || NT > 1 ? 2 : 4;
   static constexpr int MP = D * NT > 128 ? 1 : KP;
   static constexpr int kWarps = D * NT > 64 ? 8 : 12;
@@ -1016,7 +1024,10 @@ size_t piece_bytes(int dim, int nt) {
 
 // Rows with this many columns (new tokens x query heads of a group) go to the
 // tile pass: half a tile of queries, from where its products beat walking the
-// pages once for every 16 columns.
+// pages once for every 8 columns.  Eight rows on 8 kv heads behind 4000 keys, tile
+// and stream pass: 64 columns 43 and 53 us at head size 64, 56 and 71 at 128; 32
+// columns 59 and 33, 67 and 41; 64 columns behind 500 keys 18.6 and 18.5, 20.6 and
+// 22.3.
 constexpr int kTileFrom = 64;
 
 bool with_tiles(int max_row_tokens, int hq, int hkv, int dim) {

@@ -33,7 +33,17 @@
 // one reference m for  l = sum 2^(s_j - m)  and  O = sum (2^(s_j - m) 2^ev_j) d_j,
 // d_j the codes: the weights in brackets are what F16 has to hold, so m follows
 // max (s_j + ev_j), lazily, and o = O / l.  (2^(s_j - m + E') 2^(ev_j - E') d_j
-// where E' is taken out: the weights are then the exponentials themselves.)  Every wait is bounded (common.cuh).
+// where E' is taken out: the weights are then the exponentials themselves.)
+// Every wait is bounded (common.cuh).
+//
+// Measured, 32 heads on 8 of 128: 2048 tokens behind 8192 keys 372 us (831
+// TFLOP/s of the causal products, 49 % of what cuBLAS reaches), 512 behind 1024
+// 28.8 us (373).  A step with two query tiles is 4.7k cycles, of which the products
+// are 2.8k: the rest is a group's chain, scores, maximum and exponentials (3.0k),
+// products, next scores, for which TMEM has no second buffer beside two results of
+// 128 dimensions.  With one query tile a step is 2.5k, and the codes' conversion
+// (2.7k a tile, K and V side by side) is as long.  Unrolling the passes over the
+// scores, or keeping 64 of them in registers, was slower by a third.
 #include <algorithm>
 #include <type_traits>
 
@@ -248,6 +258,18 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, const Share<D>& h, int
   }
 }
 
+// Keys that the last of `columns` columns from x0 on sees.
+__device__ __forceinline__ int seen_keys(const Kv8Row& x, int group, int x0, int columns) {
+  const int last_token = (min(x0 + columns, x.count * group) - 1) / group;
+  return max(0, x.len - x.count + last_token + 1);
+}
+// The splits that `tiles` key tiles are worth, of those that were launched: a
+// piece costs about two tiles to begin and to join.
+constexpr int kLeastTiles = 4;
+__device__ __forceinline__ int parts_of(int tiles, int splits) {
+  return max(1, min(splits, tiles / kLeastTiles));
+}
+
 template <int D, bool SHARED>
 __global__ void __launch_bounds__(kThreads, 1)
     kv8_tile_kernel(const Kv8AttnArgs a, int group, int tile_from, float* partial) {
@@ -339,11 +361,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int x0 = found[1] * kCta, cols = x.count * group;
   const int past = x.len - x.count;  // position of the row's first new token
   // Keys that the CTA's last column sees, and this split's share of their tiles.
-  const int last_token = (min(x0 + kCta, cols) - 1) / group;
-  const int keys = max(0, past + last_token + 1);
+  const int keys = seen_keys(x, group, x0, kCta);
   const int all = (keys + kKeys - 1) / kKeys;
-  const int kt0 = static_cast<int>(static_cast<long long>(all) * blockIdx.z / gridDim.z);
-  const int n = static_cast<int>(static_cast<long long>(all) * (blockIdx.z + 1) / gridDim.z) - kt0;
+  const int parts = parts_of(all, gridDim.z), part = blockIdx.z;
+  if (part >= parts) {  // too few keys for this many splits
+    if (warp == 0) tmem_dealloc(tmem, 512);
+    return;
+  }
+  const int kt0 = static_cast<int>(static_cast<long long>(all) * part / parts);
+  const int n = static_cast<int>(static_cast<long long>(all) * (part + 1) / parts) - kt0;
 
   if (warp == 16) {
     // ---------------------------------------------------------------- products
@@ -735,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_after();
     if (ok) {
-      const bool split = !SHARED && gridDim.z > 1;
+      const bool split = !SHARED && parts > 1;
       const size_t cell = (static_cast<size_t>(found[2]) * hkv + kvh) * gridDim.z + blockIdx.z;
       float4* piece = reinterpret_cast<float4*>(partial + cell * T::kPiece);
       const float inv = l == 0.f ? 0.f : 1.f / l;  // 0: no key on a page that is there
@@ -818,6 +844,8 @@ __global__ void __launch_bounds__(256)
   if (found[0] < 0) return;
   const Kv8Row x = kv8_row(a, found[0], group, kRows, tile_from, false, true);
   const int kvh = blockIdx.y, x0 = found[1] * kRows, cols = x.count * group;
+  const int parts = parts_of((seen_keys(x, group, x0, kRows) + kKeys - 1) / kKeys, splits);
+  if (parts == 1) return;  // the tile pass wrote the result
   const float4* base = reinterpret_cast<const float4*>(
       partial + (static_cast<size_t>(blockIdx.x) * a.cache.hkv + kvh) * splits * T::kPiece);
   // A thread takes one row's eight dimensions.
@@ -829,10 +857,10 @@ __global__ void __launch_bounds__(256)
                                                     128 * (D / 4)) + r);
     };
     float m = kNoReference;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, ml_of(s).x);
+    for (int s = 0; s < parts; ++s) m = fmaxf(m, ml_of(s).x);
     float l = 0.f;
     float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
-    for (int s = 0; s < splits; ++s) {
+    for (int s = 0; s < parts; ++s) {
       const float4* piece = base + static_cast<size_t>(s) * (T::kPiece / 4);
       const float2 ml = ml_of(s);
       const float w = ex2(ml.x - m);
@@ -867,7 +895,7 @@ struct Plan {
   bool shared;
   int tiles, splits;
 };
-constexpr int kMostSplits = 8;
+constexpr int kMostSplits = 16;
 Plan plan_tiles(int rows, int tokens, int hq, int hkv, int sm_count) {
   const int group = hq / hkv;
   // Two query tiles a CTA halve the conversions; worth it from two waves on.
@@ -875,8 +903,14 @@ Plan plan_tiles(int rows, int tokens, int hq, int hkv, int sm_count) {
   Plan p{};
   p.shared = static_cast<long long>(tokens) * group / kRows * hkv >= 2LL * sm_count;
   p.tiles = static_cast<int>(p.shared ? most_tiles(rows, tokens, group, 2 * kRows) : single);
+  // Splits for the CTAs that have work: a row has one tile at least, and most
+  // batches about the larger of both counts (eight rows of 64 columns on 8 kv
+  // heads behind 4000 keys: 59 -> 43 us at head size 64, 67 -> 56 at 128).
+  const long long likely = std::max(static_cast<long long>(tokens) * group / kRows,
+                                    static_cast<long long>(std::min(rows, tokens)));
   p.splits = p.shared ? 1
-                      : static_cast<int>(std::max(1LL, std::min<long long>(kMostSplits, sm_count / std::max(1LL, single * hkv))));
+                      : static_cast<int>(std::max(
+                            1LL, std::min<long long>(kMostSplits, sm_count / std::max(1LL, likely * hkv))));
   return p;
 }
 
@@ -896,9 +930,10 @@ cudaError_t launch_tile(const Kv8AttnArgs& a, const Plan& p, int tile_from, floa
 bool kv8_tile_supported(int dim) { return dim == 64 || dim == 128; }
 
 size_t kv8_tile_workspace(int dim, int sm_count) {
-  // Splits are made while the CTAs are no more than the SMs; fewer tokens can
-  // have more of them, so the room is for any count up to these.
-  return static_cast<size_t>(sm_count) * 128 * (dim + 2) * sizeof(float);
+  // Splits are made while the likely CTAs are no more than the SMs, and the grid
+  // has at most twice as many.  Fewer tokens can have more splits, so the room is
+  // for any count up to these.
+  return static_cast<size_t>(sm_count) * 2 * 128 * (dim + 2) * sizeof(float);
 }
 
 cudaError_t kv8_tile_launch(const Kv8AttnArgs& a, int tile_from, float* partial, cudaStream_t stream) {
