@@ -160,9 +160,13 @@ __global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 4 : 6)
       Eight<float> w0, w1;
       w0.load(w + i0, w != nullptr && live);
       w1.load(w + i1, w != nullptr && live);
-      float ss = 0.f;
+      float2 squares = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ss += y[e] * y[e];
+      for (int e = 0; e < 16; e += 2) {
+        const float2 v = make_float2(y[e], y[e + 1]);
+        squares = fma2(v, v, squares);
+      }
+      float ss = squares.x + squares.y;
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       if (w != nullptr) {
@@ -171,7 +175,12 @@ __global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 4 : 6)
         w0.values(m);
         w1.values(m + 8);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[e] = y[e] * inv * m[e];
+        for (int e = 0; e < 16; e += 2) {
+          const float2 v = mul2f(mul2f(make_float2(y[e], y[e + 1]), make_float2(inv, inv)),
+                                 make_float2(m[e], m[e + 1]));
+          y[e] = v.x;
+          y[e + 1] = v.y;
+        }
       }
     }
     if constexpr (FORM == kHalves) {
@@ -214,14 +223,10 @@ __global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 4 : 6)
     }
     if (base + kHeads <= hq) continue;  // q only: the same for the whole warp
     float top = 0.f;
-    bool plain = true;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float m = fabsf(y[e]);
-      plain = plain && m <= kKv8Limit;
-      top = fmaxf(top, m);
-    }
-    if (!plain) {  // values that are not finite, or past the format
+    for (int e = 0; e < 16; ++e)
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(y[e])));
+    if (!(top <= kKv8Limit)) {  // values that are not finite, or past the format
       top = 0.f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -239,8 +244,11 @@ __global__ void __launch_bounds__(kWriteThreads, FORM == kExchange ? 4 : 6)
       uint8_t* dst = (is_v ? a.cache.v : a.cache.k) + at * d;
       uint32_t c[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        c[k] = kv8_codes(y[4 * k] * inv, y[4 * k + 1] * inv, y[4 * k + 2] * inv, y[4 * k + 3] * inv);
+      for (int k = 0; k < 4; ++k) {
+        const float2 lo = mul2f(make_float2(y[4 * k], y[4 * k + 1]), make_float2(inv, inv));
+        const float2 hi = mul2f(make_float2(y[4 * k + 2], y[4 * k + 3]), make_float2(inv, inv));
+        c[k] = kv8_codes(lo.x, lo.y, hi.x, hi.y);
+      }
       *reinterpret_cast<uint2*>(dst + i0) = make_uint2(c[0], c[1]);
       *reinterpret_cast<uint2*>(dst + i1) = make_uint2(c[2], c[3]);
       if (j == 0) (is_v ? a.cache.v_scale : a.cache.k_scale)[at] = static_cast<uint8_t>(e + 127);

@@ -103,33 +103,6 @@ __device__ __forceinline__ void mma_commit(bool on, uint64_t* bar) {
       : "memory");
 }
 
-// Two F32 operations an instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<unsigned long long&>(d))
-      : "l"(reinterpret_cast<const unsigned long long&>(a)),
-        "l"(reinterpret_cast<const unsigned long long&>(b)),
-        "l"(reinterpret_cast<const unsigned long long&>(c)));
-  return d;
-}
-__device__ __forceinline__ float2 mul2f(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<unsigned long long&>(d))
-      : "l"(reinterpret_cast<const unsigned long long&>(a)),
-        "l"(reinterpret_cast<const unsigned long long&>(b)));
-  return d;
-}
-__device__ __forceinline__ float2 add2f(float2 a, float2 b) {
-  float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<unsigned long long&>(d))
-      : "l"(reinterpret_cast<const unsigned long long&>(a)),
-        "l"(reinterpret_cast<const unsigned long long&>(b)));
-  return d;
-}
-
 // 2^y of two numbers on the FMA pipes, beside the exponentials of the special
 // function unit, which bounds a softmax: y = n + r with n the nearest integer
 // (found in the low bits of y + 1.5 2^23), 2^r by a polynomial of degree 5 fitted
