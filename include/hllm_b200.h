@@ -450,7 +450,8 @@ hllm_b200_status hllm_b200_sample(const float* logits, uint32_t rows, uint64_t v
  *   code_i = e4m3(x_i * 2^-e), ties to even; value_i = code_i * 2^e.
  * The maximum is over finite values of at most 448 * 2^39 in size; any other
  * value is stored as NaN.  head_dim is a multiple of 32, at most 256.
- * The arrays are 16-byte aligned.  All calls below are asynchronous, allocate
+ * The arrays are 16-byte aligned; blocks x 16 and blocks x kv_heads are below
+ * 2^31.  All calls below are asynchronous, allocate
  * nothing, keep nothing between calls and run on the current device, whose
  * memory every pointer names; they can be captured into a graph, and a
  * captured call serves any positions, slots, lengths and tables within the
@@ -527,10 +528,10 @@ hllm_b200_status hllm_b200_kv8_read(const hllm_b200_kv8* cache, const int32_t* b
  * cu_seqlens[r + 1]) of q (F16, row stride ld_q), at positions lengths[r] -
  * count ... lengths[r] - 1, and each attends to the keys up to its own.  A
  * token whose position is negative has no key: its output is zeros.  Outputs
- * are F16 (infinite past its range) at row stride ld_out; rows of no sequence are left as they are.
- * max_row_tokens bounds the rows' new tokens (1 for a decode batch); a longer
- * row, or one past `tokens` or max_blocks, is skipped and sets a status bit.
- * Keys of a missing page are left out and set one (a token that sees no other
+ * are F16 (infinite past its range) at row stride ld_out; rows of no sequence
+ * are left as they are.  max_row_tokens bounds the rows' new tokens (1 for a
+ * decode batch); a longer row, or one past `tokens` or max_blocks, is skipped
+ * and sets a status bit.  Keys of a missing page are left out and set one (a token that sees no other
  * gives zeros).  q and out are 16-byte aligned, ld_q and ld_out multiples of 8.
  * `workspace` (16-byte aligned) has at least hllm_b200_kv8_attention_workspace
  * bytes for these or larger counts and the same heads; its contents before and
