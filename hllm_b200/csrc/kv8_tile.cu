@@ -709,28 +709,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       mbar_arrive(&p_full[g]);
     }
-    // The sums are whole: those of this group, or, where both work on one tile of
-    // queries, of both (a group without a key tile has none).
-    auto finish = [&](int h) {  // the last of group h's products
-      const int uses = SHARED ? n : (n + 1 - h) >> 1;
-      if (uses > 0) ok = ok && mbar_wait(&o_done[h], (uses - 1) & 1, a.status);
-      return uses > 0;
-    };
+    // The last of this group's products; where both groups work on one tile of
+    // queries, each waits for its own, and they meet (a group without a key tile
+    // has no sums).
+    if (mine > 0)
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&o_done[g], (mine - 1) & 1, a.status));
+    const bool have0 = n > 0, have1 = !SHARED && n > 1;
     float w0 = 1.f, w1 = 0.f;  // weights of the groups' sums
-    bool have0, have1 = false;
-    if (SHARED) {
-      have0 = finish(g);
-      ok = __all_sync(0xffffffffu, ok);
-    } else {
+    if (!SHARED) {
       group_ml[g][tid] = make_float2(m, l);
-      have0 = finish(0);
-      have1 = finish(1);
+      tc_fence_before();
       ok = named_bar_all(1, kSoftmax, ok);
-      const float2 x0 = group_ml[0][tid], x1 = group_ml[1][tid];
-      m = fmaxf(x0.x, x1.x);
-      w0 = ex2(x0.x - m);
-      w1 = ex2(x1.x - m);
-      l = x0.y * w0 + x1.y * w1;
+      const float2 ml0 = group_ml[0][tid], ml1 = group_ml[1][tid];
+      m = fmaxf(ml0.x, ml1.x);
+      w0 = ex2(ml0.x - m);
+      w1 = ex2(ml1.x - m);
+      l = ml0.y * w0 + ml1.y * w1;
     }
     tc_fence_after();
     if (ok) {
