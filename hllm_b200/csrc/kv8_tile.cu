@@ -36,9 +36,9 @@
 // where E' is taken out: the weights are then the exponentials themselves.)
 // Every wait is bounded (common.cuh).
 //
-// Measured, 32 heads on 8 of 128: 2048 tokens behind 8192 keys 372 us (831
-// TFLOP/s of the causal products, 49 % of what cuBLAS reaches), 512 behind 1024
-// 28.8 us (373).  A step with two query tiles is 4.7k cycles, of which the products
+// Measured, 32 heads on 8 of 128: 2048 tokens behind 8192 keys 366 us (845
+// TFLOP/s of the causal products, 50 % of what cuBLAS reaches), 512 behind 1024
+// 28.5 us (377).  A step with two query tiles is 4.7k cycles, of which the products
 // are 2.8k: the rest is a group's chain, scores, maximum and exponentials (3.0k),
 // products, next scores, for which TMEM has no second buffer beside two results of
 // 128 dimensions.  With one query tile a step is 2.5k, and the codes' conversion
