@@ -243,6 +243,21 @@ __device__ __forceinline__ int parts_of(int tiles, int splits) {
   return max(1, min(splits, tiles / kLeastTiles));
 }
 
+// Tiles of a group of 32 rows up to each lane's, whose own they are.
+__device__ __forceinline__ int tiles_upto(int own, int lane) {
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, own, off);
+    if (lane >= off) own += v;
+  }
+  return own;
+}
+// Whether a row's tiles, numbered in the rows' order, are among the `most` that
+// were launched and that the workspace has pieces for.  They are unless
+// cu_seqlens decreases, so that rows overlap: the rows past that number are
+// skipped, in the tile pass and in the join alike.
+__device__ __forceinline__ bool fits(int before, int upto, int most) { return before + upto <= most; }
+
 template <int D, bool SHARED>
 __global__ void __launch_bounds__(kThreads, 1)
     kv8_tile_kernel(const Kv8AttnArgs a, int group, int tile_from, float* partial) {
@@ -283,6 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // and of a row the late tiles; all kv heads of a tile together; and the CTAs
     // that the grid has too many last.
     const bool reports = blockIdx.x + blockIdx.z == 0;
+    const int most = static_cast<int>(gridDim.x) / a.cache.hkv;  // tiles that the grid has
     int w = static_cast<int>(blockIdx.x) / a.cache.hkv;  // tiles before it
     int row = -1, tile = 0, cell = 0, tiles_before = 0;  // cell: its number in the rows' order
     for (int base = 0; base < a.rows && (row < 0 || reports); base += 32) {
@@ -292,11 +308,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         own = x.chunks;
         len = x.len;
       }
-      int first = 0, lower = 0;  // tiles of rows that go before this one, and that stand before it
+      const int upto = tiles_upto(own, lane), all = __shfl_sync(0xffffffffu, upto, 31);
+      const int lower = upto - own;  // tiles of rows that stand before this one
+      if (!fits(tiles_before, upto, most)) {
+        if (reports && own) atomicOr(a.status, kDevBadIndex);
+        own = 0;
+      }
+      int first = 0;  // tiles of rows that go before this one
       for (int j = 0; j < min(32, a.rows - base); ++j) {
         const int chunks = __shfl_sync(0xffffffffu, own, j), keys = __shfl_sync(0xffffffffu, len, j);
         if (keys > len || (keys == len && j < lane)) first += chunks;
-        if (j < lane) lower += chunks;
       }
       const unsigned hit = __ballot_sync(0xffffffffu, row < 0 && w >= first && w < first + own);
       if (hit) {
@@ -305,9 +326,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tile = __shfl_sync(0xffffffffu, own - 1 - (w - first), src);
         cell = tiles_before + __shfl_sync(0xffffffffu, lower, src) + tile;
       }
-      const int sum = __reduce_add_sync(0xffffffffu, own);
-      w -= sum;
-      tiles_before += sum;
+      w -= __reduce_add_sync(0xffffffffu, own);
+      tiles_before = min(tiles_before + all, most);
     }
     if (lane == 0) {
       found[0] = row;
@@ -782,25 +802,20 @@ __global__ void __launch_bounds__(256)
   griddep_enter();
   const int lane = threadIdx.x & 31;
   if (threadIdx.x < 32) {
-    const int want = blockIdx.x;
+    const int want = blockIdx.x, most = gridDim.x;
     int row = -1, before = 0;
-    for (int base = 0; base < a.rows && row < 0; base += 32) {
+    for (int base = 0; base < a.rows && before <= want; base += 32) {
       const int r = base + lane;
-      int incl = r < a.rows ? kv8_row(a, r, group, kRows, tile_from, false, true).chunks : 0;
-      const int own = incl;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += v;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > want);
+      const int own = r < a.rows ? kv8_row(a, r, group, kRows, tile_from, false, true).chunks : 0;
+      const int upto = tiles_upto(own, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, before + upto > want);
       if (hit) {
         const int src = __ffs(hit) - 1;
-        row = base + src;
-        before += __shfl_sync(0xffffffffu, incl - own, src);
-      } else {
-        before += __shfl_sync(0xffffffffu, incl, 31);
+        row = __shfl_sync(0xffffffffu, fits(before, upto, most) ? r : -1, src);
+        before += __shfl_sync(0xffffffffu, upto - own, src);
+        break;
       }
+      before += __shfl_sync(0xffffffffu, upto, 31);
     }
     if (lane == 0) {
       found[0] = row;
