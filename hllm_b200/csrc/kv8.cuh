@@ -178,6 +178,10 @@ __device__ __forceinline__ uint32_t kv8_half2_hi(uint32_t w) {
       : "r"(w));
   return h;
 }
+// 0xff in the bytes of four codes that are NaN.
+__device__ __forceinline__ uint32_t kv8_nan_codes(uint32_t w) {
+  return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 255u;
+}
 // Four values as codes (the first in the low byte), ties to even.
 __device__ __forceinline__ uint32_t kv8_codes(float a, float b, float c, float d) {
   uint32_t w;

@@ -112,9 +112,11 @@ struct Layout {
   __device__ static bool swapped(int g, int t) {
     return BOX == 128 ? g & 1 : BOX == 64 ? g >> 1 & 1 : t >> 1;
   }
-  __device__ static int v_at(int g, int t, int h, int s) {
-    const int row = value_key(t, h), byte = (s * 8 + g) * VW * 4;
+  __device__ static int byte_at(int row, int byte) {
     return byte / BOX * (16 * BOX) + row * BOX + ((byte % BOX / 16 ^ swizzle(row)) << 4) + byte % 16;
+  }
+  __device__ static int v_at(int g, int t, int h, int s) {
+    return byte_at(value_key(t, h), (s * 8 + g) * VW * 4);
   }
 };
 
@@ -258,7 +260,10 @@ __device__ __forceinline__ void store_unit(const Output& c0, const Output& c1, i
   if (c1.to) *reinterpret_cast<__half2*>(c1.to + dim) = __floats2half2_rn(v.y * c1.factor, v.w * c1.factor);
 }
 
-template <int D, int NT>
+// CHUNKS: rows may have several new tokens, so a stream's columns may see
+// different keys (hide_nan).  Batches of one token a row go without that code: 64
+// long rows take 141 us so, 144 with it.
+template <int D, int NT, bool CHUNKS>
 __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
     kv8_stream_kernel(const __grid_constant__ PoolMaps maps, const Kv8AttnArgs a, int group,
                       int tile_from, bool beside) {
@@ -726,6 +731,44 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       }
     };
 
+    // Value rows of a unit that some columns see and others do not: a weight of 0
+    // would not hide a NaN code.  Such codes make NaN of the sums of the columns
+    // that see them, and become zeros, before the unit is multiplied.
+    auto hide_nan = [&](uint8_t* unit, unsigned there, int key) {
+      const int r0 = max(0, edge + 1 - key), r1 = min(KP * kKv8Page, at.x.len - key);
+      auto codes = [&](int r, int byte) {
+        return unit + r / kKv8Page * S::kPage + 16 * D + S::byte_at(r % kKv8Page, byte);
+      };
+      uint32_t nan = 0u;
+#pragma unroll 1
+      for (int r = r0; r < r1; ++r)
+        if (there >> r / kKv8Page & 1u)
+          for (int w = lane; w < D / 4; w += 32)
+            nan |= kv8_nan_codes(*reinterpret_cast<const uint32_t*>(codes(r, 4 * w)));
+      if (!__any_sync(0xffffffffu, nan != 0u)) return;
+#pragma unroll 1
+      for (int r = r0; r < r1; ++r) {
+        if (!(there >> r / kKv8Page & 1u)) continue;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const uint32_t two = *reinterpret_cast<const uint16_t*>(codes(r, S::dim_of(i, g)));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if ((two >> (e >> 1) * 8 & 0x7fu) == 0x7fu && key + r <= lim[nt][e & 1])
+                o[nt][i][e] = __uint_as_float(0x7fffffffu);
+        }
+        __syncwarp();
+        for (int w = lane; w < D / 4; w += 32) {
+          uint32_t* const at_w = reinterpret_cast<uint32_t*>(codes(r, 4 * w));
+          *at_w &= ~kv8_nan_codes(*at_w);
+        }
+      }
+      fence_proxy_async();  // the slot's next boxes come after these stores
+      __syncwarp();
+    };
+
     auto sum_l = [&]() {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -798,6 +841,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
       const unsigned there = have >> (stage * KP) & ((1u << KP) - 1u);
       if (i + ST - 1 < n) fetch(next, false);  // the stage that every lane has left behind
       const bool ends = at.unit == at.units - 1, more = i + 1 < n;
+      if (CHUNKS && edge < at.x.len - 1 && (at.unit + 1) * (KP * kKv8Page) - 1 > edge)
+        hide_nan(ring + stage * S::kStage, there, at.unit * (KP * kKv8Page));
 #pragma unroll 1
       for (int j = 0; j < KP; j += MP)
         if (const unsigned some = there >> j & ((1u << MP) - 1u))
@@ -1000,21 +1045,27 @@ bool make_maps(PoolMaps* maps, const Kv8Cache& c, int box) {
 
 int stream_ctas(int sm_count) { return sm_count; }
 
-template <int D, int NT>
+template <int D, int NT, bool CHUNKS>
 cudaError_t launch_stream(const Kv8AttnArgs& a, int tile_from, bool beside, cudaStream_t stream) {
   using S = Shape<D, NT>;
   PoolMaps maps;
   if (!make_maps(&maps, a.cache, S::BOX)) return cudaErrorUnknown;
   static Kv8Configured configured;
-  cudaError_t e = configured.once(kv8_stream_kernel<D, NT>, S::kSmem);
+  cudaError_t e = configured.once(kv8_stream_kernel<D, NT, CHUNKS>, S::kSmem);
   if (e != cudaSuccess) return e;
   const int group = a.hq / a.cache.hkv;
   const int ctas = stream_ctas(a.sm_count);
-  e = launch_dependent(kv8_stream_kernel<D, NT>, dim3(ctas), dim3(S::kThreads), S::kSmem, stream,
+  e = launch_dependent(kv8_stream_kernel<D, NT, CHUNKS>, dim3(ctas), dim3(S::kThreads), S::kSmem, stream,
                        maps, a, group, tile_from, beside);
   if (e != cudaSuccess) return e;
   return launch_dependent(kv8_join_kernel<D, NT>, dim3(ctas), dim3(Join<D, NT>::kThreads), 0, stream, a,
                           group);
+}
+
+template <int D, int NT>
+cudaError_t by_tokens(const Kv8AttnArgs& a, int tile_from, bool beside, cudaStream_t stream) {
+  return a.max_row_tokens > 1 ? launch_stream<D, NT, true>(a, tile_from, beside, stream)
+                              : launch_stream<D, NT, false>(a, tile_from, beside, stream);
 }
 
 // Bytes of a piece: Shape<dim, nt>::kPieceBytes.
@@ -1061,8 +1112,8 @@ cudaError_t kv8_attention_launch(const Kv8AttnArgs& a, cudaStream_t stream) {
   switch (a.cache.dim) {
 #define HB_KV8_DIM(D)                                                                        \
   case D:                                                                                    \
-    e = wide && D <= 128 ? launch_stream<D, D <= 128 ? 2 : 1>(a, tile_from, tiles, stream)   \
-                         : launch_stream<D, 1>(a, tile_from, tiles, stream);                 \
+    e = wide && D <= 128 ? by_tokens<D, D <= 128 ? 2 : 1>(a, tile_from, tiles, stream)       \
+                         : by_tokens<D, 1>(a, tile_from, tiles, stream);                     \
     break;
     HB_KV8_DIM(32)
     HB_KV8_DIM(64)

@@ -1,10 +1,11 @@
-"""The 8-bit KV cache on the GPU where its calls end: rows that overlap."""
+"""The 8-bit KV cache on the GPU where its calls end: rows that overlap, and
+keys that a token may not see."""
 import numpy as np
 import pytest
 
 from hllm_b200._lib import StageError
 from tests.gpu_util import torch_cuda
-from tests.test_kv8_gpu import ints, random_cache, tables_for
+from tests.test_kv8_gpu import bytes_of, ints, random_cache, tables_for
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +50,47 @@ def test_decreasing_offsets_stay_inside_the_workspace(torch, kv8, d, turns):
         again = kv8.attention(cache, q, *good, max_tokens=T, workspace=buffer[:need])
         cache.check()
         assert torch.equal(again, clean)
+
+
+def check_nan(torch, kv8, heads, n, count, keys, most=None):
+    """NaN codes in K and in V rows reach the tokens at their position and later
+    ones, of their kv head, in V their dimension alone; everything else keeps its bits."""
+    hq, hkv, d = heads
+    rng = np.random.default_rng(n + count + d)
+    pages = (n + 15) // 16
+    cache = random_cache(torch, kv8, rng, pages + 3, hkv, d)
+    table = tables_for(torch, rng, [pages], pages + 3)
+    q = torch.randn((count, hq * d), device="cuda").half()
+    args = (ints(torch, [0, count]), ints(torch, [n]), ints(torch, table))
+    clean = kv8.attention(cache, q, *args, max_tokens=most or count).view(count, hq, d)
+    assert not bool(clean.isnan().any())
+    position = torch.arange(n - count, n, device="cuda")
+    for which in (0, 2):
+        codes = bytes_of(torch, cache)[which]
+        keep = codes.clone()
+        want = torch.zeros_like(clean, dtype=torch.bool)
+        for i, key in enumerate(keys):
+            head, dim = (key + i) % hkv, key * 7 % d
+            codes[table[0, key // 16], head, key % 16, dim] = 0x7f if i % 2 else 0xff
+            mine = slice(head * (hq // hkv), (head + 1) * (hq // hkv))
+            want[position >= key, mine, dim if which else slice(None)] = True
+        got = kv8.attention(cache, q, *args, max_tokens=most or count).view(count, hq, d)
+        assert torch.equal(got.isnan(), want)
+        assert torch.equal(got[~want], clean[~want])
+        codes.copy_(keep)
+    cache.check()
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 128), (32, 8, 128), (8, 8, 64), (4, 2, 64), (6, 2, 256), (3, 1, 32),
+                                   (12, 4, 96), (4, 4, 160), (7, 1, 192), (2, 1, 224), (16, 1, 128), (20, 1, 64)])
+@pytest.mark.parametrize("past,count", [(0, 3), (29, 2), (100, 3), (14, 15)])
+def test_nan_in_keys_that_some_tokens_do_not_see(torch, kv8, heads, past, count):
+    count = min(count, 63 * heads[1] // heads[0])  # few enough columns for the stream pass
+    n = past + count
+    check_nan(torch, kv8, heads, n, count, sorted({0, past // 2, past, past + 1, n - 2, n - 1} & set(range(n))))
+
+
+@pytest.mark.parametrize("heads", [(6, 2, 256), (4, 4, 96), (3, 1, 32)])
+def test_nan_in_the_middle_of_chunks_at_other_head_sizes(torch, kv8, heads):
+    check_nan(torch, kv8, heads, 150, 90, (35, 60, 97, 113, 149))
+    check_nan(torch, kv8, heads, 3000, 40, (7, 2959, 2960, 2975, 2976, 2998))
