@@ -231,6 +231,42 @@ __device__ __forceinline__ void store_codes(uint8_t* dst, const Share<D>& h, int
   }
 }
 
+// The codes of V at a key of a row, null where its page is missing.
+__device__ __forceinline__ const uint8_t* value_row(const Kv8AttnArgs& a, int row, int kvh, int key, int dim) {
+  const int id = __ldg(a.tables + static_cast<size_t>(row) * a.max_blocks + key / kKv8Page);
+  if (id < 0 || id >= a.cache.blocks) return nullptr;
+  return a.cache.v + ((static_cast<size_t>(id) * a.cache.hkv + kvh) * kKv8Page + key % kKv8Page) * dim;
+}
+// A weight of 0 would not hide a NaN code of V from the columns that do not see
+// its key.  So what this thread stored of such codes, in keys from `first` on,
+// becomes zeros, and the columns that see them get their NaN with the result.
+// (Neither is inlined: hardly a call needs them, and the passes have no registers
+// to spare.)
+template <int D>
+__device__ __noinline__ void hide_nan(uint8_t* dst, Share<D> h, int first) {
+  for (int r = h.row; r < kKeys; r += Share<D>::kRows) {
+    if (r < first) continue;
+    for (int c = h.chunk * 16; c < h.chunk * 16 + 16; ++c) {
+      uint16_t* const at = reinterpret_cast<uint16_t*>(
+          dst + (c >> 6) * (128 * 128) + r * 128 + (((c >> 3 & 7) ^ (r & 7)) << 4) + (c & 7) * 2);
+      if ((*at & 0x7fffu) > 0x7c00u) *at = 0;
+    }
+  }
+}
+// `to` is the column's result: F16, or a partial result's sums.
+template <int D>
+__device__ __noinline__ void put_nan(const Kv8AttnArgs& a, int row, int kvh, int key0, int key1, int c0, int c1,
+                                     __half* to, float* piece) {
+  for (int key = key0; key < key1; ++key) {
+    const uint8_t* codes = value_row(a, row, kvh, key, D);
+    for (int c = c0; codes && c < c1; ++c) {
+      if ((__ldg(codes + c) & 0x7f) != 0x7f) continue;
+      if (piece) piece[c / 4 * (128 * 4) + c % 4] = __uint_as_float(0x7fffffffu);
+      else to[c] = __ushort_as_half(0x7fff);
+    }
+  }
+}
+
 // Keys that the last of `columns` columns from x0 on sees.
 __device__ __forceinline__ int seen_keys(const Kv8Row& x, int group, int x0, int columns) {
   const int last_token = (min(x0 + columns, x.count * group) - 1) / group;
@@ -260,13 +296,13 @@ __device__ __forceinline__ bool fits(int before, int upto, int most) { return be
 
 template <int D, bool SHARED>
 __global__ void __launch_bounds__(kThreads, 1)
-    kv8_tile_kernel(const Kv8AttnArgs a, int group, int tile_from, float* partial) {
+    kv8_tile_kernel(const __grid_constant__ Kv8AttnArgs a, int group, int tile_from, float* partial) {
   using T = Tile<D, SHARED>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   __shared__ uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2],
-      o_done[2];
+      o_done[2], looked;
   __shared__ uint32_t tmem_slot;
   __shared__ float2 group_ml[2][kRows];  // m and l of the groups, where they share a tile
   __shared__ int found[3];             // row, tile of the row, tile of all rows
@@ -276,12 +312,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(16) float value_scale[4][2 * kKeys];
   __shared__ int extremes[2][2][4][3];          // by group, tile and warp: E, E' + 127, least ev + 127
   __shared__ uint8_t scale_byte[2][2][kKeys];   // by group and tile
+  __shared__ volatile int nan_hidden;  // whether V has NaN codes in keys that some columns do not see
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kCta = T::kQueries * kRows;  // columns of a CTA
 
   griddep_enter();
   if (threadIdx.x == 0) {
+    nan_hidden = 0;
     mbar_init(&q_full, kSoftmax);
+    mbar_init(&looked, kSoftmax);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], 128);
       mbar_init(&v_full[s], 128);
@@ -363,6 +402,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const int kt0 = static_cast<int>(static_cast<long long>(all) * part / parts);
   const int n = static_cast<int>(static_cast<long long>(all) * (part + 1) / parts) - kt0;
+
+  // The keys of this split that some columns of the CTA do not see.
+  const int hidden0 = max(kt0 * kKeys, past + x0 / group + 1), hidden1 = min(keys, (kt0 + n) * kKeys);
 
   if (warp == 16) {
     // ---------------------------------------------------------------- products
@@ -556,6 +598,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         store_codes<D>(dst, share, p, c[p], factor[p]);
         c[p] = load_codes<D>(share, pool, page[p], p, left);
       }
+      if (values && (kt0 + t + 1) * kKeys > hidden0) {
+        ok = mbar_wait(&looked, 0, a.status) && ok;
+        if (nan_hidden) hide_nan<D>(dst, share, hidden0 - (kt0 + t) * kKeys);
+      }
       fence_proxy_async();
       mbar_arrive(&full[t & 1]);
     }
@@ -592,6 +638,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async();
       mbar_arrive(&q_full);
     }
+    // While the first scores are on their way: NaN codes in V of those keys.
+    constexpr int kPieces = D / 16;
+#pragma unroll 1
+    for (int i0 = threadIdx.x; i0 < (hidden1 - hidden0) * kPieces; i0 += 4 * kSoftmax) {
+      const uint8_t* at[4];
+      uint32_t nan = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = hidden0 + (i0 + i * kSoftmax) / kPieces;
+        at[i] = key < hidden1 ? value_row(a, row, kvh, key, D) : nullptr;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 c = load16_if(at[i] + (i0 + i * kSoftmax) % kPieces * 16, at[i] != nullptr);
+        nan |= kv8_nan_codes(c.x) | kv8_nan_codes(c.y) | kv8_nan_codes(c.z) | kv8_nan_codes(c.w);
+      }
+      if (nan) nan_hidden = 1;
+    }
+    mbar_arrive(&looked);
     const int col = x0 + (SHARED ? g * kRows : 0) + tid;
     const int lim = col < cols ? min(past + col / group, keys - 1) : -1;  // last key seen
     const float sl2 = a.scale * kLog2e;
@@ -785,6 +850,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (split && g == 0) reinterpret_cast<float2*>(piece + 128 * (D / 4))[tid] = make_float2(m, l);
+      if (nan_hidden && col < cols)
+        put_nan<D>(a, row, kvh, hidden0, min(lim + 1, hidden1), SHARED ? 0 : g * (D / 2),
+                   SHARED ? D : (g + 1) * (D / 2), out,
+                   split ? reinterpret_cast<float*>(piece + tid) : nullptr);
     }
   }
   tc_fence_before();

@@ -527,7 +527,8 @@ hllm_b200_status hllm_b200_kv8_read(const hllm_b200_kv8* cache, const int32_t* b
  * and mixes of them: row r's new tokens are rows [cu_seqlens[r],
  * cu_seqlens[r + 1]) of q (F16, row stride ld_q), at positions lengths[r] -
  * count ... lengths[r] - 1, and each attends to the keys up to its own.  A
- * token whose position is negative has no key: its output is zeros.  Outputs
+ * token whose position is negative has no key: its output is zeros.  NaN codes
+ * reach the tokens that see their key, and no others.  Outputs
  * are F16 (infinite past its range) at row stride ld_out; rows of no sequence
  * are left as they are.  max_row_tokens bounds the rows' new tokens (1 for a
  * decode batch); a longer row, or one past `tokens` or max_blocks, is skipped

@@ -94,3 +94,17 @@ def test_nan_in_keys_that_some_tokens_do_not_see(torch, kv8, heads, past, count)
 def test_nan_in_the_middle_of_chunks_at_other_head_sizes(torch, kv8, heads):
     check_nan(torch, kv8, heads, 150, 90, (35, 60, 97, 113, 149))
     check_nan(torch, kv8, heads, 3000, 40, (7, 2959, 2960, 2975, 2976, 2998))
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 2, 64), (32, 8, 128), (8, 8, 64), (16, 1, 128)])
+@pytest.mark.parametrize("past,count", [(0, 140), (80, 70), (1000, 130), (2900, 100), (5, 400)])
+def test_nan_in_the_middle_of_prompt_chunks(torch, kv8, heads, past, count):
+    n = past + count
+    keys = {0, 35, past, past + 1, past + count // 2, past + 63, past + 127, n - 2, n - 1}
+    check_nan(torch, kv8, heads, n, count, sorted(k for k in keys if k < n))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_in_the_middle_of_a_long_chunk(torch, kv8, d):
+    """CTAs of two query tiles."""
+    check_nan(torch, kv8, (16, 8, d), 2600, 2500, (35, 100, 127, 128, 1000, 1383, 2047, 2500, 2599))
