@@ -10,13 +10,12 @@
 //   warps 8-11  converters of K, warps 12-15 of V: a tile's codes from their
 //               pages into shared memory as swizzled F16 operands, the next
 //               tile's loads going out as the registers become free.  K rows
-//               are code * 2^(e - E) with E the tile's largest exponent, so that
-//               F16 holds rows of any size; what it rounds lies 2^-34 below the
-//               largest row, and E goes into the score scale of the tile.  V
-//               rows likewise where the tile's exponents lie within 2^8 of their
-//               largest E' (exact then), which goes into the weights' exponent;
-//               else they are the codes, and each key's scale goes into its
-//               weights.
+//               are code * 2^(e - E) with E the tile's largest exponent, which
+//               goes into the score scale of the tile, and V rows likewise, where
+//               the tile's exponents lie within 2^15 and 2^8 of their largest:
+//               nothing is rounded then (a code's lowest bit is 2^-9, F16's 2^-24).
+//               Else both are the codes, and each key's scales go into its score
+//               and its weights: no key, seen or hidden, coarsens another.
 //   warp 16     one thread issues the products.
 //   warps 0-7   two softmax groups of 128 threads, one row (TMEM lane) a
 //               thread.  The weights go back into TMEM over the scores they
@@ -57,7 +56,8 @@ constexpr int kKeys = 128;       // keys of a tile
 constexpr int kRows = 128;       // columns of a query tile
 constexpr int kSoftmax = 256;    // threads of the softmax groups
 constexpr int kThreads = kSoftmax + 256 + 32;
-constexpr int kSpread = 8;        // V exponents this near their tile's largest are taken out of the weights
+constexpr int kSpread = 8;        // V exponents this near their tile's largest are taken out of the weights,
+constexpr int kSpreadK = 15;      // and K exponents this near out of the scores, exactly
 constexpr int kApart = 1000;      // others
 
 // The products' instructions, by the lane for which `on` holds, in code that a
@@ -307,10 +307,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ float2 group_ml[2][kRows];  // m and l of the groups, where they share a tile
   __shared__ int found[3];             // row, tile of the row, tile of all rows
   // By key tile: E + 127 of its K; E' of its V, or kApart; and then each key's
-  // 2^ev (0 where there is no key) and ev (-inf).
+  // 2^ev (0 where there is no key), ev (-inf) and 2^ek (0).
   __shared__ volatile int exps[4][2];
-  __shared__ __align__(16) float value_scale[4][2 * kKeys];
-  __shared__ int extremes[2][2][4][3];          // by group, tile and warp: E, E' + 127, least ev + 127
+  __shared__ __align__(16) float value_scale[4][3 * kKeys];
+  __shared__ int extremes[2][2][4][4];          // by group, tile and warp: E, E', least ev and ek, all + 127
   __shared__ uint8_t scale_byte[2][2][kKeys];   // by group and tile
   __shared__ volatile int nan_hidden;  // whether V has NaN codes in keys that some columns do not see
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -546,12 +546,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int ev = __reduce_max_sync(0xffffffffu, have ? static_cast<int>(vs) : 0);
       // A missing page takes the path that looks at each key.
       const int least = __reduce_min_sync(0xffffffffu, have ? static_cast<int>(vs) : hole ? -1000 : 1000);
+      const int least_k = __reduce_min_sync(0xffffffffu, have ? static_cast<int>(ks) : 1000);
       if (lane == 0) {
         extremes[group_of][t & 1][cw][0] = ek;
         extremes[group_of][t & 1][cw][1] = ev;
         extremes[group_of][t & 1][cw][2] = least;
+        extremes[group_of][t & 1][cw][3] = least_k;
       }
-      const float scale = have ? kv8_scale(vs) : 0.f;
+      const float scale = have ? kv8_scale(vs) : 0.f, k_scale = have ? kv8_scale(ks) : 0.f;
       const float exponent = have ? static_cast<float>(static_cast<int>(vs) - 127) : -INFINITY;
       pages = pages_of(ids);  // -1 everywhere past the last tile
       ids = load_ids(t + 2);
@@ -559,26 +561,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       // All four warps go on, or none: a wait that ran out is known to all here.
       ok = named_bar_all(3 + group_of, 128, ok);
       if (!ok) break;
-      int e_k = 0, e_v = 0, low = 1000;
+      int e_k = 0, e_v = 0, low = 1000, low_k = 1000;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         e_k = max(e_k, extremes[group_of][t & 1][w][0]);
         e_v = max(e_v, extremes[group_of][t & 1][w][1]);
         low = min(low, extremes[group_of][t & 1][w][2]);
+        low_k = min(low_k, extremes[group_of][t & 1][w][3]);
       }
       // (max (s f) is max (s) f for a scale >= 0 only.)
-      const bool apart = e_v - low > kSpread || !(a.scale >= 0.f);
+      const bool apart = e_v - low > kSpread || e_k - low_k > kSpreadK || !(a.scale >= 0.f);
       ok = t < 2 || mbar_wait(&empty[t & 1], ((t - 2) >> 1) & 1, a.status);
       if (!values) {
         // The scores of tile t - 2 followed the sums of tile t - 4, so that
         // tile's entry is read by nobody any more.
         if (tid == 0) {
-          exps[t & 3][0] = e_k > 0 ? e_k : 127;
+          exps[t & 3][0] = e_k > 0 && !apart ? e_k : 127;
           exps[t & 3][1] = apart ? kApart : e_v - 127;
         }
         if (apart) {
           value_scale[t & 3][tid] = scale;
           value_scale[t & 3][kKeys + tid] = exponent;
+          value_scale[t & 3][2 * kKeys + tid] = k_scale;
         }
       }
       uint8_t* dst = operand + (t & 1) * T::kOperand;
@@ -591,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int p = 0; p < kPasses; ++p) {
         page[p] = page_of(p);
         const int byte = scale_byte[group_of][t & 1][p * Share<D>::kRows + share.row];
-        factor[p] = values && apart ? 0x3c003c00u : half_power2(byte - top + 127);
+        factor[p] = apart ? 0x3c003c00u : half_power2(byte - top + 127);
       }
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
@@ -691,9 +695,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 16; i += 4) {
             float2 y0 = pair_of(x[i], x[i + 1]), y1 = pair_of(x[i + 2], x[i + 3]);
             if (kEach) {
-              const float4 ev = vs[(kKeys + c + i) / 4];
-              y0 = fma2(y0, f2, make_float2(ev.x, ev.y));
-              y1 = fma2(y1, f2, make_float2(ev.z, ev.w));
+              const float4 ev = vs[(kKeys + c + i) / 4], ks = vs[(2 * kKeys + c + i) / 4];
+              y0 = fma2(mul2f(y0, make_float2(ks.x, ks.y)), f2, make_float2(ev.x, ev.y));
+              y1 = fma2(mul2f(y1, make_float2(ks.z, ks.w)), f2, make_float2(ev.z, ev.w));
             }
             if (kMasked) {
               if (c + i > seen) y0.x = -INFINITY;
@@ -730,8 +734,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t pk[8];
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
-            float2 y0 = fma2(pair_of(x[i], x[i + 1]), f2, minus);
-            float2 y1 = fma2(pair_of(x[i + 2], x[i + 3]), f2, minus);
+            float2 y0 = pair_of(x[i], x[i + 1]), y1 = pair_of(x[i + 2], x[i + 3]);
+            if (kEach) {
+              const float4 ks = vs[(2 * kKeys + c + i) / 4];
+              y0 = mul2f(y0, make_float2(ks.x, ks.y));
+              y1 = mul2f(y1, make_float2(ks.z, ks.w));
+            }
+            y0 = fma2(y0, f2, minus);
+            y1 = fma2(y1, f2, minus);
             if (kMasked) {
               if (c + i > seen) y0.x = -INFINITY;
               if (c + i + 1 > seen) y0.y = -INFINITY;

@@ -1,9 +1,12 @@
-"""The 8-bit KV cache on the GPU where its calls end: rows that overlap, and
-keys that a token may not see."""
+"""The 8-bit KV cache on the GPU where its calls end: rows that overlap,
+keys that a token may not see, sizes far apart."""
+import math
+
 import numpy as np
 import pytest
 
 from hllm_b200._lib import StageError
+from tests import kv8_util
 from tests.gpu_util import torch_cuda
 from tests.test_kv8_gpu import bytes_of, ints, random_cache, tables_for
 
@@ -108,3 +111,64 @@ def test_nan_in_the_middle_of_prompt_chunks(torch, kv8, heads, past, count):
 def test_nan_in_the_middle_of_a_long_chunk(torch, kv8, d):
     """CTAs of two query tiles."""
     check_nan(torch, kv8, (16, 8, d), 2600, 2500, (35, 100, 127, 128, 1000, 1383, 2047, 2500, 2599))
+
+
+def attend(torch, k, v, q, position, scale):
+    """One head of one row in 64 bits, with the error that its arithmetic may
+    have: k, v [n, d], q [count, d], position [count].  A score's error counts by
+    its own terms, so a key's size loosens nothing for the others:
+      * score j, in F32: r_j = 2 (d + 8) 2^-23 sum_i |q_i k_ji| scale + 2^-20 (exp2 and
+        scales), absolutely, which moves weight j by r_j of itself;
+      * weight j to F16: 2^-11 of it, or half of F16's least step, 2^-25 of a
+        reference that the largest weight times value scale reaches;
+      * the sums of n terms: 2 n 2^-23 each, over all keys that there are;
+      * the normaliser: sum_j p_j r_j and the sum's, of the output;
+      * the output to F16: 2^-11 of it, or 2^-25."""
+    n, d = k.shape
+    hidden = torch.arange(n, device=q.device)[None, :] > position[:, None]
+    p = torch.softmax((q @ k.T * scale).masked_fill(hidden, -math.inf), -1)
+    o = p @ v
+    r = 2 * (d + 8) * 2.0 ** -23 * (q.abs() @ k.abs().T * scale) + 2.0 ** -20
+    pr = torch.where(p > 0, p * r, 0.0)
+    sums = 2 * n * 2.0 ** -23
+    share = p @ v.abs()
+    amax = (p * 2 * v.abs().amax(-1)).amax(-1, keepdim=True)  # a value is at most 2 amax of its row
+    tol = (pr @ v.abs() + (2.0 ** -11 + sums) * share + n * 2.0 ** -25 * amax +
+           (pr.sum(-1, keepdim=True) + sums) * share + 2.0 ** -11 * o.abs() + 2.0 ** -25)
+    return o, tol
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 2, 64), (16, 8, 128), (8, 8, 64), (6, 2, 256)])
+@pytest.mark.parametrize("past,count", [(60, 100), (300, 5), (700, 600), (2, 3000)])
+@pytest.mark.parametrize("octaves", [14, 18, 34, 44])
+def test_large_keys_coarsen_no_others(torch, kv8, heads, past, count, octaves):
+    """Keys 2^octaves times the others, along a direction of their own in which
+    all queries point away from them: their weight is 0 where they are seen, and
+    they are hidden from early tokens.  Others' scores keep their precision."""
+    hq, hkv, d = heads
+    n = past + count
+    rng = np.random.default_rng(octaves)
+    pages = (n + 15) // 16
+    cache = random_cache(torch, kv8, rng, pages + 3, hkv, d)
+    table = tables_for(torch, rng, [pages], pages + 3)
+    kc, ks, vc, vs = bytes_of(torch, cache)
+    kc[..., 0] = 0
+    for key in sorted({0, past // 2, past, past + count // 3, n - 2}):
+        at = int(table[0, key // 16]), slice(None), key % 16
+        kc[at] = 0
+        kc[at[0], :, at[2], 0] = 0xc0  # -2
+        ks[at] = min(122 + octaves, 127 + 39)
+    q = (1.5 * torch.randn((count, hq, d), device="cuda")).half()
+    q[..., 0] = 16.0
+    got = kv8.attention(cache, q.view(count, hq * d), ints(torch, [0, count]), ints(torch, [n]),
+                        ints(torch, table)).view(count, hq, d).double()
+    cache.check()
+    at = torch.as_tensor(table[0], device="cuda").long()
+    k, v = (kv8_util.values(torch, c[at], e[at]).transpose(1, 2).reshape(-1, hkv, d)[:n]
+            for c, e in ((kc, ks), (vc, vs)))
+    position = torch.arange(past, n, device="cuda")
+    for h in range(hq):
+        want, tol = attend(torch, k[:, h // (hq // hkv)], v[:, h // (hq // hkv)], q[:, h].double(), position,
+                           1 / math.sqrt(d))
+        err = (got[:, h] - want).abs() / tol
+        assert bool((err <= 1).all()), (h, float(err.max()), err.amax(-1).nonzero()[:5])
