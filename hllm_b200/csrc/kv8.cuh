@@ -113,8 +113,14 @@ struct Kv8Configured {
 // ---------------------------------------------------------------- device side
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoReference = -1e30f;  // below every finite score
-constexpr float kLazy = 8.f;            // log2 of the growth that moves a softmax reference
-constexpr float kMostWeight = 256.f;    // 2^kLazy
+// A softmax reference moves when a weight (with its value row's scale) would pass
+// 2^kMost, and then so that the largest is 2^kTop: F16 keeps weights down to
+// 2^-24, so 2^-31 of the largest at least, and a long tail of small ones counts.
+// (With the largest at 1 a flat tail 2^-25 below one key went missing from the
+// sums, 2^-8 of the output at 131071 keys.)  2^kMost leaves F16 a factor of 4 for
+// what large scores round.
+constexpr float kTop = 7.f, kMost = 14.f;
+constexpr float kMostWeight = 16384.f;  // 2^kMost
 
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);

@@ -8,8 +8,8 @@
 //   l = sum 2^(s_j - m),   O = sum (2^(s_j - m) 2^ev_j) d_j,   o = O / l.
 // The weights in brackets are what the products round (F16, by 2^-11), so m
 // follows max (s_j + ev_j): they keep their precision whatever the sizes of the
-// value rows.  It is raised only when a weight passes 2^8: most pages rescale
-// nothing.
+// value rows.  It is raised only when a weight passes 2^14, to where the largest is
+// 2^7: most pages rescale nothing.
 //
 // Work.  A row's new tokens and the query heads of one kv head form columns
 // (token, head), 8 NT of them a stream; a stream walks the row's pages, one to
@@ -675,9 +675,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
                 mx = fmaxf(mx, s[j][nt][0][2 * h + e] + static_cast<float>(static_cast<int>(vb[j][h]) - 127));
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            if (mx > m[nt][e]) {
-              const float f = ex2(m[nt][e] - mx);
-              m[nt][e] = mx;
+            const float to = mx - kTop;
+            if (to > m[nt][e]) {
+              const float f = ex2(m[nt][e] - to);
+              m[nt][e] = to;
               l[nt][e] *= f;
 #pragma unroll
               for (int i = 0; i < D / 16; ++i) {

@@ -721,11 +721,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float offset = kEach ? 0.f : static_cast<float>(e_v);
         const float mx = kEach ? fmaxf(m0, m1) : fmaf(fmaxf(m0, m1), f, offset);
-        // A reference moves only when a weight would pass 2^8: it becomes the
-        // row's largest so far.
-        if (mx > m + kLazy) {
-          alpha = ex2(m - mx);
-          m = mx;
+        // A reference moves only when a weight, rounded as below, would pass 2^14.
+        if ((kEach ? mx - m : fmaf(fmaxf(m0, m1), f, offset - m)) > kMost) {
+          alpha = ex2(m - (mx - kTop));
+          m = mx - kTop;
         }
         float2 sum = make_float2(0.f, 0.f);
         const float2 minus = make_float2(offset - m, offset - m);

@@ -1,5 +1,5 @@
 """The 8-bit KV cache on the GPU where its calls end: rows that overlap,
-keys that a token may not see, sizes far apart."""
+keys that a token may not see, sizes far apart, tails of small weights."""
 import math
 
 import numpy as np
@@ -113,14 +113,16 @@ def test_nan_in_the_middle_of_a_long_chunk(torch, kv8, d):
     check_nan(torch, kv8, (16, 8, d), 2600, 2500, (35, 100, 127, 128, 1000, 1383, 2047, 2500, 2599))
 
 
-def attend(torch, k, v, q, position, scale):
+def attend(torch, k, v, q, position, scale, spread=0):
     """One head of one row in 64 bits, with the error that its arithmetic may
     have: k, v [n, d], q [count, d], position [count].  A score's error counts by
     its own terms, so a key's size loosens nothing for the others:
       * score j, in F32: r_j = 2 (d + 8) 2^-23 sum_i |q_i k_ji| scale + 2^-20 (exp2 and
         scales), absolutely, which moves weight j by r_j of itself;
-      * weight j to F16: 2^-11 of it, or half of F16's least step, 2^-25 of a
-        reference that the largest weight times value scale reaches;
+      * weight j to F16: 2^-11 of it, or half of F16's least step, 2^-25, where the
+        largest weight times value scale is 2^7 at least: 2^-32 of that.  Where the
+        reference counts a tile's largest value scale (exponents within 2^spread of
+        it, 2^8 at most), the largest may be 2^spread less: 2^(spread - 32);
       * the sums of n terms: 2 n 2^-23 each, over all keys that there are;
       * the normaliser: sum_j p_j r_j and the sum's, of the output;
       * the output to F16: 2^-11 of it, or 2^-25."""
@@ -133,7 +135,7 @@ def attend(torch, k, v, q, position, scale):
     sums = 2 * n * 2.0 ** -23
     share = p @ v.abs()
     amax = (p * 2 * v.abs().amax(-1)).amax(-1, keepdim=True)  # a value is at most 2 amax of its row
-    tol = (pr @ v.abs() + (2.0 ** -11 + sums) * share + n * 2.0 ** -25 * amax +
+    tol = (pr @ v.abs() + (2.0 ** -11 + sums) * share + n * 2.0 ** (min(spread, 8) - 32) * amax +
            (pr.sum(-1, keepdim=True) + sums) * share + 2.0 ** -11 * o.abs() + 2.0 ** -25)
     return o, tol
 
@@ -167,8 +169,45 @@ def test_large_keys_coarsen_no_others(torch, kv8, heads, past, count, octaves):
     k, v = (kv8_util.values(torch, c[at], e[at]).transpose(1, 2).reshape(-1, hkv, d)[:n]
             for c, e in ((kc, ks), (vc, vs)))
     position = torch.arange(past, n, device="cuda")
+    spread = int(vs.max()) - int(vs.min())
     for h in range(hq):
         want, tol = attend(torch, k[:, h // (hq // hkv)], v[:, h // (hq // hkv)], q[:, h].double(), position,
-                           1 / math.sqrt(d))
+                           1 / math.sqrt(d), spread)
         err = (got[:, h] - want).abs() / tol
         assert bool((err <= 1).all()), (h, float(err.max()), err.amax(-1).nonzero()[:5])
+
+
+@pytest.mark.parametrize("heads", [(2, 1, 128), (4, 2, 64), (1, 1, 256), (16, 1, 128), (8, 2, 128)])
+@pytest.mark.parametrize("n,count,rows", [(131072, 1, 1), (100001, 2, 1), (4000, 1, 1), (70003, 64, 1), (3001, 600, 1),
+                                          (4000, 1, 1500), (3000, 2, 700)])
+@pytest.mark.parametrize("octaves", [12, 20, 25])
+def test_a_long_tail_of_small_weights_counts(torch, kv8, heads, n, count, rows, octaves):
+    """One key 2^octaves times as heavy as each of all the others, whose values
+    are 1 in every dimension and its own 0 in all but one: what the output holds is
+    the others' share, 2^-8 for 2^17 of them at 25 octaves.  (Of one row the keys are
+    split, and most splits do not have the key; of many rows they are not.)"""
+    hq, hkv, d = heads
+    rng = np.random.default_rng(octaves)
+    pages = (n + 15) // 16
+    cache = kv8.Cache(pages + 2, hkv, d)
+    table = tables_for(torch, rng, [pages], pages + 2)
+    kc, ks, vc, vs = bytes_of(torch, cache)
+    vc[...] = 0x38  # 1
+    heavy = n // 3
+    at = int(table[0, heavy // 16]), heavy % 16
+    kc[at[0], :, at[1], 0] = 0x38
+    vc[at[0], :, at[1]] = 0
+    vc[at[0], :, at[1], 1] = 0x38
+    q = torch.zeros((count * rows, hq, d), device="cuda", dtype=torch.float16)
+    q[..., 0] = octaves
+    scale = math.log(2.0)
+    got = kv8.attention(cache, q.view(-1, hq * d), ints(torch, np.arange(rows + 1) * count), ints(torch, [n] * rows),
+                        ints(torch, np.repeat(table, rows, 0)), max_tokens=count, scale=scale)
+    got = got.view(rows, count, hq, d).double()
+    cache.check()
+    pages_at = torch.as_tensor(table[0], device="cuda").long()
+    k, v = (kv8_util.values(torch, c[pages_at, 0], e[pages_at, 0]).reshape(-1, d)[:n]
+            for c, e in ((kc, ks), (vc, vs)))
+    want, tol = attend(torch, k, v, q[:count, 0].double(), torch.arange(n - count, n, device="cuda"), scale)
+    err = (got - want[:, None]).abs() / tol[:, None]
+    assert bool((err <= 1).all()), float(err.max())
