@@ -267,7 +267,9 @@ def attention(cache: Cache, q, cu_seqlens, lengths, block_tables, max_tokens: Op
         _refuse(f"out must be a float16 {(tokens, width)} matrix on {cache.device}")
     ld_q = ld_out = width
     if tokens > 0:
-        (ld_q, across), (ld_out, out_across) = q.stride(), out.stride()
+        (step_q, across), (step_out, out_across) = q.stride(), out.stride()
+        if tokens > 1:  # (torch leaves the stride of a single row open)
+            ld_q, ld_out = step_q, step_out
         if across != 1 or ld_q < width:
             _refuse("q must have contiguous rows")
         if out_across != 1 or ld_out < width:

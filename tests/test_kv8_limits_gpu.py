@@ -211,3 +211,23 @@ def test_a_long_tail_of_small_weights_counts(torch, kv8, heads, n, count, rows, 
     want, tol = attend(torch, k, v, q[:count, 0].double(), torch.arange(n - count, n, device="cuda"), scale)
     err = (got - want[:, None]).abs() / tol[:, None]
     assert bool((err <= 1).all()), float(err.max())
+
+
+def test_a_single_row_may_have_any_step(torch, kv8):
+    """torch leaves the stride of a dimension of one row open: a column's transpose,
+    a row of a matrix of odd width, a row said to be repeated."""
+    hq, hkv, d = 4, 2, 64
+    rng = np.random.default_rng(1)
+    cache = random_cache(torch, kv8, rng, 6, hkv, d)
+    args = (ints(torch, [0, 1]), ints(torch, [40]), ints(torch, tables_for(torch, rng, [3], 6)))
+    q = torch.randn((1, hq * d), device="cuda").half()
+    want = kv8.attention(cache, q, *args)
+    column = q.t().contiguous()
+    odd = torch.empty((2, hq * d + 5), dtype=torch.float16, device="cuda")
+    odd[0, :hq * d] = q[0]
+    for given in (column.t(), odd[:1, :hq * d], q[0].expand(1, hq * d)):
+        assert torch.equal(kv8.attention(cache, given, *args), want)
+    for out in (torch.empty_like(column).t(), odd[:1, :hq * d]):
+        assert torch.equal(kv8.attention(cache, q, *args, out=out), want)
+        assert torch.equal(out, want)
+    cache.check()
