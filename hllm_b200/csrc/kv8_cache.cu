@@ -335,7 +335,15 @@ __global__ void __launch_bounds__(kReadThreads)
   if (threadIdx.x < kReadTokens) ends[threadIdx.x] = 0;
   __syncthreads();
   for (int base = warp * 32; base < a.rows; base += kReadThreads) {
-    const int k = base + lane < a.rows ? max(__ldg(a.offsets + base + lane + 1), t0) - t0 : kReadTokens;
+    int k = kReadTokens;
+    if (base + lane < a.rows) {
+      const int end = __ldg(a.offsets + base + lane + 1);
+      k = max(end, t0) - t0;
+      if (blockIdx.x == 0) {  // one CTA reports rows that end past the output, or before they begin
+        const int begin = __ldg(a.offsets + base + lane);
+        if (begin < 0 || end < begin || end > a.tokens) atomicOr(a.status, kDevBadIndex);
+      }
+    }
     const unsigned before = __ballot_sync(0xffffffffu, k == 0);
     if (lane == 0 && before) atomicAdd(&ends[0], __popc(before));
     if (k > 0 && k < kReadTokens) atomicAdd(&ends[k], 1);

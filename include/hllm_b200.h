@@ -516,7 +516,8 @@ hllm_b200_status hllm_b200_kv8_write(const hllm_b200_kv8* cache, const void* qkv
  * v_out [tokens][kv_heads][head_dim], gathered through block_tables
  * [rows][max_blocks].  Output rows at or past offsets[rows] are left as they
  * are; a position without a page, or past its row's length, is zeros and sets
- * a status bit. */
+ * a status bit, as do offsets that decrease or pass `tokens` (whose rows are left
+ * out). */
 hllm_b200_status hllm_b200_kv8_read(const hllm_b200_kv8* cache, const int32_t* block_tables,
                                     uint32_t rows, uint32_t max_blocks, const int32_t* first,
                                     const int32_t* lengths, const int32_t* offsets,

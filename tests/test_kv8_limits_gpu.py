@@ -231,3 +231,32 @@ def test_a_single_row_may_have_any_step(torch, kv8):
         assert torch.equal(kv8.attention(cache, q, *args, out=out), want)
         assert torch.equal(out, want)
     cache.check()
+
+
+def test_read_reports_offsets_out_of_range(torch, kv8):
+    """Rows that the output has no room for, or that end before they begin."""
+    rng = np.random.default_rng(2)
+    rows, n = 300, 20
+    cache = random_cache(torch, kv8, rng, 2 * rows, 2, 64)
+    table = ints(torch, tables_for(torch, rng, [2] * rows, 2 * rows))
+    lengths = ints(torch, [n] * rows)
+    good = np.arange(rows + 1) * n
+    T = rows * n
+    k, v = kv8.read(cache, table, lengths, ints(torch, good), T)
+    cache.check()
+    for change, kept in ((lambda c: c[-1:].__iadd__(1), T), (lambda c: c[280:].__iadd__(7), 280 * n),
+                         (lambda c: c[5:6].__isub__(200), 0), (lambda c: c[:1].__isub__(n), 0)):
+        cu = good.copy()
+        change(cu)
+        out = tuple(torch.full_like(k, 7.0) for _ in range(2))
+        kv8.read(cache, table, lengths, ints(torch, cu), T, out=out)
+        with pytest.raises(StageError, match="out of range"):
+            cache.check()
+        assert torch.equal(out[0][:kept], k[:kept]) and torch.equal(out[1][:kept], v[:kept])
+    # A shorter output: the rows that fit are whole.
+    out = tuple(torch.full_like(k, 7.0) for _ in range(2))
+    kv8.read(cache, table, lengths, ints(torch, good), T - 2 * n, out=(out[0][:T - 2 * n], out[1][:T - 2 * n]))
+    with pytest.raises(StageError, match="out of range"):
+        cache.check()
+    assert torch.equal(out[0][:T - 2 * n], k[:T - 2 * n]) and bool((out[0][T - 2 * n:] == 7).all())
+    assert torch.equal(out[1][:T - 2 * n], v[:T - 2 * n]) and bool((out[1][T - 2 * n:] == 7).all())
