@@ -35,6 +35,9 @@ hllm_b200_status cuda_status(cudaError_t e) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 constexpr uint64_t kMaxInt = 0x7fffffff;
+// Keys of a row in attention: its passes count, in 32 bits, up to a few key tiles
+// past the last one.
+constexpr uint64_t kMostKeys = kMaxInt - 4096;
 
 // The first fault of a cache description, or null.
 const char* cache_fault(const hllm_b200_kv8* c) {
@@ -246,7 +249,7 @@ hllm_b200_status hllm_b200_kv8_attention(const hllm_b200_kv8* cache, const uint1
   if (const char* why = cache_fault(cache)) return refuse(why);
   if (const char* why = heads_fault(hq, cache->kv_heads)) return refuse(why);
   if (rows > kMaxInt / 2 || tokens > kMaxInt || max_row_tokens > kMaxInt ||
-      max_blocks > kMaxInt / hb::kKv8Page)
+      max_blocks > kMostKeys / hb::kKv8Page)
     return refuse("8-bit KV attention: rows, tokens or max_blocks out of range");
   if (!std::isfinite(scale)) return refuse("8-bit KV attention: bad scale");
   if (!status) return refuse("8-bit KV attention: null status");

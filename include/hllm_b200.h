@@ -535,7 +535,8 @@ hllm_b200_status hllm_b200_kv8_read(const hllm_b200_kv8* cache, const int32_t* b
  * decode batch); a longer row, or one past `tokens` or max_blocks, is skipped
  * and sets a status bit.  Where cu_seqlens decreases a bit is set, and which of
  * the rows that then overlap are answered is not said.  Keys of a missing page are left out and set one (a token that sees no other
- * gives zeros).  q and out are 16-byte aligned, ld_q and ld_out multiples of 8.
+ * gives zeros).  q and out are 16-byte aligned, ld_q and ld_out multiples of 8;
+ * max_blocks x 16 is at most 2^31 - 4097.
  * `workspace` (16-byte aligned) has at least hllm_b200_kv8_attention_workspace
  * bytes for these or larger counts and the same heads; its contents before and
  * after the call mean nothing. */
