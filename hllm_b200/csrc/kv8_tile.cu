@@ -347,16 +347,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         own = x.chunks;
         len = x.len;
       }
-      const int upto = tiles_upto(own, lane), all = __shfl_sync(0xffffffffu, upto, 31);
-      const int lower = upto - own;  // tiles of rows that stand before this one
-      if (!fits(tiles_before, upto, most)) {
-        if (reports && own) atomicOr(a.status, kDevBadIndex);
-        own = 0;
+      const int all = __reduce_add_sync(0xffffffffu, own);
+      if (!fits(tiles_before, all, most)) {
+        const int upto = tiles_upto(own, lane);  // (of the whole warp)
+        const bool skipped = own > 0 && !fits(tiles_before, upto, most);
+        if (skipped && reports) atomicOr(a.status, kDevBadIndex);
+        if (skipped) own = 0;
       }
-      int first = 0;  // tiles of rows that go before this one
+      int first = 0, lower = 0;  // tiles of rows that go before this one, and that stand before it
       for (int j = 0; j < min(32, a.rows - base); ++j) {
         const int chunks = __shfl_sync(0xffffffffu, own, j), keys = __shfl_sync(0xffffffffu, len, j);
         if (keys > len || (keys == len && j < lane)) first += chunks;
+        if (j < lane) lower += chunks;
       }
       const unsigned hit = __ballot_sync(0xffffffffu, row < 0 && w >= first && w < first + own);
       if (hit) {
