@@ -1,7 +1,7 @@
 """Per-operator timing of the executor's kernels through the C ABI.
 
-    python opbench.py [gemm|attn|prefill|envelope|c5|all] [--ncu-gemm M,K,N,PAIR,EPI]
-                      [--ncu-attn ROWS] [--ncu-prefill FIRST,COUNT]
+    python opbench.py [gemm|attn|prefill|envelope|c5|kv8|all] [--ncu-gemm M,K,N,PAIR,EPI]
+                      [--ncu-attn ROWS] [--ncu-prefill FIRST,COUNT] [--ncu-kv8 CASE]
 
 Times the projection GEMM at the Qwen3-4B shapes (decode width 16/64 tokens,
 prefill width 575 tokens) and the paged decode attention at configuration-5
@@ -12,6 +12,9 @@ runs three launches of one GEMM shape and `--ncu-attn` three of the decode
 attention over ROWS configuration-3-like contexts (for profiler captures).
 `c5` runs configuration 5 (decode attention and GEMVs at batch 1-256, each
 launch after an L2 flush) as a markdown table of HBM GB/s against the roof.
+`kv8` times the 8-bit KV cache on the cases of perf/operators.py and at head
+size 256 and 16 query heads a kv head, calls in a graph and from Python;
+`--ncu-kv8` runs three calls of one of its cases.
 `envelope` times the boundary wire codec (host encode/decode, and the
 envelope built from device memory when a GPU is present).
 Device memory comes from torch; all compute is libhllm_b200.so.
@@ -253,6 +256,62 @@ def steady_decode_contexts(rows=64, seed=3):
     return (prompt + rng.integers(1, 513, rows)).astype(int).tolist()
 
 
+def kv8_cases():
+    """perf/operators.py, set to call the kernels, and its cases and some more."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "perf", "operators.py")
+    spec = importlib.util.spec_from_file_location("operators", path)
+    ops = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ops)
+    ops.own = True
+
+    def chunk(count, past):
+        return dict(chunks=1, count_lo=count, count_hi=count, past_lo=past, past_hi=past)
+
+    more = [ops._attention("d256_decode_64_long", (6, 2, 256), 64, 1024, 16384),
+            ops._attention("d256_prefill_512_at_1024", (6, 2, 256), **chunk(512, 1024)),
+            ops._attention("d256_prefill_2048_at_8192", (6, 2, 256), **chunk(2048, 8192)),
+            ops._attention("d64_decode_64_long", (32, 8, 64), 64, 1024, 16384),
+            ops._attention("group16_decode_64_long", (128, 8, 128), 64, 1024, 16384)]
+    return ops, ops.listed() + more
+
+
+def kv8_suite(calls=18):
+    """Each case: GPU time per call of `calls` in a CUDA graph, on three sets of
+    inputs in turn (median of 7 replays), and time per call from Python."""
+    import time
+    torch = _torch()
+    ops, cases = kv8_cases()
+    for case in cases:
+        states = [ops.prepare(case, seed) for seed in (1, 2, 3)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for s in states:
+                ops.run(s)
+        torch.cuda.synchronize()
+        graph, kept = torch.cuda.CUDAGraph(), []
+        with torch.cuda.graph(graph):
+            for i in range(calls):
+                kept.append(ops.run(states[i % 3]))
+        gpu = sorted(ev_time(graph.replay, iters=1) / calls for _ in range(7))[3]
+        for i in range(30):
+            ops.run(states[i % 3])
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        for i in range(198):
+            ops.run(states[i % 3])
+        torch.cuda.synchronize()
+        python = (time.perf_counter() - t0) / 198 * 1e6
+        work = ops.work(case)
+        print(f"{case['name']:26s} {gpu:8.2f} us  ({work['bytes'] / gpu / 1e3:7.1f} GB/s, "
+              f"{work['flops'] / gpu / 1e6:7.1f} TFLOP/s)  from Python {python:8.2f} us", flush=True)
+        for s in states:
+            s["cache"].check()
+        del states, kept, graph
+
+
 def envelope_suite(tokens=512, width=2560, iters=200):
     """The boundary wire codec at a 512-token Qwen3-4B chunk (2.6 MB of F16):
     host encode and decode through the C ABI (no GPU needed), then, on a GPU,
@@ -317,6 +376,13 @@ def main(argv):
         first, count = (int(x) for x in argv[argv.index("--ncu-prefill") + 1].split(","))
         prefill_case(first, count, iters=3)
         return
+    if "--ncu-kv8" in argv:
+        name = argv[argv.index("--ncu-kv8") + 1]
+        ops, cases = kv8_cases()
+        for seed in (1, 2, 3):
+            ops.run(ops.prepare(next(c for c in cases if c["name"] == name), seed))
+        _torch().cuda.synchronize()
+        return
     if "--ncu-attn" in argv:
         rows = int(argv[argv.index("--ncu-attn") + 1])
         attn_case(steady_decode_contexts(rows), iters=3)
@@ -336,6 +402,8 @@ def main(argv):
         envelope_suite()
     if what == "c5":
         c5_sweep()
+    if what == "kv8":
+        kv8_suite()
 
 
 if __name__ == "__main__":

@@ -24,6 +24,11 @@ def kv8(torch):
     return kv8
 
 
+def normal(torch, shape, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(shape, device="cuda", generator=g)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("turns", [2, 5, 40])
 def test_decreasing_offsets_stay_inside_the_workspace(torch, kv8, d, turns):
@@ -38,7 +43,7 @@ def test_decreasing_offsets_stay_inside_the_workspace(torch, kv8, d, turns):
     cu = ints(torch, [0, T] * turns)
     lengths = ints(torch, np.linspace(T, n, rows).astype(np.int32))  # the last rows' tiles are taken first
     tables = ints(torch, np.repeat(table, rows, 0))
-    q = torch.randn((T, hq * d), device="cuda").half()
+    q = normal(torch, (T, hq * d), turns).half()
     need = kv8.attention_workspace(rows, T, T, hq, hkv, d).numel()
     buffer = torch.full((need + (64 << 20),), 0xa5, dtype=torch.uint8, device="cuda")
     out = torch.full((T + 1, hq * d), 9.0, dtype=torch.float16, device="cuda")
@@ -63,7 +68,7 @@ def check_nan(torch, kv8, heads, n, count, keys, most=None):
     pages = (n + 15) // 16
     cache = random_cache(torch, kv8, rng, pages + 3, hkv, d)
     table = tables_for(torch, rng, [pages], pages + 3)
-    q = torch.randn((count, hq * d), device="cuda").half()
+    q = normal(torch, (count, hq * d), n).half()
     args = (ints(torch, [0, count]), ints(torch, [n]), ints(torch, table))
     clean = kv8.attention(cache, q, *args, max_tokens=most or count).view(count, hq, d)
     assert not bool(clean.isnan().any())
@@ -105,6 +110,13 @@ def test_nan_in_the_middle_of_prompt_chunks(torch, kv8, heads, past, count):
     n = past + count
     keys = {0, 35, past, past + 1, past + count // 2, past + 63, past + 127, n - 2, n - 1}
     check_nan(torch, kv8, heads, n, count, sorted(k for k in keys if k < n))
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 2, 64), (6, 2, 256)])
+@pytest.mark.parametrize("n,count", [(3, 6), (20, 90), (40, 300)])
+def test_nan_where_early_tokens_have_no_key(torch, kv8, heads, n, count):
+    """More new tokens than keys: the first see none, and give zeros."""
+    check_nan(torch, kv8, heads, n, count, (0, 1, n - 1))
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -160,7 +172,7 @@ def test_large_keys_coarsen_no_others(torch, kv8, heads, past, count, octaves):
         kc[at] = 0
         kc[at[0], :, at[2], 0] = 0xc0  # -2
         ks[at] = min(122 + octaves, 127 + 39)
-    q = (1.5 * torch.randn((count, hq, d), device="cuda")).half()
+    q = (1.5 * normal(torch, (count, hq, d), octaves)).half()
     q[..., 0] = 16.0
     got = kv8.attention(cache, q.view(count, hq * d), ints(torch, [0, count]), ints(torch, [n]),
                         ints(torch, table)).view(count, hq, d).double()
@@ -220,7 +232,7 @@ def test_a_single_row_may_have_any_step(torch, kv8):
     rng = np.random.default_rng(1)
     cache = random_cache(torch, kv8, rng, 6, hkv, d)
     args = (ints(torch, [0, 1]), ints(torch, [40]), ints(torch, tables_for(torch, rng, [3], 6)))
-    q = torch.randn((1, hq * d), device="cuda").half()
+    q = normal(torch, (1, hq * d), 1).half()
     want = kv8.attention(cache, q, *args)
     column = q.t().contiguous()
     odd = torch.empty((2, hq * d + 5), dtype=torch.float16, device="cuda")
