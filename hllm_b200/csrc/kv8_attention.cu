@@ -144,7 +144,8 @@ struct Shape : Layout<D> {
   using Layout<D>::VW;
   static constexpr int kCols = 8 * NT;
   // Enough warps to hide the latency of one unit's chain of products, and
-  // enough bytes in flight to hide that of memory (192 KB an SM at D = 128).
+  // enough bytes in flight to hide that of memory (at D = 128 two units of 8 KB a
+  // warp beside the one in use, 128 KB an SM).
   // Pages of a unit, which share its waits and copies, and of them at a time in
   // registers.  64 long rows: D = 64, 8 columns 100 us at two pages a unit, 87 at
   // four; 16 columns, D = 64 173 at one, 135 at two; D = 128 215 and 186.

@@ -69,7 +69,7 @@ struct Eight<float> {
 // kept and put back to first order: cos(a + r) = cos a - r sin a.
 constexpr int kWriteThreads = 128;
 constexpr int kWriteWarps = kWriteThreads / 32;
-// Warps that a call should have (three rounds of full SMs): below it a token's
+// Warps that a call should have (three rounds of a B200's 148 SMs at 24 warps): below it a token's
 // heads are spread over several warps, each with the token's cosines to
 // compute.  8192 tokens of 32 + 8 + 8 heads of 128 in F16: 40.5 us (4.6 TB/s) so,
 // 48 at one round; the cosines in registers (80 of them a thread) 45, the loads

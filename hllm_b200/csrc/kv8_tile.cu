@@ -35,9 +35,9 @@
 // where E' is taken out: the weights are then the exponentials themselves.)
 // Every wait is bounded (common.cuh).
 //
-// Measured, 32 heads on 8 of 128: 2048 tokens behind 8192 keys 366 us (845
+// Measured, 32 heads on 8 of 128: 2048 tokens behind 8192 keys 369 us (838
 // TFLOP/s of the causal products, 50 % of what cuBLAS reaches), 512 behind 1024
-// 28.5 us (377).  A step with two query tiles is 4.7k cycles, of which the products
+// 29.7 us (362).  A step with two query tiles is 4.7k cycles, of which the products
 // are 2.8k: the rest is a group's chain, scores, maximum and exponentials (3.0k),
 // products, next scores, for which TMEM has no second buffer beside two results of
 // 128 dimensions.  With one query tile a step is 2.5k, and the codes' conversion
@@ -106,7 +106,8 @@ __device__ __forceinline__ void mma_commit(bool on, uint64_t* bar) {
 // 2^y of two numbers on the FMA pipes, beside the exponentials of the special
 // function unit, which bounds a softmax: y = n + r with n the nearest integer
 // (found in the low bits of y + 1.5 2^23), 2^r by a polynomial of degree 5 fitted
-// to the least largest relative error on [-1/2, 1/2] (Remez; 7.5e-8), times 2^n.
+// to a small largest relative error on [-1/2, 1/2] (Remez, then rounded: 1.6e-7 with
+// these coefficients, 2.2e-7 in F32 arithmetic), times 2^n.
 // Numbers below -120 count as that; NaN stays NaN.
 __device__ __forceinline__ float2 exp2_fma(float2 y) {
   float2 t;

@@ -128,7 +128,8 @@ class Cache:
         self._ref = C.byref(self._c)
 
     def check(self) -> None:
-        """Waits for the device word, clears it, and raises what it reports."""
+        """Waits for the device word on the current stream, clears it, and raises
+        what it reports of the calls that this stream has waited for."""
         bits = int(self.status.item())
         if bits:
             self.status.zero_()

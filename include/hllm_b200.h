@@ -496,7 +496,8 @@ hllm_b200_status hllm_b200_rope_turns(const hllm_b200_rope* rope, double* turns,
 
 /* hllm_b200_qkv_post for the 8-bit cache and any rotary form: per token and
  * head of qkv [tokens][(Hq + 2 Hkv) d] (`dtype` F32, F16 or BF16), q and k
- * RMSNorm where q_norm / k_norm (F32 [d]) are given, rotation at positions[t]
+ * RMSNorm where q_norm / k_norm (F32 [d]) are given (squares summed in F32: values
+ * past about 10^18 leave its range), rotation at positions[t]
  * (angles reduced in 64 bits; turns [rotary_dim / 2] F64 and factor from
  * hllm_b200_rope_turns, turns on the device), q to q_out F16 [tokens][Hq d],
  * K and V quantised into slots[t].  A token with slot -1 is not stored.  The
